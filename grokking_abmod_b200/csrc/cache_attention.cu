@@ -1,0 +1,609 @@
+// Attention of new rows over the 8-bit paged cache.
+//
+// For row i of sequence b (n new rows, L tokens in the cache with them) and
+// query head a of key head h = a / G, over the positions j that the row sees,
+// first_b <= j <= L - n + i:
+//
+//   s_j = scale q . k_j,   p_j = e^(s_j - m),   o = sum_j p_j v_j / sum_j p_j
+//
+// A row that sees nothing gives 0, and -inf as its log-sum-exp.
+//
+// Codes are small integers, exact in FP16, so the products run on FP16
+// tensor-core instructions with FP32 accumulation and the scales of K and V,
+// powers of two, multiply scores and probabilities without rounding.  q and p
+// enter as FP16 pairs hi + lo (22 bits) after an exact scaling by a power of
+// two: q by its row's largest magnitude, p times 2^14, which keeps the
+// smallest kept part 2^-39 of the row's largest probability.
+//
+// The split kernel serves rows that share a key head and are few: 8 at a
+// time, one tile of 32 tokens after the other, bound by the bytes of the
+// cache.  The 8 rows' hi parts are rows 0-7 and their lo parts rows 8-15 of
+// the 16-row operand, so the second term costs nothing.  Every warp runs its
+// own ring of bulk copies and its own running softmax (no barrier between
+// warps until the end); the four warps' results, and the chunks that a long
+// sequence is cut into, are joined by their maxima in a fixed order.
+
+#include <algorithm>
+#include <cmath>
+
+#include "cache_host.h"
+#include "common.cuh"
+#include "dtype.cuh"
+#include "tc05.cuh"
+
+namespace mb {
+namespace cache {
+
+constexpr unsigned kFull = 0xFFFFFFFFu;
+constexpr int kTile = 32;        // tokens a warp takes at a time
+constexpr int kSplitWarps = 4;
+constexpr int kSplitThreads = kSplitWarps * 32;
+constexpr int kSplitRows = 8;    // query rows of a unit
+constexpr int kSplitStages = 3;  // tiles a warp has in flight
+
+struct Queries {
+  const void* q;
+  size_t row_stride, head_stride;
+  void* out;   // [rows][q_heads][head_dim]
+  float* lse;  // [q_heads][rows] base 2, or null
+  int heads, group, head_dim;
+  float scale_log2;  // softmax scale times log2 e
+  const int32_t* first;
+  int max_new;
+  int* status;
+};
+
+// Partial results of the chunks: [unit][chunk][row] log-sum-exp and
+// [unit][chunk][row][width] normalised outputs.
+struct Partials {
+  float* lse;
+  float* o;
+  int chunks;       // per unit
+  int chunk_tiles;  // tiles of a chunk; the last one takes what is left
+};
+
+template <int D>
+struct SplitSmem {
+  static constexpr int kTileBytes = kTile * D;
+  static constexpr int kWarpBytes = kSplitStages * 2 * kTileBytes;
+  static constexpr int kBars = kSplitWarps * kWarpBytes;
+  static constexpr int kMeta = kBars + kSplitWarps * kSplitStages * 8;          // scales of each stage
+  static constexpr int kJoin = kMeta + kSplitWarps * kSplitStages * 16;         // m, l, exponent per warp and row
+  static constexpr int kBytes = kJoin + kSplitWarps * kSplitRows * 12 + 16;
+};
+
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+      "%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Two codes u = c + 128 (bytes of `biased` picked by `select`) as FP16: the
+// byte under the exponent of 1024 is 1024 + u, and 1152 comes off exactly.
+__device__ __forceinline__ uint32_t codes_to_f16(uint32_t biased, uint32_t select) {
+  const uint32_t w = __byte_perm(biased, 0x64646464u, select);
+  const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&w), __half2half2(__ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int WORDS>
+__device__ __forceinline__ void load_words(const int8_t* p, uint32_t (&w)[WORDS]) {
+  if constexpr (WORDS % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < WORDS; i += 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p + 4 * i);
+      w[i] = v.x;
+      w[i + 1] = v.y;
+      w[i + 2] = v.z;
+      w[i + 3] = v.w;
+    }
+  } else if constexpr (WORDS % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < WORDS; i += 2) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p + 4 * i);
+      w[i] = v.x;
+      w[i + 1] = v.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) w[i] = *reinterpret_cast<const uint32_t*>(p + 4 * i);
+  }
+}
+
+__device__ __forceinline__ int exponent_of(float power) { return (int)(__float_as_uint(power) >> 23) - 127; }
+
+__device__ __forceinline__ float quad_max(float v) {
+  v = fmaxf(v, __shfl_xor_sync(kFull, v, 1));
+  return fmaxf(v, __shfl_xor_sync(kFull, v, 2));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  v += __shfl_xor_sync(kFull, v, 1);
+  return v + __shfl_xor_sync(kFull, v, 2);
+}
+
+// What a unit (sequence, 8 rows, key head) covers.
+struct Unit {
+  int b, row0, rows;     // rows of the group's row list: row r is token r / G, head r % G
+  int length, fresh;
+  size_t first_row;
+  int lo;                // first visible position
+  int hi;                // one past the last that any of its rows sees
+  bool bad;
+};
+
+template <int ROWS>
+__device__ __forceinline__ Unit unit_of(const View& c, const Batch& t, const Queries& q, int z, int blocks_per_seq) {
+  Unit u;
+  u.b = z / blocks_per_seq;
+  u.row0 = (z % blocks_per_seq) * ROWS;
+  const Span s = span_of(t, c, u.b);
+  u.length = s.length;
+  u.fresh = s.fresh;
+  u.first_row = s.row;
+  u.rows = (int)min((long long)ROWS, (long long)s.fresh * q.group - u.row0);
+  u.bad = s.flags != 0;
+  const int old = s.length - s.fresh;
+  u.lo = q.first ? max(0, q.first[u.b]) : 0;
+  u.hi = u.rows > 0 ? old + (u.row0 + u.rows - 1) / q.group + 1 : 0;
+  return u;
+}
+
+// Rows past the announced number are not visited: the last block of a
+// sequence gives them NaN; a sequence whose numbers do not fit, all its rows.
+template <class T>
+__device__ __forceinline__ void refuse_rows(const Batch& t, const Queries& q, int head, const Unit& u, int from_row,
+                                            int threads) {
+  const size_t count = (size_t)u.fresh * q.group;
+  for (size_t r = from_row; r < count; ++r) {
+    const size_t row = u.first_row + r / q.group;
+    const int a = head * q.group + (int)(r % q.group);
+    T* out = static_cast<T*>(q.out) + (row * q.heads + a) * q.head_dim;
+    for (int ch = threadIdx.x; ch < q.head_dim; ch += threads) out[ch] = Element<T>::from(NAN);
+    if (threadIdx.x == 0 && q.lse) q.lse[(size_t)a * t.rows + row] = NAN;
+  }
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(kSplitThreads)
+    attend_split(View c, Batch t, Queries q, Partials part, int blocks_per_seq) {
+  using S = SplitSmem<D>;
+  constexpr int KW = D / 16;  // words of a K row that a thread reads: one K step of 16 channels each
+  constexpr int VW = D / 32;  // words of a V row
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, tq = lane & 3;
+  const int chunk = blockIdx.x % part.chunks, head = blockIdx.y, z = blockIdx.x / part.chunks;
+  const Unit u = unit_of<kSplitRows>(c, t, q, z, blocks_per_seq);
+  const bool last_block = z % blocks_per_seq == blocks_per_seq - 1;
+
+  if (u.bad) {
+    if (chunk == 0 && z % blocks_per_seq == 0) {
+      refuse_rows<T>(t, q, head, u, 0, kSplitThreads);
+      if (q.status && threadIdx.x == 0) atomicOr(q.status, span_of(t, c, u.b).flags);
+    }
+  } else if (last_block && chunk == 0 && (long long)u.fresh * q.group > u.row0 + kSplitRows) {
+    refuse_rows<T>(t, q, head, u, u.row0 + kSplitRows, kSplitThreads);
+    if (q.status && threadIdx.x == 0) atomicOr(q.status, kBadRows);
+  }
+  if (u.bad || u.rows <= 0) return;
+
+  const int tile_lo = u.lo / kTile, tile_hi = u.hi > u.lo ? (u.hi + kTile - 1) / kTile : tile_lo;
+  const int begin = (int)min((long long)tile_hi, tile_lo + (long long)chunk * part.chunk_tiles);
+  const int end = chunk == part.chunks - 1 ? tile_hi : min(tile_hi, begin + part.chunk_tiles);
+  const size_t slot = ((size_t)z * c.heads + head) * part.chunks + chunk;
+  if (begin >= end && part.chunks > 1) {
+    if (threadIdx.x < kSplitRows) part.lse[slot * kSplitRows + threadIdx.x] = -INFINITY;
+    return;
+  }
+
+  int8_t* ring = reinterpret_cast<int8_t*>(smem) + warp * S::kWarpBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars) + warp * kSplitStages;
+  float4* meta = reinterpret_cast<float4*>(smem + S::kMeta) + warp * kSplitStages;
+  float* join = reinterpret_cast<float*>(smem + S::kJoin);
+  int* gave_up = reinterpret_cast<int*>(smem + S::kJoin + kSplitWarps * kSplitRows * 12);
+  if (lane == 0)
+    for (int s = 0; s < kSplitStages; ++s) tc::bar_init(&bars[s], 1);
+  tc::bar_init_fence();
+  if (threadIdx.x == 0) *gave_up = 0;
+  __syncthreads();
+
+  const int mine = end > begin + warp ? (end - begin - warp + kSplitWarps - 1) / kSplitWarps : 0;  // this warp's tiles
+  const bool two = c.tokens == kTile / 2;  // a tile spans two pages
+
+  // page numbers and scales of 32 tiles, one a lane
+  int page0 = -1, page1 = -1;
+  float ks0 = 0.f, ks1 = 0.f, vs0 = 0.f, vs1 = 0.f;
+  auto look_up = [&](int n) {
+    page0 = page1 = -1;
+    ks0 = ks1 = vs0 = vs1 = 0.f;
+    if (n + lane >= mine) return;
+    const int pos = (begin + warp + (n + lane) * kSplitWarps) * kTile;
+    // scales of pages that no row sees stay 0: theirs may be anything
+    bool bad = false;
+    if (!two || pos + kTile / 2 > u.lo) {
+      page0 = page_of(t, c, u.b, pos >> c.shift);
+      bad = page0 < 0;
+      ks0 = bad ? NAN : __ldg(c.k_scale + c.scale_at(page0, head));
+      vs0 = bad ? NAN : __ldg(c.v_scale + c.scale_at(page0, head));
+    }
+    if (!two) {
+      ks1 = ks0;
+      vs1 = vs0;
+    } else if (pos + kTile / 2 < u.hi) {
+      page1 = page_of(t, c, u.b, (pos >> c.shift) + 1);
+      ks1 = page1 < 0 ? NAN : __ldg(c.k_scale + c.scale_at(page1, head));
+      vs1 = page1 < 0 ? NAN : __ldg(c.v_scale + c.scale_at(page1, head));
+      bad = bad || page1 < 0;
+    }
+    if (bad && q.status) atomicOr(q.status, kBadPage);
+  };
+  auto issue = [&](int n) {
+    const int s = n % kSplitStages, from = n & 31;
+    const int p0 = __shfl_sync(kFull, page0, from), p1 = __shfl_sync(kFull, page1, from);
+    const float4 m = make_float4(__shfl_sync(kFull, ks0, from), __shfl_sync(kFull, ks1, from),
+                                 __shfl_sync(kFull, vs0, from), __shfl_sync(kFull, vs1, from));
+    if (lane == 0) {
+      meta[s] = m;
+      int8_t* k_at = ring + s * 2 * S::kTileBytes;
+      int8_t* v_at = k_at + S::kTileBytes;
+      const int inside = ((begin + warp + n * kSplitWarps) * kTile) & (c.tokens - 1);
+      const uint32_t bytes = two ? S::kTileBytes / 2 : S::kTileBytes;
+      tc::bar_expect_tx(&bars[s], 2 * bytes * ((p0 >= 0) + (p1 >= 0)));
+      if (p0 >= 0) {
+        tc::bulk_g2s(k_at, c.k + c.row(p0, head, inside), bytes, &bars[s]);
+        tc::bulk_g2s(v_at, c.v + c.row(p0, head, inside), bytes, &bars[s]);
+      }
+      if (p1 >= 0) {
+        tc::bulk_g2s(k_at + bytes, c.k + c.row(p1, head, 0), bytes, &bars[s]);
+        tc::bulk_g2s(v_at + bytes, c.v + c.row(p1, head, 0), bytes, &bars[s]);
+      }
+    }
+  };
+
+  look_up(0);
+  int issued = 0;
+  for (; issued < kSplitStages - 1 && issued < mine; ++issued) issue(issued);
+
+  // This lane's query row (g): hi parts as operand row g, lo parts as g + 8.
+  uint32_t qh[KW][2], ql[KW][2];
+  float row_factor;
+  int limit;  // last position the row sees
+  {
+    const int r = u.row0 + g;
+    const bool there = g < u.rows;
+    const int tok = r / q.group, a = head * q.group + r % q.group;
+    limit = there ? u.length - u.fresh + tok : -1;
+    const T* src = static_cast<const T*>(q.q) + (u.first_row + tok) * q.row_stride + (size_t)a * q.head_stride;
+    float x[KW][4];
+    float most = 0.f;
+#pragma unroll
+    for (int w = 0; w < KW; ++w)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int ch = tq * (D / 4) + 4 * w + e;
+        x[w][e] = there && ch < q.head_dim ? Element<T>::to(src[ch]) : 0.f;
+        most = fmaxf(most, fabsf(x[w][e]));
+      }
+    const float up = tc::f16_scale(quad_max(most));
+#pragma unroll
+    for (int w = 0; w < KW; ++w)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) tc::split_f16x2(x[w][2 * e] * up, x[w][2 * e + 1] * up, qh[w][e], ql[w][e]);
+    row_factor = q.scale_log2 / up;
+  }
+  const int sure = u.length - u.fresh + u.row0 / q.group;  // the last position that every row sees
+
+  float o[D / 8][4];
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  int ev = -126;  // o carries 2^(14 - ev)
+
+  for (int n = 0; n < mine; ++n) {
+    if (issued < mine) {
+      if ((issued & 31) == 0) look_up(issued);
+      issue(issued++);
+    }
+    const int s = n % kSplitStages;
+    if (!__all_sync(kFull, tc::bar_wait(&bars[s], (n / kSplitStages) & 1))) {
+      *gave_up = 1;
+      // the copies behind it may still land: none is left when the CTA ends
+      for (int k = n + 1; k < issued; ++k) tc::bar_wait(&bars[k % kSplitStages], (k / kSplitStages) & 1);
+      break;
+    }
+    const float4 sc = meta[s];
+    const int8_t* kt = ring + s * 2 * S::kTileBytes;
+    const int8_t* vt = kt + S::kTileBytes;
+    const int pos = (begin + warp + n * kSplitWarps) * kTile;
+
+    float x[4][2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t w[KW];
+      load_words<KW>(kt + (8 * j + g) * D + tq * (D / 4), w);
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KW; ++k) {
+        const uint32_t biased = w[k] ^ 0x80808080u;
+        mma16816(acc, qh[k][0], ql[k][0], qh[k][1], ql[k][1], codes_to_f16(biased, 0x4140),
+                 codes_to_f16(biased, 0x4342));
+      }
+      const float f = (j < 2 ? sc.x : sc.y) * row_factor;
+      x[j][0] = (acc[0] + acc[2]) * f;
+      x[j][1] = (acc[1] + acc[3]) * f;
+    }
+    if (pos < u.lo || pos + kTile - 1 > sure) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int at = pos + 8 * j + 2 * tq + e;
+          if (at < u.lo || at > limit) x[j][e] = -INFINITY;
+        }
+    }
+    float mx = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1])),
+                     fmaxf(fmaxf(x[2][0], x[2][1]), fmaxf(x[3][0], x[3][1])));
+    mx = fmaxf(m, quad_max(mx));
+    const float base = mx == -INFINITY ? 0.f : mx;
+    const float shrink = ex2_ftz(m - base);
+    m = mx;
+    // V's exponent: o is kept relative to the largest V scale so far
+    int top = ev;
+    if (sc.z == sc.z) top = max(top, exponent_of(sc.z));
+    if (sc.w == sc.w) top = max(top, exponent_of(sc.w));
+    float change = shrink;
+    if (top != ev) change *= power_of_two(max(ev - top, -126));
+    ev = top;
+    l *= shrink;
+    if (__any_sync(kFull, change != 1.0f)) {
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][e] *= change;
+    }
+    const float unit = power_of_two(-ev);
+    const float f0 = sc.z * unit * 16384.f, f1 = sc.w * unit * 16384.f;
+    uint32_t ph[4], pl[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float p0 = ex2_ftz(x[j][0] - base), p1 = ex2_ftz(x[j][1] - base);
+      l += p0 + p1;
+      const float f = j < 2 ? f0 : f1;
+      tc::split_f16x2(p0 * f, p1 * f, ph[j], pl[j]);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      uint32_t v0[VW], v1[VW], v2[VW], v3[VW];
+      const int8_t* vr = vt + (16 * k + 2 * tq) * D + g * (D / 8);
+      load_words<VW>(vr, v0);
+      load_words<VW>(vr + D, v1);
+      load_words<VW>(vr + 8 * D, v2);
+      load_words<VW>(vr + 9 * D, v3);
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+        const uint32_t a = v0[w] ^ 0x80808080u, b = v1[w] ^ 0x80808080u;
+        const uint32_t d = v2[w] ^ 0x80808080u, e = v3[w] ^ 0x80808080u;
+        // bytes of the two rows side by side: channels 0, 1 and 2, 3
+        const uint32_t ab0 = __byte_perm(a, b, 0x5140), ab1 = __byte_perm(a, b, 0x7362);
+        const uint32_t de0 = __byte_perm(d, e, 0x5140), de1 = __byte_perm(d, e, 0x7362);
+        mma16816(o[4 * w + 0], ph[2 * k], pl[2 * k], ph[2 * k + 1], pl[2 * k + 1], codes_to_f16(ab0, 0x4140),
+                 codes_to_f16(de0, 0x4140));
+        mma16816(o[4 * w + 1], ph[2 * k], pl[2 * k], ph[2 * k + 1], pl[2 * k + 1], codes_to_f16(ab0, 0x4342),
+                 codes_to_f16(de0, 0x4342));
+        mma16816(o[4 * w + 2], ph[2 * k], pl[2 * k], ph[2 * k + 1], pl[2 * k + 1], codes_to_f16(ab1, 0x4140),
+                 codes_to_f16(de1, 0x4140));
+        mma16816(o[4 * w + 3], ph[2 * k], pl[2 * k], ph[2 * k + 1], pl[2 * k + 1], codes_to_f16(ab1, 0x4342),
+                 codes_to_f16(de1, 0x4342));
+      }
+    }
+    __syncwarp();  // the stage is read: its next copy may be issued
+  }
+
+  // The four warps' results side by side; every copy issued has landed.
+  l = quad_sum(l);
+  if (tq == 0) {
+    float* w = join + (warp * kSplitRows + g) * 3;
+    w[0] = m;
+    w[1] = l;
+    w[2] = power_of_two(ev);
+  }
+  __syncwarp();
+  float* mine_o = reinterpret_cast<float*>(ring);  // [8][D]
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) {
+    // n-tile i, column n is channel n D/8 + i
+    mine_o[g * D + (2 * tq) * (D / 8) + i] = o[i][0] + o[i][2];
+    mine_o[g * D + (2 * tq + 1) * (D / 8) + i] = o[i][1] + o[i][3];
+  }
+  __syncthreads();
+  const bool failed = *gave_up != 0;
+  if (failed && threadIdx.x == 0 && q.status) atomicOr(q.status, kGaveUp);
+  for (int e = threadIdx.x; e < u.rows * D; e += kSplitThreads) {
+    const int r = e / D, ch = e % D;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kSplitWarps; ++w) top = fmaxf(top, join[(w * kSplitRows + r) * 3]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, value = 0.f;
+#pragma unroll
+    for (int w = 0; w < kSplitWarps; ++w) {
+      const float* jw = join + (w * kSplitRows + r) * 3;
+      const float f = ex2_ftz(jw[0] - base);
+      const float ow = reinterpret_cast<const float*>(smem + w * S::kWarpBytes)[e];
+      sum = fmaf(jw[1], f, sum);
+      value = fmaf(ow * (1.0f / 16384.f) * jw[2], f, value);
+    }
+    float lse = sum == 0.f ? -INFINITY : base + log2f(sum);
+    value = sum == 0.f ? 0.f : value / sum;
+    if (failed) lse = value = NAN;
+    if (part.chunks > 1) {
+      part.o[(slot * kSplitRows + r) * D + ch] = value;
+      if (ch == 0) part.lse[slot * kSplitRows + r] = lse;
+    } else {
+      const int row = u.row0 + r;
+      const size_t at = u.first_row + row / q.group;
+      const int a = head * q.group + row % q.group;
+      if (ch < q.head_dim) static_cast<T*>(q.out)[(at * q.heads + a) * q.head_dim + ch] = Element<T>::from(value);
+      if (ch == 0 && q.lse) q.lse[(size_t)a * t.rows + at] = lse;
+    }
+  }
+}
+
+// Joins the chunks of a unit's rows: one warp a row.
+template <class T, int D, int ROWS>
+__global__ void __launch_bounds__(256)
+    join_chunks(View c, Batch t, Queries q, Partials part, int blocks_per_seq) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const int head = blockIdx.y, z = blockIdx.x;
+  const int r = blockIdx.z * 8 + (threadIdx.x >> 5);
+  const Unit u = unit_of<ROWS>(c, t, q, z, blocks_per_seq);
+  if (u.bad || r >= u.rows) return;
+  const size_t slot = ((size_t)z * c.heads + head) * part.chunks;
+  float top = -INFINITY;
+  for (int i = lane; i < part.chunks; i += 32) top = fmaxf(top, part.lse[(slot + i) * ROWS + r]);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+  const float base = top == -INFINITY ? 0.f : top;
+  float sum = 0.f, value[D / 32];
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k) value[k] = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < part.chunks; ++i) {
+    const float x = part.lse[(slot + i) * ROWS + r];
+    if (x == -INFINITY) continue;  // saw nothing: its outputs were not written
+    const float f = ex2_ftz(x - base);
+    sum += f;
+    const float* po = part.o + ((slot + i) * ROWS + r) * D;
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) value[k] = fmaf(f, po[lane + 32 * k], value[k]);
+  }
+  const int row = u.row0 + r;
+  const size_t at = u.first_row + row / q.group;
+  const int a = head * q.group + row % q.group;
+  T* out = static_cast<T*>(q.out) + (at * q.heads + a) * q.head_dim;
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k)
+    if (lane + 32 * k < q.head_dim) out[lane + 32 * k] = Element<T>::from(sum == 0.f ? 0.f : value[k] / sum);
+  if (lane == 0 && q.lse) q.lse[(size_t)a * t.rows + at] = sum == 0.f ? -INFINITY : base + log2f(sum);
+}
+
+// ---------------------------------------------------------------- host side
+inline int sm_count() {
+  int dev = 0, sms = 1;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    throw Error(MB_ERR_CUDA, "no CUDA device");
+  return sms;
+}
+
+struct Plan {
+  int blocks_per_seq;  // row blocks of a sequence
+  size_t units;        // sequences times row blocks
+  int chunks, chunk_tiles;
+  size_t workspace;    // bytes
+};
+
+inline Plan make_plan(size_t batch, uint32_t kv_heads, uint32_t group, uint32_t width, uint32_t max_new,
+                      uint32_t max_tokens) {
+  Plan p;
+  const size_t rows = (size_t)max_new * group;
+  require(rows <= (1u << 30), "too many new rows for one call");
+  p.blocks_per_seq = (int)((rows + kSplitRows - 1) / kSplitRows);
+  p.units = batch * p.blocks_per_seq;
+  // Chunks for about three CTAs on every SM, none shorter than two tiles a warp.
+  const size_t want = (size_t)sm_count() * 3, have = std::max<size_t>(1, p.units * kv_heads);
+  const size_t tiles = std::max<size_t>(1, ((size_t)max_tokens + kTile - 1) / kTile);
+  const size_t most = (tiles + 2 * kSplitWarps - 1) / (2 * kSplitWarps);
+  const size_t chunks = std::max<size_t>(1, std::min(most, want / have));
+  p.chunk_tiles = (int)((tiles + chunks - 1) / chunks + kSplitWarps - 1) / kSplitWarps * kSplitWarps;
+  p.chunks = (int)((tiles + p.chunk_tiles - 1) / p.chunk_tiles);
+  p.workspace = p.chunks > 1 ? p.units * kv_heads * p.chunks * kSplitRows * (width + 1) * sizeof(float) : 0;
+  return p;
+}
+
+template <class T, int D>
+void launch_split(const View& c, const Batch& t, const Queries& q, const Plan& p, void* workspace, cudaStream_t st) {
+  const size_t slots = p.units * c.heads * p.chunks;
+  const Partials part{static_cast<float*>(workspace), static_cast<float*>(workspace) + slots * kSplitRows, p.chunks,
+                      p.chunk_tiles};
+  constexpr int bytes = SplitSmem<D>::kBytes;
+  auto kernel = attend_split<T, D>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  require(e == cudaSuccess, std::string("cache attention: ") + cudaGetErrorString(e), MB_ERR_CUDA);
+  kernel<<<dim3((unsigned)(p.units * p.chunks), (unsigned)c.heads), kSplitThreads, bytes, st>>>(
+      c, t, q, part, p.blocks_per_seq);
+  launched("cache attention");
+  if (p.chunks == 1) return;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)p.units, (unsigned)c.heads);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, join_chunks<T, D, kSplitRows>, c, t, q, part, p.blocks_per_seq);
+  require(e == cudaSuccess, std::string("cache attention join: ") + cudaGetErrorString(e), MB_ERR_CUDA);
+}
+
+}  // namespace cache
+}  // namespace mb
+
+extern "C" {
+
+int mb_op_cache_attention_workspace(uint32_t batch, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,
+                                    uint32_t max_new, uint32_t max_tokens, size_t* bytes) {
+  using namespace mb::cache;
+  return mb::guarded([&] {
+    mb::need(bytes, "bytes");
+    mb::require(kv_heads >= 1 && q_heads >= 1 && q_heads % kv_heads == 0, "kv_heads must divide q_heads");
+    *bytes = make_plan(batch, kv_heads, q_heads / kv_heads, (head_dim + 31) / 32 * 32, max_new, max_tokens).workspace;
+  });
+}
+
+int mb_op_cache_attention(const mb_kv_cache* cache, const mb_cache_rows* where, const int32_t* first, const void* q,
+                          size_t q_row_stride, size_t q_head_stride, uint32_t q_heads, uint32_t head_dim,
+                          uint32_t dtype, float scale, uint32_t max_new, uint32_t max_tokens, void* out, float* lse,
+                          void* workspace, size_t workspace_bytes, int* d_status, void* stream) {
+  using namespace mb::cache;
+  return mb::guarded([&] {
+    const View c = view_of(cache, head_dim);
+    const Batch t = batch_of(where, max_new);
+    mb::require(q_heads >= 1 && q_heads % c.heads == 0 && q_heads / c.heads <= 1024,
+                "the cache's heads must divide q_heads");
+    mb::require(std::isfinite(scale), "scale must be finite");
+    mb::require(max_tokens <= (uint32_t)INT_MAX, "max_tokens must be below 2^31");
+    if (t.rows == 0 || t.count == 0) return;
+    mb::require(max_new >= 1, "max_new must be positive where there are rows");
+    mb::need(q, "q");
+    mb::need(out, "out");
+    const Queries qs{q, q_row_stride, q_head_stride, out, lse, (int)q_heads, (int)(q_heads / c.heads), (int)head_dim,
+                     scale * mb::kLog2e, first, (int)max_new, d_status};
+    const Plan p = make_plan(t.count, c.heads, qs.group, c.width, max_new, max_tokens);
+    mb::require(p.units * p.chunks <= (size_t)INT_MAX, "too many row blocks for one call");
+    mb::require(p.workspace == 0 || (workspace != nullptr && workspace_bytes >= p.workspace &&
+                                     reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
+                "workspace missing, too small or not 16-byte aligned");
+    cudaStream_t st = (cudaStream_t)stream;
+    mb::with_dtype(dtype, [&](auto tag) {
+      using T = typename decltype(tag)::type;
+      for (const void* x : {q, (const void*)out})
+        mb::require(reinterpret_cast<uintptr_t>(x) % sizeof(T) == 0, "q and out must be aligned to their elements");
+      switch (c.width) {
+        case 32: return launch_split<T, 32>(c, t, qs, p, workspace, st);
+        case 64: return launch_split<T, 64>(c, t, qs, p, workspace, st);
+        case 96: return launch_split<T, 96>(c, t, qs, p, workspace, st);
+        default: return launch_split<T, 128>(c, t, qs, p, workspace, st);
+      }
+    });
+  });
+}
+
+}  // extern "C"

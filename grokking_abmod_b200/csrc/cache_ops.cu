@@ -1,0 +1,305 @@
+// Writing new rows of K and V into the 8-bit paged cache, and reading a range
+// of it back as floats.  Both move each byte once: the write reads a page's
+// new rows into registers, reduces their largest magnitude, and stores the
+// codes from the registers; the read loads codes and stores values.
+
+#include <algorithm>
+#include <climits>
+
+#include "cache_host.h"
+#include "dtype.cuh"
+
+namespace mb {
+namespace cache {
+
+constexpr int kThreads = 256;
+constexpr int kHeld = 8;  // 16-byte input vectors a thread holds between the reduction and the store
+
+template <class T>
+struct Rows {
+  const T* p;
+  size_t row_stride, head_stride;
+  bool vector;  // base and strides allow 16-byte loads
+};
+
+// VEC channels [c, c + VEC) of a row; channels from head_dim on are 0.
+template <class T>
+__device__ __forceinline__ uint4 load_chunk(const Rows<T>& rows, size_t row, int head, int c, int head_dim) {
+  constexpr int VEC = Element<T>::kVec;
+  const T* p = rows.p + row * rows.row_stride + (size_t)head * rows.head_stride + c;
+  if (rows.vector && c + VEC <= head_dim) return __ldg(reinterpret_cast<const uint4*>(p));
+  union {
+    uint4 v;
+    T e[VEC];
+  } u;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) u.e[i] = c + i < head_dim ? p[i] : Element<T>::from(0.f);
+  return u.v;
+}
+
+template <class T>
+__device__ __forceinline__ uint32_t magnitude(uint4 raw) {
+  float x[Element<T>::kVec];
+  Element<T>::unpack(raw, x);
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < Element<T>::kVec; ++i) m = max(m, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+  return m;
+}
+
+__device__ __forceinline__ uint32_t pack_codes(float a, float b, float c, float d) {
+  // a NaN scale gives code 0
+  return (uint32_t)(__float2int_rn(a) & 0xFF) | (uint32_t)(__float2int_rn(b) & 0xFF) << 8 |
+         (uint32_t)(__float2int_rn(c) & 0xFF) << 16 | (uint32_t)(__float2int_rn(d) & 0xFF) << 24;
+}
+
+template <class T>
+__device__ __forceinline__ void store_codes(int8_t* at, uint4 raw, float inverse) {
+  float x[Element<T>::kVec];
+  Element<T>::unpack(raw, x);
+#pragma unroll
+  for (int i = 0; i < Element<T>::kVec; ++i) x[i] *= inverse;
+  if constexpr (Element<T>::kVec == 4) {
+    *reinterpret_cast<uint32_t*>(at) = pack_codes(x[0], x[1], x[2], x[3]);
+  } else {
+    *reinterpret_cast<uint2*>(at) = make_uint2(pack_codes(x[0], x[1], x[2], x[3]), pack_codes(x[4], x[5], x[6], x[7]));
+  }
+}
+
+// A group of G threads (32: a warp, kThreads: the CTA) writes one page of one
+// head, of K (blockIdx.y 0) or V (1).
+template <class T, int G>
+__global__ void __launch_bounds__(kThreads)
+    write_pages(View c, Batch t, Rows<T> k, Rows<T> v, int head_dim, int page_slots, int* status) {
+  constexpr int VEC = Element<T>::kVec;
+  const int id = threadIdx.x % G;
+  const size_t unit = (size_t)blockIdx.x * (kThreads / G) + threadIdx.x / G;
+  const int head = (int)(unit % c.heads);
+  const size_t rest = unit / c.heads;
+  const int b = (int)(rest / page_slots), slot_page = (int)(rest % page_slots);
+  if (b >= t.count) return;
+  const Span s = span_of(t, c, b);
+  const bool report = status != nullptr && id == 0 && head == 0 && blockIdx.y == 0;
+  if (report && slot_page == 0) {
+    // pages past the announced number of new rows are not visited
+    const bool missed = s.fresh && ((s.length - s.fresh) >> c.shift) + page_slots <= (s.length - 1) >> c.shift;
+    const int flags = s.flags ? s.flags : missed ? kBadRows : 0;
+    if (flags) atomicOr(status, flags);
+  }
+  if (s.flags || s.fresh == 0) return;  // nothing is written for a sequence whose numbers do not fit
+  const int old = s.length - s.fresh;   // tokens before the new ones
+  const int index = (old >> c.shift) + slot_page;
+  if (index > (s.length - 1) >> c.shift) return;
+  const int lo = index << c.shift;
+  const int from = max(lo, old), to = lo + min(c.tokens, s.length - lo);
+  const int page = page_of(t, c, b, index);
+  if (page < 0) {
+    if (report) atomicOr(status, kBadPage);
+    return;
+  }
+  const Rows<T>& in = blockIdx.y ? v : k;
+  int8_t* codes = (blockIdx.y ? c.v : c.k) + c.row(page, head, 0);
+  float* scale_at = (blockIdx.y ? c.v_scale : c.k_scale) + c.scale_at(page, head);
+  const float before = from > lo ? *scale_at : 0.f;
+
+  const int per_row = c.width / VEC;  // width is a multiple of 32
+  const int chunks = (to - from) * per_row;
+  const size_t row0 = s.row + (from - old);
+  uint4 raw[kHeld];
+  uint32_t most = 0;
+  const bool held = chunks <= G * kHeld;
+  for (int base = 0; base < chunks; base += G * kHeld) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int e = base + i * G + id;
+      if (e < chunks) {
+        const int r = e / per_row;
+        raw[i] = load_chunk(in, row0 + r, head, (e - r * per_row) * VEC, head_dim);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (base + i * G + id < chunks) most = max(most, magnitude<T>(raw[i]));
+  }
+  most = __reduce_max_sync(0xFFFFFFFFu, most);
+  if constexpr (G > 32) {
+    __shared__ uint32_t parts[G / 32];
+    if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = most;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < G / 32; ++w) most = max(most, parts[w]);
+  }
+  float scale = scale_for(most);
+  if (from > lo) {
+    // the page's earlier tokens: the scale never shrinks, NaN stays
+    if (before != before || before > scale) scale = before;
+    if (scale != before) {
+      const float ratio = before / scale;
+      uint32_t* w = reinterpret_cast<uint32_t*>(codes);
+      for (int e = id; e < (from - lo) * (c.width / 4); e += G) {
+        const uint32_t q = w[e];
+        w[e] = pack_codes(rintf((float)(int8_t)q * ratio), rintf((float)(int8_t)(q >> 8) * ratio),
+                          rintf((float)(int8_t)(q >> 16) * ratio), rintf((float)(int8_t)(q >> 24) * ratio));
+      }
+    }
+  }
+  // the group read `before` before this store: in lockstep for a warp, behind
+  // the barrier above for a CTA
+  if (id == 0) *scale_at = scale;
+  const float inverse = 1.0f / scale;
+  codes += (size_t)(from - lo) * c.width;
+  for (int base = 0; base < chunks; base += G * kHeld) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      const int e = base + i * G + id;
+      if (e < chunks) {
+        if (!held) {
+          const int r = e / per_row;
+          raw[i] = load_chunk(in, row0 + r, head, (e - r * per_row) * VEC, head_dim);
+        }
+        store_codes<T>(codes + (size_t)e * VEC, raw[i], inverse);
+      }
+    }
+  }
+}
+
+constexpr int kReadTokens = 4;  // tokens a thread has in flight
+
+// out [batch][tokens][heads][head_dim]: blockIdx.x a run of tokens of one
+// sequence, blockIdx.y a run of columns (head, chunk), blockIdx.z K or V.
+template <class T, int CHUNK>
+__global__ void __launch_bounds__(kThreads)
+    read_pages(View c, Batch t, const int32_t* __restrict__ first, int tokens, int head_dim, int columns,
+               int columns_here, int runs, T* __restrict__ k_out, T* __restrict__ v_out, int* status) {
+  const int b = blockIdx.x / runs, run = blockIdx.x % runs;
+  const int lanes = kThreads / columns_here;  // tokens side by side
+  const int column = blockIdx.y * columns_here + threadIdx.x % columns_here;
+  const int lane = threadIdx.x / columns_here;
+  if (lane >= lanes || column >= columns) return;
+  const int chunks = head_dim / CHUNK;
+  const int head = column / chunks, ch = (column - head * chunks) * CHUNK;
+  const int8_t* codes = blockIdx.z ? c.v : c.k;
+  const float* scales = blockIdx.z ? c.v_scale : c.k_scale;
+  T* out = blockIdx.z ? v_out : k_out;
+  const int n = t.lengths[b];
+  const long long room = (long long)t.table_pages << c.shift;
+  const int length = (int)(n < 0 ? 0 : n > room ? room : n);
+  if (status && run == 0 && column == 0 && lane == 0 && blockIdx.z == 0 && length != n) atomicOr(status, kBadLength);
+  const long long start = first ? first[b] : 0;
+  uint2 q[kReadTokens];
+  float scale[kReadTokens];
+#pragma unroll
+  for (int u = 0; u < kReadTokens; ++u) {
+    const int i = (run * kReadTokens + u) * lanes + lane;
+    const long long pos = start + i;
+    q[u] = make_uint2(0u, 0u);
+    scale[u] = 0.f;
+    if (i < tokens && pos >= 0 && pos < length) {
+      const int page = page_of(t, c, b, (int)(pos >> c.shift));
+      if (page >= 0) {
+        const int8_t* at = codes + c.row(page, head, (int)pos & (c.tokens - 1)) + ch;
+        if constexpr (CHUNK == 8) q[u] = __ldg(reinterpret_cast<const uint2*>(at));
+        else if constexpr (CHUNK == 4) q[u].x = __ldg(reinterpret_cast<const uint32_t*>(at));
+        else q[u].x = (uint8_t)*at;
+        scale[u] = __ldg(scales + c.scale_at(page, head));
+      } else {
+        scale[u] = NAN;  // the tokens that should be there
+        if (status) atomicOr(status, kBadPage);
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kReadTokens; ++u) {
+    const int i = (run * kReadTokens + u) * lanes + lane;
+    if (i >= tokens) continue;
+    T* o = out + (((size_t)b * tokens + i) * c.heads + head) * head_dim + ch;
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < CHUNK; ++e)
+      x[e] = (float)(int8_t)((e < 4 ? q[u].x : q[u].y) >> (8 * (e & 3))) * scale[u];
+    if constexpr (CHUNK == 1) *o = Element<T>::from(x[0]);
+    else *reinterpret_cast<uint4*>(o) = Element<T>::pack(x);
+  }
+}
+
+template <class T>
+Rows<T> make_rows(const void* p, size_t row_stride, size_t head_stride) {
+  constexpr size_t VEC = Element<T>::kVec;
+  require(reinterpret_cast<uintptr_t>(p) % sizeof(T) == 0, "rows must be aligned to their elements");
+  return Rows<T>{static_cast<const T*>(p), row_stride, head_stride,
+                 reinterpret_cast<uintptr_t>(p) % 16 == 0 && row_stride % VEC == 0 && head_stride % VEC == 0};
+}
+
+}  // namespace cache
+}  // namespace mb
+
+extern "C" {
+
+int mb_op_cache_write(const mb_kv_cache* cache, const mb_cache_rows* where, uint32_t head_dim, const void* k,
+                      size_t k_row_stride, size_t k_head_stride, const void* v, size_t v_row_stride,
+                      size_t v_head_stride, uint32_t dtype, uint32_t max_new, int* d_status, void* stream) {
+  using namespace mb::cache;
+  return mb::guarded([&] {
+    const View c = view_of(cache, head_dim);
+    const Batch t = batch_of(where, max_new);
+    if (t.rows == 0 || max_new == 0 || t.count == 0) return;
+    mb::need(k, "k");
+    mb::need(v, "v");
+    const int page_slots = (int)(((size_t)max_new + c.tokens - 2) / c.tokens + 1);
+    const size_t units = (size_t)t.count * page_slots * c.heads;
+    cudaStream_t st = (cudaStream_t)stream;
+    mb::with_dtype(dtype, [&](auto tag) {
+      using T = typename decltype(tag)::type;
+      const Rows<T> kr = make_rows<T>(k, k_row_stride, k_head_stride), vr = make_rows<T>(v, v_row_stride, v_head_stride);
+      // a warp where it can hold a page's new rows in registers, else a CTA
+      const size_t vectors = std::min<size_t>(max_new, c.tokens) * c.width / mb::Element<T>::kVec;
+      const bool warp = vectors <= 32 * kHeld;
+      const size_t blocks = warp ? (units + kThreads / 32 - 1) / (kThreads / 32) : units;
+      mb::require(blocks <= (size_t)INT_MAX, "too many pages for one call");
+      const dim3 grid((unsigned)blocks, 2);
+      if (warp)
+        write_pages<T, 32><<<grid, kThreads, 0, st>>>(c, t, kr, vr, (int)head_dim, page_slots, d_status);
+      else
+        write_pages<T, kThreads><<<grid, kThreads, 0, st>>>(c, t, kr, vr, (int)head_dim, page_slots, d_status);
+      mb::launched("cache write");
+    });
+  });
+}
+
+int mb_op_cache_read(const mb_kv_cache* cache, const mb_cache_rows* where, uint32_t head_dim, const int32_t* first,
+                     uint32_t tokens, void* k_out, void* v_out, uint32_t dtype, int* d_status, void* stream) {
+  using namespace mb::cache;
+  return mb::guarded([&] {
+    const View c = view_of(cache, head_dim);
+    const Batch t = batch_of(where, 0);
+    mb::require(tokens <= (1u << 30), "tokens must be at most 2^30");
+    if (tokens == 0 || t.count == 0) return;
+    mb::need(k_out, "k_out");
+    mb::need(v_out, "v_out");
+    cudaStream_t st = (cudaStream_t)stream;
+    mb::with_dtype(dtype, [&](auto tag) {
+      using T = typename decltype(tag)::type;
+      constexpr int VEC = mb::Element<T>::kVec;
+      for (const void* p : {(const void*)k_out, (const void*)v_out})
+        mb::require(reinterpret_cast<uintptr_t>(p) % sizeof(T) == 0, "outputs must be aligned to their elements");
+      const bool vector = head_dim % VEC == 0 && reinterpret_cast<uintptr_t>(k_out) % 16 == 0 &&
+                          reinterpret_cast<uintptr_t>(v_out) % 16 == 0;
+      const int columns = c.heads * (int)(head_dim / (vector ? VEC : 1));
+      const int here = std::min(columns, kThreads);
+      const int per_block = kThreads / here * kReadTokens;
+      const size_t runs = (tokens + (size_t)per_block - 1) / per_block;
+      mb::require(runs * t.count <= (size_t)INT_MAX && (columns + here - 1) / here <= 65535,
+                  "too many tokens for one call");
+      const dim3 grid((unsigned)(runs * t.count), (unsigned)((columns + here - 1) / here), 2);
+      if (vector)
+        read_pages<T, VEC><<<grid, kThreads, 0, st>>>(c, t, first, (int)tokens, (int)head_dim, columns, here,
+                                                      (int)runs, (T*)k_out, (T*)v_out, d_status);
+      else
+        read_pages<T, 1><<<grid, kThreads, 0, st>>>(c, t, first, (int)tokens, (int)head_dim, columns, here,
+                                                    (int)runs, (T*)k_out, (T*)v_out, d_status);
+      mb::launched("cache read");
+    });
+  });
+}
+
+}  // extern "C"

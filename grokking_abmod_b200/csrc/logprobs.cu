@@ -1,0 +1,602 @@
+// Log-probabilities of given tokens from rows of logits, with the rows'
+// entropy and their k most likely tokens, and the gradient of the first two.
+//
+//   m = max_j x_j, d_j = m - x_j, s = sum_j e^-d_j
+//   lse = m + ln s, logprob = x_t - lse, H = ln s + (sum_j e^-d_j d_j) / s
+//   dx_j = g (1[j = t] - p_j) - h p_j (ln p_j + H),  p_j = e^(x_j - lse)
+//
+// H is a sum of nonnegative terms, so nothing cancels where one token takes
+// nearly all the probability.  The forward reads each logit once: every
+// thread keeps a running (m, s, sum) of its own elements, rescaled when its
+// maximum rises, and the triples are joined at the end in a fixed order.
+//
+// Top tokens order by (value descending, index ascending), a total order, so
+// ties go to the lowest index whatever the launch shape.  Values map to
+// integers in that order; a warp holds its candidates sorted, one a lane, and
+// a new element enters only if it beats the k-th best that any warp of its
+// CTA has so far - after the first elements of a row that is rare, and costs
+// one compare per 16 or 32 elements.
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+
+#include "common.cuh"
+#include "dtype.cuh"
+
+namespace mb {
+namespace logprobs {
+
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kMaxTop = 32;
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kUnroll = 4;      // 16-byte vectors a thread has in flight
+constexpr int kRowLanes = 1024; // vocabularies up to here take one warp per row
+constexpr unsigned kFull = 0xFFFFFFFFu;
+
+using u64 = unsigned long long;
+
+// Running statistics in base-2 units: s = sum 2^-t, a = sum 2^-t t with
+// t = (m - x) log2 e.
+struct Stats {
+  float m, s, a;
+};
+
+__device__ __forceinline__ Stats empty_stats() { return Stats{-INFINITY, 0.f, 0.f}; }
+
+// Moves the statistics to a maximum m >= s.m.
+__device__ __forceinline__ Stats rebase(Stats s, float m) {
+  if (s.m == -INFINITY) return Stats{m, s.s, s.a};  // nothing counted (or only NaN terms)
+  const float t = (m - s.m) * kLog2e;
+  const float c = ex2_ftz(-t);
+  return Stats{m, s.s * c, c * fmaf(t, s.s, s.a)};
+}
+
+__device__ __forceinline__ Stats join(Stats p, Stats q) {
+  // a maximum of -inf on both sides: sums of empty sets, or NaN that stay NaN
+  const float m = fmaxf(p.m, q.m);
+  if (m == -INFINITY) return Stats{m, p.s + q.s, p.a + q.a};
+  p = rebase(p, m);
+  q = rebase(q, m);
+  return Stats{m, p.s + q.s, p.a + q.a};
+}
+
+__device__ __forceinline__ Stats warp_join(Stats v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    Stats w;
+    w.m = __shfl_xor_sync(kFull, v.m, o);
+    w.s = __shfl_xor_sync(kFull, v.s, o);
+    w.a = __shfl_xor_sync(kFull, v.a, o);
+    v = join(v, w);
+  }
+  return v;
+}
+
+// Adds N elements whose largest is mx.
+template <int N>
+__device__ __forceinline__ void accumulate(Stats& st, const float (&x)[N], float mx) {
+  if (mx > st.m) st = rebase(st, mx);
+  // all of them -inf so far: differences from 0 keep the terms at 2^-inf = 0
+  const float m = st.m == -INFINITY ? 0.f : st.m;
+  const float2 mm = splat2(m), scale = splat2(kLog2e);
+  float2 s = make_float2(0.f, 0.f), a = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const float2 t = mul2(add2(mm, make_float2(-x[i], -x[i + 1])), scale);
+    const float2 e = make_float2(ex2_ftz(-t.x), ex2_ftz(-t.y));
+    s = add2(s, e);
+    // a masked logit (-inf) has t = +inf and e = 0: its term is 0, not NaN
+    a = fma2(e, make_float2(fminf(t.x, 1e30f), fminf(t.y, 1e30f)), a);
+  }
+  st.s += s.x + s.y;
+  st.a += a.x + a.y;
+}
+
+// The order of the top list: larger keys first.  -0 counts as +0, NaN above
+// everything; 0 is below every element.
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const uint32_t b = __float_as_uint(x + 0.0f);
+  if (x != x) return 0xFFFFFFFFu;
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float unordered(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k);
+}
+__device__ __forceinline__ u64 top_key(float x, uint32_t index) { return ((u64)ordered(x) << 32) | (uint32_t)~index; }
+
+// Inserts a warp-uniform key into the warp's list (lane i holds the i-th
+// largest).  The keys of a row are distinct.
+__device__ __forceinline__ void insert(u64& mine, u64 key, int lane) {
+  const int pos = __popc(__ballot_sync(kFull, mine > key));
+  const u64 up = __shfl_up_sync(kFull, mine, 1);
+  if (lane == pos) mine = key;
+  if (lane > pos) mine = up;
+}
+
+// Offers each lane's key to the list; keys at or below `floor` are out.
+__device__ __forceinline__ void offer(u64& mine, u64 key, u64 floor, int top, int lane) {
+  u64 least = __shfl_sync(kFull, mine, top - 1);
+  if (least < floor) least = floor;
+  unsigned who = __ballot_sync(kFull, key > least);
+  while (who) {
+    const int src = __ffs(who) - 1;
+    who &= who - 1;
+    const u64 k = __shfl_sync(kFull, key, src);
+    if (k > least) {
+      insert(mine, k, lane);
+      least = __shfl_sync(kFull, mine, top - 1);
+      if (least < floor) least = floor;
+    }
+  }
+}
+
+struct Out {
+  float *logprob, *entropy, *lse, *top_logprob;
+  int* top_index;
+  int* status;
+};
+
+// Writes a row's results; one warp, with the joined statistics in every lane
+// and the list in its lanes.
+template <class T>
+__device__ __forceinline__ void finish(const Out& o, size_t row, const T* x, int vocab, const int* tokens, int top,
+                                       Stats st, u64 mine, int lane) {
+  const bool none = st.m == -INFINITY && st.s == 0.f;  // every token masked
+  const float log_s = logf(st.s);
+  const float lse = none ? -INFINITY : (st.m == -INFINITY ? st.s : st.m + log_s);
+  if (lane == 0) {
+    o.lse[row] = lse;
+    o.entropy[row] = none ? 0.f : log_s + st.a / st.s * kLn2;
+    const int t = tokens[row];
+    float lp = 0.f;
+    if (t != -1) {
+      if ((unsigned)t < (unsigned)vocab) {
+        lp = none ? -INFINITY : Element<T>::to(x[t]) - lse;
+      } else {
+        lp = NAN;
+        if (o.status) atomicOr(o.status, 2);
+      }
+    }
+    o.logprob[row] = lp;
+  }
+  if (lane < top) {
+    const float v = unordered((uint32_t)(mine >> 32));
+    o.top_logprob[row * top + lane] = v == -INFINITY ? v : v - lse;
+    o.top_index[row * top + lane] = (int)~(uint32_t)mine;
+  }
+}
+
+// One warp per row, the whole row in registers (R elements a lane).
+template <class T, int R>
+__global__ void __launch_bounds__(kThreads)
+    forward_small(const T* __restrict__ logits, size_t stride, size_t rows, int vocab, const int* __restrict__ tokens,
+                  int top, Out o) {
+  const int lane = threadIdx.x & 31;
+  const size_t row = (size_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const T* x = logits + row * stride;
+  float v[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) v[r] = lane + 32 * r < vocab ? Element<T>::to(x[lane + 32 * r]) : -INFINITY;
+  float mx = v[0];
+#pragma unroll
+  for (int r = 1; r < R; ++r) mx = fmaxf(mx, v[r]);
+  Stats st = empty_stats();
+  accumulate(st, v, mx);
+  st = warp_join(st);
+  u64 mine = 0;
+  if (top) {
+    // k times: the largest key of all lanes, taken out of the lane it is in
+    uint32_t best = 0, at = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const uint32_t k = lane + 32 * r < vocab ? ordered(v[r]) : 0u;
+      if (k > best) best = k, at = r;
+    }
+    uint32_t taken = 0;  // bit r: v[r] is in the list
+    for (int i = 0; i < top; ++i) {
+      const uint32_t k = __reduce_max_sync(kFull, best);
+      const uint32_t index = __reduce_min_sync(kFull, best == k ? lane + 32u * at : kFull);
+      if (lane == i) mine = ((u64)k << 32) | (uint32_t)~index;
+      if (lane == (int)(index & 31u)) {
+        taken |= 1u << at;
+        best = 0;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const uint32_t c = lane + 32 * r < vocab && !((taken >> r) & 1u) ? ordered(v[r]) : 0u;
+          if (c > best) best = c, at = r;
+        }
+      }
+    }
+  }
+  finish(o, row, x, vocab, tokens, top, st, mine, lane);
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+// Reads 4 bytes at the address that `p` has in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t remote_u32(const void* p, uint32_t rank) {
+  uint32_t a = (uint32_t)__cvta_generic_to_shared(p), v;
+  asm volatile(
+      "{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %1, %2;\n\tld.shared::cluster.u32 %0, [r];\n\t}"
+      : "=r"(v)
+      : "r"(a), "r"(rank)
+      : "memory");
+  return v;
+}
+
+// A thread's statistics and its warp's list, fed N elements a step.
+struct Running {
+  Stats st = empty_stats();
+  u64 mine = 0, floor = 0;  // keys at or below floor are out
+  bool first = true;
+  int lane, top;
+  u64* floor_key;  // the CTA's highest k-th best
+
+  // Element i of x is element at + (i / VEC) * apart + i % VEC of the row;
+  // those from `end` on are -inf and not of the row.
+  template <int VEC, int N>
+  __device__ __forceinline__ void step(const float (&x)[N], int at, int apart, int end) {
+    float mx = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) mx = fmaxf(mx, x[i]);
+    accumulate(st, x, mx);
+    if (!top) return;
+    const u64 shared = *(volatile u64*)floor_key;
+    if (shared > floor) floor = shared;
+    if (first) {
+      // k lanes hold an element at or above the k-th largest lane maximum,
+      // so nothing below that can be in the list
+      first = false;
+      u64 best = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const u64 k = key<VEC>(x[i], i, at, apart, end);
+        if (k > best) best = k;
+      }
+      int above = 0;
+      for (int l = 0; l < 32; ++l) above += __shfl_sync(kFull, best, l) > best;
+      const unsigned kth = __ballot_sync(kFull, best != 0 && above == top - 1);
+      if (kth) {
+        const u64 k = __shfl_sync(kFull, best, __ffs(kth) - 1) - 1;
+        if (k > floor) floor = k;
+      }
+    }
+    const u64 last = __shfl_sync(kFull, mine, top - 1);
+    const uint32_t least = (uint32_t)((last > floor ? last : floor) >> 32);
+    // a maximum does not show NaN, the sum does
+    if (__any_sync(kFull, ordered(mx) >= least || st.s != st.s)) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) offer(mine, key<VEC>(x[i], i, at, apart, end), floor, top, lane);
+      if (lane == top - 1 && mine > floor) atomicMax(floor_key, mine);
+    }
+  }
+
+  template <int VEC>
+  static __device__ __forceinline__ u64 key(float x, int i, int at, int apart, int end) {
+    const int index = at + (i / VEC) * apart + i % VEC;
+    return index < end ? top_key(x, (uint32_t)index) : 0;
+  }
+};
+
+// One cluster per row, each CTA a contiguous share of it.  The ragged head
+// and tail around the 16-byte aligned body (odd vocabularies leave rows
+// unaligned) are one more step of single elements.
+template <class T>
+__global__ void __launch_bounds__(kThreads)
+    forward_wide(const T* __restrict__ logits, size_t stride, int vocab, const int* __restrict__ tokens, int top,
+                 Out o) {
+  constexpr int VEC = Element<T>::kVec, N = kUnroll * VEC;
+  __shared__ Stats warp_stats[kWarps];
+  __shared__ u64 lists[kWarps][kMaxTop];
+  __shared__ u64 floor_key;
+  __shared__ uint32_t cta_stats[3];
+  __shared__ uint32_t cta_list[2 * kMaxTop];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t rank = cluster_rank(), ranks = cluster_size();
+  const size_t row = blockIdx.x / ranks;
+  const T* x = logits + row * stride;
+  if (threadIdx.x == 0) floor_key = 0;
+  __syncthreads();
+
+  const int lead = (int)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(T));
+  const int head = lead < vocab ? lead : vocab;
+  const int vectors = (vocab - head) / VEC;
+  const int tail = head + vectors * VEC;  // [tail, vocab) is left over
+  const int share = (vectors + ranks - 1) / ranks;
+  const int begin = min(vectors, (int)rank * share), end = min(vectors, begin + share);
+  const uint4* body = reinterpret_cast<const uint4*>(x + head);
+
+  Running run;
+  run.lane = lane;
+  run.top = top;
+  run.floor_key = &floor_key;
+
+  // whole warps take part in every step (the list code votes)
+  for (int j = begin + warp * 32; j < end; j += kThreads * kUnroll) {
+    float v[N];
+    uint4 raw[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int at = j + lane + u * kThreads;
+      if (at < end) raw[u] = __ldg(body + at);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      if (j + lane + u * kThreads < end) {
+        Element<T>::unpack(raw[u], v + u * VEC);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[u * VEC + i] = -INFINITY;
+      }
+    }
+    run.step<VEC, N>(v, head + (j + lane) * VEC, kThreads * VEC, head + end * VEC);
+  }
+  if (rank == 0 && warp == 0) {
+    // head + tail: fewer than 2 VEC elements, one a lane
+    const int left = head + vocab - tail;
+    const int at = lane < head ? lane : tail + lane - head;
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = -INFINITY;
+    if (lane < left) v[0] = Element<T>::to(x[at]);
+    run.step<1, N>(v, at, 1, lane < left ? at + 1 : 0);
+  }
+
+  Stats st = warp_join(run.st);
+  u64 mine = run.mine;
+  if (lane == 0) warp_stats[warp] = st;
+  if (lane < top) lists[warp][lane] = mine;
+  __syncthreads();
+  if (warp == 0) {
+    st = warp_stats[0];
+    for (int w = 1; w < kWarps; ++w) st = join(st, warp_stats[w]);
+    if (top)
+      for (int w = 1; w < kWarps; ++w) offer(mine, lane < top ? lists[w][lane] : 0, 0, top, lane);
+    if (ranks > 1) {
+      if (lane == 0) {
+        cta_stats[0] = __float_as_uint(st.m);
+        cta_stats[1] = __float_as_uint(st.s);
+        cta_stats[2] = __float_as_uint(st.a);
+      }
+      cta_list[2 * lane] = (uint32_t)mine;
+      cta_list[2 * lane + 1] = (uint32_t)(mine >> 32);
+    }
+  }
+  if (ranks > 1) {
+    cluster_sync();
+    if (rank == 0 && warp == 0) {
+      for (uint32_t r = 1; r < ranks; ++r) {
+        Stats q;
+        q.m = __uint_as_float(remote_u32(&cta_stats[0], r));
+        q.s = __uint_as_float(remote_u32(&cta_stats[1], r));
+        q.a = __uint_as_float(remote_u32(&cta_stats[2], r));
+        st = join(st, q);
+        if (top) {
+          const u64 lo = remote_u32(&cta_list[2 * lane], r), hi = remote_u32(&cta_list[2 * lane + 1], r);
+          offer(mine, lane < top ? (hi << 32) | lo : 0, 0, top, lane);
+        }
+      }
+    }
+    cluster_sync();  // the lists stay in place until they have been read
+  }
+  if (rank == 0 && warp == 0) finish(o, row, x, vocab, tokens, top, st, mine, lane);
+}
+
+// ---------------------------------------------------------------- gradient
+// Per row: the coefficients of dx_j = [j = t] g - p_j (g + h (ln p_j + H)).
+struct RowGrad {
+  float lse, g, h, gh;  // gh = g + h H
+  int token;
+  bool none;
+};
+
+struct GradIn {
+  const int* tokens;
+  const float *lse, *entropy, *dlogprob, *dentropy;
+  int* status;
+};
+
+__device__ __forceinline__ RowGrad row_grad(const GradIn& in, size_t row, int vocab, bool report) {
+  RowGrad r;
+  r.lse = in.lse[row];
+  r.token = in.tokens[row];
+  r.none = r.lse == -INFINITY;  // nothing to move
+  r.g = in.dlogprob && r.token != -1 ? in.dlogprob[row] : 0.f;
+  r.h = in.dentropy ? in.dentropy[row] : 0.f;
+  r.gh = r.h != 0.f ? fmaf(r.h, in.entropy[row], r.g) : r.g;
+  if (r.token != -1 && (unsigned)r.token >= (unsigned)vocab) {
+    r.g = r.gh = NAN;
+    if (report && in.status) atomicOr(in.status, 2);
+  }
+  return r;
+}
+
+__device__ __forceinline__ float element_grad(const RowGrad& r, float x, int j) {
+  const float logp = x - r.lse;
+  const float p = ex2_ftz(logp * kLog2e);
+  // p = 0 where the token is masked: its ln p is not looked at
+  float d = -p * fmaf(r.h, fmaxf(logp, -1e30f), r.gh);
+  if (j == r.token) d += r.g;
+  return r.none ? 0.f : d;
+}
+
+// A group of G threads per row (32: a warp; kThreads: the CTA).
+template <class T, int G>
+__global__ void __launch_bounds__(kThreads)
+    backward_rows(const T* __restrict__ logits, size_t stride, size_t rows, int vocab, GradIn in,
+                  T* __restrict__ dlogits) {
+  constexpr int VEC = Element<T>::kVec;
+  const int id = threadIdx.x % G;
+  const size_t row = (size_t)blockIdx.x * (kThreads / G) + threadIdx.x / G;
+  if (row >= rows) return;
+  const T* x = logits + row * stride;
+  T* d = dlogits + row * vocab;
+  const RowGrad r = row_grad(in, row, vocab, id == 0);
+  const int part = G == kThreads ? blockIdx.y : 0, parts = G == kThreads ? gridDim.y : 1;
+  if (((uintptr_t)x & 15) == ((uintptr_t)d & 15)) {
+    const int lead = (int)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(T));
+    const int head = lead < vocab ? lead : vocab;
+    const int vectors = (vocab - head) / VEC, tail = head + vectors * VEC;
+    const uint4* bx = reinterpret_cast<const uint4*>(x + head);
+    uint4* bd = reinterpret_cast<uint4*>(d + head);
+    for (int j = part * G * kUnroll + id; j < vectors; j += parts * G * kUnroll) {
+      uint4 raw[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (j + u * G < vectors) raw[u] = __ldg(bx + j + u * G);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (j + u * G < vectors) {
+          float v[VEC];
+          Element<T>::unpack(raw[u], v);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) v[i] = element_grad(r, v[i], head + (j + u * G) * VEC + i);
+          bd[j + u * G] = Element<T>::pack(v);
+        }
+    }
+    if (part == 0 && id < head + vocab - tail) {
+      const int at = id < head ? id : tail + id - head;
+      d[at] = Element<T>::from(element_grad(r, Element<T>::to(x[at]), at));
+    }
+  } else {
+    for (int j = part * G + id; j < vocab; j += parts * G)
+      d[j] = Element<T>::from(element_grad(r, Element<T>::to(x[j]), j));
+  }
+}
+
+inline int sm_count() {
+  int dev = 0, sms = 1;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    throw Error(MB_ERR_CUDA, "no CUDA device");
+  return sms;
+}
+
+// CTAs per row: enough rows fill the GPU with one each; few rows are cut into
+// up to 8 shares (the portable cluster size) of at least 4096 elements.
+inline unsigned row_shares(size_t rows, int vocab) {
+  const size_t want = (size_t)sm_count() * 4;
+  unsigned n = 1;
+  while (n < 8 && rows * n * 2 <= want && vocab / (int)(n * 2) >= 4096) n *= 2;
+  return n;
+}
+
+inline void shape(size_t rows, uint32_t vocab, size_t stride) {
+  require(rows >= 1 && rows <= (size_t)INT_MAX / 8, "rows must be in 1..2^28");
+  require(vocab >= 1 && vocab <= (1u << 30), "vocab must be in 1..2^30");
+  require(stride >= vocab || rows == 1, "the row stride must be at least vocab");
+}
+
+inline void aligned(const void* p, size_t bytes, const char* what) {
+  require((reinterpret_cast<uintptr_t>(p) % bytes) == 0, std::string(what) + " must be aligned to its elements");
+}
+
+template <class T, int R>
+void launch_small(const T* x, size_t stride, size_t rows, uint32_t vocab, const int* tokens, uint32_t top, const Out& o,
+                  cudaStream_t st) {
+  forward_small<T, R><<<(unsigned)((rows + kWarps - 1) / kWarps), kThreads, 0, st>>>(x, stride, rows, (int)vocab,
+                                                                                    tokens, (int)top, o);
+}
+
+template <class T>
+void launch_forward(const T* x, size_t stride, size_t rows, uint32_t vocab, const int* tokens, uint32_t top,
+                    const Out& o, cudaStream_t st) {
+  if (vocab <= 64) return launch_small<T, 2>(x, stride, rows, vocab, tokens, top, o, st);
+  if (vocab <= 128) return launch_small<T, 4>(x, stride, rows, vocab, tokens, top, o, st);
+  if (vocab <= 256) return launch_small<T, 8>(x, stride, rows, vocab, tokens, top, o, st);
+  if (vocab <= 512) return launch_small<T, 16>(x, stride, rows, vocab, tokens, top, o, st);
+  if (vocab <= (uint32_t)kRowLanes) return launch_small<T, 32>(x, stride, rows, vocab, tokens, top, o, st);
+  const unsigned shares = row_shares(rows, (int)vocab);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows * shares));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = shares;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, forward_wide<T>, x, stride, (int)vocab, tokens, (int)top, o);
+  require(e == cudaSuccess, std::string("token log-probabilities: ") + cudaGetErrorString(e), MB_ERR_CUDA);
+}
+
+}  // namespace logprobs
+}  // namespace mb
+
+extern "C" {
+
+int mb_op_token_logprobs(const void* logits, uint32_t dtype, size_t row_stride, size_t rows, uint32_t vocab,
+                         const int32_t* tokens, uint32_t top, float* logprob, float* entropy, float* lse,
+                         float* top_logprob, int32_t* top_index, int* d_status, void* stream) {
+  using namespace mb::logprobs;
+  return mb::guarded([&] {
+    mb::need(logits, "logits");
+    mb::need(tokens, "tokens");
+    mb::need(logprob, "logprob");
+    mb::need(entropy, "entropy");
+    mb::need(lse, "lse");
+    shape(rows, vocab, row_stride);
+    mb::require(top <= (uint32_t)kMaxTop && top <= vocab, "top must be in 0..32 and at most vocab");
+    if (top) {
+      mb::need(top_logprob, "top_logprob");
+      mb::need(top_index, "top_index");
+    }
+    const Out o{logprob, entropy, lse, top_logprob, top_index, d_status};
+    cudaStream_t st = (cudaStream_t)stream;
+    mb::with_dtype(dtype, [&](auto tag) {
+      using T = typename decltype(tag)::type;
+      aligned(logits, sizeof(T), "logits");
+      launch_forward<T>(static_cast<const T*>(logits), row_stride, rows, vocab, tokens, top, o, st);
+      mb::launched("token log-probabilities");
+    });
+  });
+}
+
+int mb_op_token_logprobs_backward(const void* logits, uint32_t dtype, size_t row_stride, size_t rows, uint32_t vocab,
+                                  const int32_t* tokens, const float* lse, const float* entropy,
+                                  const float* dlogprob, const float* dentropy, void* dlogits, int* d_status,
+                                  void* stream) {
+  using namespace mb::logprobs;
+  return mb::guarded([&] {
+    mb::need(logits, "logits");
+    mb::need(tokens, "tokens");
+    mb::need(lse, "lse");
+    mb::need(dlogits, "dlogits");
+    if (dentropy) mb::need(entropy, "entropy");
+    shape(rows, vocab, row_stride);
+    const GradIn in{tokens, lse, entropy, dlogprob, dentropy, d_status};
+    cudaStream_t st = (cudaStream_t)stream;
+    mb::with_dtype(dtype, [&](auto tag) {
+      using T = typename decltype(tag)::type;
+      aligned(logits, sizeof(T), "logits");
+      aligned(dlogits, sizeof(T), "dlogits");
+      const T* x = static_cast<const T*>(logits);
+      T* d = static_cast<T*>(dlogits);
+      if (vocab <= (uint32_t)kRowLanes) {
+        const unsigned blocks = (unsigned)((rows + kWarps - 1) / kWarps);
+        backward_rows<T, 32><<<blocks, kThreads, 0, st>>>(x, row_stride, rows, (int)vocab, in, d);
+      } else {
+        backward_rows<T, kThreads><<<dim3((unsigned)rows, row_shares(rows, (int)vocab)), kThreads, 0, st>>>(
+            x, row_stride, rows, (int)vocab, in, d);
+      }
+      mb::launched("token log-probability gradient");
+    });
+  });
+}
+
+}  // extern "C"

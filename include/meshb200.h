@@ -285,6 +285,105 @@ int mb_op_head_ce(const float* h, const float* embeddings, const uint32_t* targe
 int mb_op_adamw(float* weights, float* m, float* v, const float* gradient, size_t count, const mb_adamw* options,
                 uint32_t step, void* stream);
 
+/* ---- serving operators: an 8-bit paged key/value cache, attention over it,
+ * and token log-probabilities (no reference counterpart: the reference
+ * recomputes the whole prefix for every generated token).  Device pointers,
+ * the caller's stream, no host synchronisation and no allocation; arguments
+ * are checked on the host, what only the device sees (page numbers, lengths,
+ * offsets, tokens) in the kernels, which skip what does not fit and set bits
+ * of *d_status (device int, may be NULL): 1 a copy's wait gave up, 2 a page
+ * or token out of range, 4 a length below its new rows or past the table,
+ * 8 offsets outside the rows or more new rows than announced. ---- */
+
+/* Element types of rows, logits and outputs. */
+#define MB_F32 0
+#define MB_BF16 1
+#define MB_F16 2
+
+/* The cache: device arrays k, v [pages][heads][page_tokens][width] of signed
+ * 8-bit codes (16-byte aligned) and k_scale, v_scale [pages][heads]; a stored
+ * value is code * scale.  page_tokens 16, 32, 64 or 128; width = head_dim
+ * (1..128) rounded up to 32.  A page belongs to one sequence. */
+typedef struct mb_kv_cache {
+  int8_t* k;
+  int8_t* v;
+  float* k_scale;
+  float* v_scale;
+  uint32_t pages;
+  uint32_t heads;
+  uint32_t page_tokens;
+  uint32_t width;
+} mb_kv_cache;
+
+/* Where `batch` sequences and their new rows are (device arrays): table
+ * [batch][table_stride], the first table_pages of each row the sequence's
+ * pages in order (entries past its length are not read); lengths [batch], the
+ * tokens of each sequence with its new rows counted in; offsets [batch + 1],
+ * rows offsets[b] .. offsets[b+1] of the packed arrays belong to sequence b
+ * (NULL: row b does, one each). */
+typedef struct mb_cache_rows {
+  const int32_t* table;
+  const int32_t* lengths;
+  const int32_t* offsets;
+  size_t table_stride;
+  size_t rows;
+  uint32_t table_pages;
+  uint32_t batch;
+} mb_cache_rows;
+
+/* Writes the new rows of K and V (row r, head h at element r * row_stride +
+ * h * head_stride, channels adjacent) as the last tokens of their sequences.
+ * Per page and head: scale = the smallest 2^e >= 2^-126 with amax <= 127
+ * scale, code = round-half-even(x / scale).  In a page that holds earlier
+ * tokens the scale never shrinks; where it grows their codes are rounded to
+ * it.  An infinity or NaN makes the page and head's scale NaN until the
+ * page's first token is written again.  max_new: at least the largest number
+ * of new rows of a sequence. */
+int mb_op_cache_write(const mb_kv_cache* cache, const mb_cache_rows* where, uint32_t head_dim, const void* k,
+                      size_t k_row_stride, size_t k_head_stride, const void* v, size_t v_row_stride,
+                      size_t v_head_stride, uint32_t dtype, uint32_t max_new, int* d_status, void* stream);
+/* Reads positions first[b] .. first[b] + tokens - 1 (first NULL: from 0) of
+ * every sequence: k_out, v_out [batch][tokens][heads][head_dim], 0 outside
+ * 0 .. lengths[b] - 1, NaN for a page number out of range.  offsets and rows
+ * are not used. */
+int mb_op_cache_read(const mb_kv_cache* cache, const mb_cache_rows* where, uint32_t head_dim, const int32_t* first,
+                     uint32_t tokens, void* k_out, void* v_out, uint32_t dtype, int* d_status, void* stream);
+/* Attention of the new rows over their sequences' cached tokens (written
+ * before, the new ones too): row i of n of sequence b sees positions
+ * first[b] (NULL: 0) .. lengths[b] - n + i.  Query head a reads key head
+ * a / (q_heads / heads).  out [rows][q_heads][head_dim] in the type of q; lse
+ * [q_heads][rows] (may be NULL), the base-2 log-sum-exp of the scores scaled
+ * by scale * log2(e).  A row that sees nothing gives 0 and -inf; rows of a
+ * sequence whose numbers do not fit, and rows past max_new, NaN.  max_tokens:
+ * about the largest length, by which long sequences are cut over the GPU (any
+ * value is right).  workspace: 16-byte aligned, as many bytes as
+ * mb_op_cache_attention_workspace says for the same sizes. */
+int mb_op_cache_attention_workspace(uint32_t batch, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,
+                                    uint32_t max_new, uint32_t max_tokens, size_t* bytes);
+int mb_op_cache_attention(const mb_kv_cache* cache, const mb_cache_rows* where, const int32_t* first, const void* q,
+                          size_t q_row_stride, size_t q_head_stride, uint32_t q_heads, uint32_t head_dim,
+                          uint32_t dtype, float scale, uint32_t max_new, uint32_t max_tokens, void* out, float* lse,
+                          void* workspace, size_t workspace_bytes, int* d_status, void* stream);
+/* Per row of logits [rows][vocab] (rows row_stride elements apart): logprob =
+ * ln softmax at tokens[row] (0 for -1, MB_IGNORE_TARGET), entropy in nats,
+ * lse = ln sum e^x, and the `top` (0..32) most likely tokens by (logit
+ * descending, index ascending) with their log-probabilities, top_logprob and
+ * top_index [rows][top].  Logits of -inf are masked tokens: probability 0.  A
+ * row with nothing else gives logprob -inf, entropy 0, lse -inf.  A token
+ * out of range gives NaN and status bit 2. */
+int mb_op_token_logprobs(const void* logits, uint32_t dtype, size_t row_stride, size_t rows, uint32_t vocab,
+                         const int32_t* tokens, uint32_t top, float* logprob, float* entropy, float* lse,
+                         float* top_logprob, int32_t* top_index, int* d_status, void* stream);
+/* The gradient of sum(dlogprob . logprob + dentropy . entropy) with respect
+ * to the logits, from the forward's lse and entropy: dlogits [rows][vocab] in
+ * the type of the logits.  dlogprob or dentropy may be NULL (zeros); entropy
+ * may be NULL with dentropy.  Ignored tokens take no part in dlogprob; rows
+ * with nothing but masked tokens get 0. */
+int mb_op_token_logprobs_backward(const void* logits, uint32_t dtype, size_t row_stride, size_t rows, uint32_t vocab,
+                                  const int32_t* tokens, const float* lse, const float* entropy,
+                                  const float* dlogprob, const float* dentropy, void* dlogits, int* d_status,
+                                  void* stream);
+
 /* The same mesh stack backward without any allocation (no reference
  * counterpart: the reference always allocates its workspace).  For callers
  * that must not allocate device memory per call - a service that fixes its
