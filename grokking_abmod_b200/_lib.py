@@ -152,7 +152,8 @@ SIGNATURES = {
     "mb_op_cache_read": (ctypes.c_int, [ctypes.POINTER(KvCacheC), ctypes.POINTER(CacheRowsC), ctypes.c_uint32,
                                         ctypes.c_void_p, ctypes.c_uint32, ctypes.c_void_p, ctypes.c_void_p,
                                         ctypes.c_uint32, ctypes.c_void_p, ctypes.c_void_p]),
-    "mb_op_cache_attention_workspace": (ctypes.c_int, [ctypes.c_uint32] * 6 + [c_size_p]),
+    "mb_op_cache_attention_workspace": (ctypes.c_int, [ctypes.c_uint32, ctypes.c_size_t] + [ctypes.c_uint32] * 5 +
+                                        [c_size_p]),
     "mb_op_cache_attention": (ctypes.c_int, [ctypes.POINTER(KvCacheC), ctypes.POINTER(CacheRowsC), ctypes.c_void_p,
                                              ctypes.c_void_p, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_uint32,
                                              ctypes.c_uint32, ctypes.c_uint32, ctypes.c_float, ctypes.c_uint32,

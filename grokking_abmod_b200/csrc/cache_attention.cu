@@ -454,6 +454,450 @@ __global__ void __launch_bounds__(kSplitThreads)
   }
 }
 
+// ---------------------------------------------------------------- tiles
+// The tile kernel serves rows that are many (prompts): 256 query rows of a key
+// head against tiles of 64 tokens, on the tcgen05 tensor cores.
+//
+//   warps 0-3, 4-7  one query row a thread, rows 0-127 and 128-255: softmax of
+//                   S from tensor memory, P back over it as FP16, O rescaled
+//                   where a maximum has grown
+//   warps 8-11      converters: the tile's codes from global memory (loaded a
+//                   tile ahead), as FP16 into shared memory, once for both halves
+//   warp 12         issues the products: S = Q K^T and O += P V, the halves in
+//                   turn, so one half's products run under the other's softmax
+//
+// Q, S (P over it) and O fill tensor memory, all products take A from there:
+// with A in shared memory its reads alone would take more than the products'
+// time at 64 tokens.  K and V share one layout, rows = tokens: K-major for
+// S, MN-major for O.  Queries and probabilities of FP32 rows are FP16 pairs
+// (two products), those of 16-bit rows one FP16 (bfloat16's 8 bits fit; a
+// probability's rounding to 11 bits is below the output's own).
+//
+// O follows a row's maximum lazily: probabilities up to 2^4 are let through,
+// so that after the first tiles O is hardly ever touched; they carry 2^11,
+// 2^15 in all, inside FP16's range.
+constexpr int kKeys = 64;
+constexpr int kHalfRows = 128;
+constexpr int kTileRows = 2 * kHalfRows;
+constexpr int kTileThreads = 13 * 32;
+constexpr int kConverters = 128;
+constexpr int kStages = 2;
+constexpr float kLazy = 4.f;
+constexpr float kProbScale = 2048.f;
+
+template <int D, int TERMS>
+struct TileShape {
+  // FP32 rows 128 wide: their lo parts do not fit into tensor memory
+  static constexpr bool kLowInSmem = TERMS == 2 && D == 128;
+  static constexpr int kQ = kLowInSmem ? D / 2 : TERMS * D / 2;  // columns of a half's Q
+  static constexpr int kS = 2 * kQ;
+  static constexpr int kO = kS + 2 * kKeys;
+  static_assert(kO + 2 * D <= 512, "tensor memory");
+  static constexpr int kOperand = kKeys * D * 2;  // bytes of a K or V tile
+  static constexpr int kLow = kStages * 2 * kOperand;
+  static constexpr int kMeta = kLow + (kLowInSmem ? 2 * kHalfRows * D * 2 : 0);
+  static constexpr int kBars = kMeta + kStages * 32;
+  static constexpr int kBytes = kBars + 128;
+};
+
+// 64 columns of this thread's lane.
+__device__ __forceinline__ void tmem_ld64(uint32_t at, float (&v)[64]) {
+  tc::tmem_ld32(at, v);
+  tc::tmem_ld32(at + 32, v + 32);
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(kTileThreads, 1)
+    attend_tiles(View c, Batch t, Queries q, Partials part, int blocks_per_seq) {
+  constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
+  using S = TileShape<D, TERMS>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int chunk = blockIdx.x % part.chunks, head = blockIdx.y;
+  // the last rows see the most: they go first
+  const int block = blockIdx.x / part.chunks;
+  const int z = block / blocks_per_seq * blocks_per_seq + (blocks_per_seq - 1 - block % blocks_per_seq);
+  const Unit u = unit_of<kTileRows>(c, t, q, z, blocks_per_seq);
+  if (u.bad) {
+    if (chunk == 0 && z % blocks_per_seq == 0) {
+      refuse_rows<T>(t, q, head, u, 0, kTileThreads);
+      if (q.status && threadIdx.x == 0) atomicOr(q.status, span_of(t, c, u.b).flags);
+    }
+    return;
+  }
+  if (z % blocks_per_seq == blocks_per_seq - 1 && chunk == 0 && (long long)u.fresh * q.group > u.row0 + kTileRows) {
+    refuse_rows<T>(t, q, head, u, u.row0 + kTileRows, kTileThreads);
+    if (q.status && threadIdx.x == 0) atomicOr(q.status, kBadRows);
+  }
+  if (u.rows <= 0) return;
+
+  const int old = u.length - u.fresh;
+  // tiles of both halves, counted from the tile that holds the first visible position
+  const int tile_lo = u.lo / kKeys;
+  auto tiles_to = [&](int last_row) {
+    const int hi = old + (u.row0 + last_row) / q.group + 1;
+    return hi > u.lo ? (hi + kKeys - 1) / kKeys : tile_lo;
+  };
+  const bool both = u.rows > kHalfRows;
+  const int end1 = tiles_to(u.rows - 1), end0 = both ? tiles_to(kHalfRows - 1) : end1;
+  const int begin = (int)min((long long)end1, tile_lo + (long long)chunk * part.chunk_tiles);
+  const int end = chunk == part.chunks - 1 ? end1 : min(end1, begin + part.chunk_tiles);
+  // half h takes tiles begin .. begin + count[h]; the first half never more than the second
+  const int count1 = end - begin, count0 = max(0, min(end0, end) - begin);
+  const size_t slot = ((size_t)z * c.heads + head) * part.chunks + chunk;
+
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
+  uint64_t* kv_full = bars;               // [stage] converters -> products and softmax
+  uint64_t* kv_free = bars + kStages;     // [stage] products -> converters
+  uint64_t* s_full = bars + 2 * kStages;  // [half] products -> softmax
+  uint64_t* p_full = s_full + 2;          // [half] softmax (and Q, once) -> products
+  uint64_t* drained = p_full + 2;
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drained + 1);
+  int* failed = reinterpret_cast<int*>(tmem_at + 1);
+  float* meta = reinterpret_cast<float*>(smem + S::kMeta);  // [stage][4 K scales, 4 V scales] of 16 tokens each
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      tc::bar_init(&kv_full[s], kConverters);
+      tc::bar_init(&kv_free[s], 1);
+    }
+    for (int h = 0; h < 2; ++h) {
+      tc::bar_init(&s_full[h], 1);
+      tc::bar_init(&p_full[h], kHalfRows);
+    }
+    tc::bar_init(drained, 1);
+    *failed = 0;
+  }
+  tc::bar_init_fence();
+  if (warp == 12) tc::tmem_alloc(tmem_at, 512);
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = *tmem_at;
+
+  if (warp < 8) {
+    const int h = warp >> 2;
+    const int count = h ? (both ? count1 : 0) : (both ? count0 : count1);
+    const int r = h * kHalfRows + (warp & 3) * 32 + lane;  // row of the unit
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t at_q = lanes + h * S::kQ, at_s = lanes + S::kS + h * kKeys, at_o = lanes + S::kO + h * D;
+    const bool there = r < u.rows;
+    const int tok = (u.row0 + r) / q.group, a = head * q.group + (u.row0 + r) % q.group;
+    const int limit = there ? old + tok : -1;
+    // the last position that every row of the warp sees
+    const int sure = old + (u.row0 + (r - lane)) / q.group;
+    float factor = 0.f;
+    float m = -INFINITY, l = 0.f;
+    int ev = -126;
+    bool alive = true;
+    if (count > 0) {
+      const T* src = static_cast<const T*>(q.q) + (u.first_row + tok) * q.row_stride + (size_t)a * q.head_stride;
+      float most = 0.f;
+      if (there)
+        for (int ch = 0; ch < q.head_dim; ++ch) most = fmaxf(most, fabsf(Element<T>::to(src[ch])));
+      const float up = tc::f16_scale(most);
+      factor = q.scale_log2 / up;
+      const float sign = factor < 0.f ? -up : up;  // scores are q.k times a factor that is not negative
+      factor = fabsf(factor);
+#pragma unroll
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t hi[16], lo[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int ch = c0 + 2 * i;
+          const float x = there && ch < q.head_dim ? Element<T>::to(src[ch]) * sign : 0.f;
+          const float y = there && ch + 1 < q.head_dim ? Element<T>::to(src[ch + 1]) * sign : 0.f;
+          tc::split_f16x2(x, y, hi[i], lo[i]);
+        }
+        __syncwarp();
+        tc::tmem_st16u(at_q + c0 / 2, hi);
+        if constexpr (S::kLowInSmem) {
+          __half* low = reinterpret_cast<__half*>(smem + S::kLow) + h * kHalfRows * D;
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<uint4*>(low + tc::blk16(r & (kHalfRows - 1), c0 + 2 * i, D)) =
+                make_uint4(lo[i], lo[i + 1], lo[i + 2], lo[i + 3]);
+        } else if constexpr (TERMS == 2) {
+          tc::tmem_st16u(at_q + D / 2 + c0 / 2, lo);
+        }
+      }
+      tc::tmem_st_wait();
+      tc::fence_async_smem();
+      tc::fence_before_sync();
+      tc::bar_arrive(&p_full[h]);
+    }
+    for (int j = 0; j < count; ++j) {
+      const int stage = j % kStages;
+      // both: the tile's scales (converters) and its scores (products)
+      alive = tc::bar_wait(&kv_full[stage], (j / kStages) & 1) && tc::bar_wait(&s_full[h], j & 1);
+      if (!__all_sync(kFull, alive)) {
+        alive = false;
+        break;
+      }
+      tc::fence_after_sync();
+      float x[kKeys];
+      tmem_ld64(at_s, x);
+      const float4 ks = *reinterpret_cast<const float4*>(meta + stage * 8);
+      const float4 vs = *reinterpret_cast<const float4*>(meta + stage * 8 + 4);
+      // not 0, so that a masked score stays -inf; NaN stays
+      float fk[4] = {ks.x * factor, ks.y * factor, ks.z * factor, ks.w * factor};
+#pragma unroll
+      for (int g = 0; g < 4; ++g) fk[g] = fk[g] < 2e-38f ? 2e-38f : fk[g];
+      const float sv[4] = {vs.x, vs.y, vs.z, vs.w};
+      const int pos = (begin + j) * kKeys;
+      if (pos < u.lo || pos + kKeys - 1 > sure) {
+#pragma unroll
+        for (int i = 0; i < kKeys; ++i)
+          if (pos + i < u.lo || pos + i > limit) x[i] = -INFINITY;
+      }
+      float mx = m;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float a0 = x[16 * g], a1 = x[16 * g + 1];
+#pragma unroll
+        for (int i = 2; i < 16; i += 2) {
+          a0 = fmaxf(a0, x[16 * g + i]);
+          a1 = fmaxf(a1, x[16 * g + i + 1]);
+        }
+        a0 = fmaxf(a0, a1);
+        mx = fmaxf(mx, a0 * fk[g]);
+      }
+      int top = ev;
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        if (sv[g] == sv[g]) top = max(top, exponent_of(sv[g]));
+      if (__any_sync(kFull, mx > m + kLazy || top != ev)) {
+        const float shrink = ex2_ftz(m - (mx == -INFINITY ? 0.f : mx));
+        l *= shrink;
+        const float change = shrink * (top != ev ? power_of_two(max(ev - top, -126)) : 1.f);
+        m = mx;
+        ev = top;
+        if (j > 0) {
+#pragma unroll
+          for (int c0 = 0; c0 < D; c0 += 16) {
+            float o[16];
+            tc::tmem_ld16(at_o + c0, o);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] *= change;
+            tc::tmem_st16(at_o + c0, o);
+          }
+        }
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+      const float2 nbase = splat2(-base);
+      const float unit = power_of_two(-ev);
+      float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t hi[16], lo[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int e = 32 * half + 2 * i, g = e / 16;
+          const float2 y = fma2(make_float2(x[e], x[e + 1]), splat2(fk[g]), nbase);
+          const float2 p = make_float2(ex2_ftz(y.x), ex2_ftz(y.y));
+          sum = add2(sum, p);
+          const float2 w = mul2(p, splat2(sv[g] * unit * kProbScale));
+          if constexpr (TERMS == 2) {
+            tc::split_f16x2(w.x, w.y, hi[i], lo[i]);
+          } else {
+            const __half2 v = __floats2half2_rn(w.x, w.y);
+            hi[i] = *reinterpret_cast<const uint32_t*>(&v);
+          }
+        }
+        tc::tmem_st16u(at_s + 16 * half, hi);
+        if constexpr (TERMS == 2) tc::tmem_st16u(at_s + 32 + 16 * half, lo);
+      }
+      l += sum.x + sum.y;
+      tc::tmem_st_wait();
+      tc::fence_before_sync();
+      tc::bar_arrive(&p_full[h]);
+    }
+    if (count > 0 && alive) alive = __all_sync(kFull, tc::bar_wait(&s_full[h], count & 1));
+    if (!alive) *failed = 1;
+    tc::fence_after_sync();
+    const float inverse = l == 0.f ? 0.f : power_of_two(ev) * (1.f / kProbScale) / l;
+    float lse = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) + log2f(l);
+    if (!alive) lse = NAN;
+    const size_t row = u.first_row + tok;
+    T* out = static_cast<T*>(q.out) + (row * q.heads + a) * q.head_dim;
+    float* po = part.o + (slot * kTileRows + r) * D;
+    const bool wide = q.head_dim % Element<T>::kVec == 0 && (reinterpret_cast<uintptr_t>(q.out) & 15) == 0;
+    if (there) {
+      if (part.chunks > 1) part.lse[slot * kTileRows + r] = lse;
+      else if (q.lse) q.lse[(size_t)a * t.rows + row] = lse;
+    }
+#pragma unroll
+    for (int c0 = 0; c0 < D; c0 += 16) {
+      float o[16];
+      if (count > 0) tc::tmem_ld16(at_o + c0, o);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[i] = !alive ? NAN : l == 0.f ? 0.f : o[i] * inverse;
+      if (!there) {
+      } else if (part.chunks > 1) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          *reinterpret_cast<float4*>(po + c0 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+      } else if (wide) {
+#pragma unroll
+        for (int i = 0; i < 16; i += Element<T>::kVec)
+          if (c0 + i < q.head_dim) *reinterpret_cast<uint4*>(out + c0 + i) = Element<T>::pack(o + i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (c0 + i < q.head_dim) out[c0 + i] = Element<T>::from(o[i]);
+      }
+      __syncwarp();  // tensor memory is read by whole warps
+    }
+  } else if (warp < 12) {
+    // 16 codes a piece; 8 lanes take one piece column of 8 rows, whose FP16
+    // chunks are 128 contiguous bytes each
+    constexpr int PIECES = D / 32;  // of K and of V, a thread and tile
+    const int ct = threadIdx.x - 8 * 32;
+    uint4 kq[PIECES], vq[PIECES];
+    float sk = 0.f, sv = 0.f;
+    auto load = [&](int j) {
+      const int pos = (begin + j) * kKeys;
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const int idx = ct + kConverters * i;
+        const int row = idx / (8 * (D / 16)) * 8 + (idx & 7), at = (idx >> 3) % (D / 16) * 16;
+        kq[i] = vq[i] = make_uint4(0u, 0u, 0u, 0u);
+        const int first_of_page = (pos + row) & ~(c.tokens - 1);
+        // pages that no row sees are not looked up: their tokens are masked, as zeros
+        if (first_of_page < u.hi && first_of_page + c.tokens > u.lo) {
+          const int page = page_of(t, c, u.b, (pos + row) >> c.shift);
+          if (page >= 0) {
+            const size_t from = c.row(page, head, (pos + row) & (c.tokens - 1)) + at;
+            kq[i] = __ldg(reinterpret_cast<const uint4*>(c.k + from));
+            vq[i] = __ldg(reinterpret_cast<const uint4*>(c.v + from));
+          }
+        }
+      }
+      if (ct < 4) {
+        sk = sv = 0.f;
+        const int first_of_page = (pos + 16 * ct) & ~(c.tokens - 1);
+        if (first_of_page < u.hi && first_of_page + c.tokens > u.lo) {
+          const int page = page_of(t, c, u.b, (pos + 16 * ct) >> c.shift);
+          if (page < 0 && q.status) atomicOr(q.status, kBadPage);
+          sk = page < 0 ? NAN : __ldg(c.k_scale + c.scale_at(page, head));
+          sv = page < 0 ? NAN : __ldg(c.v_scale + c.scale_at(page, head));
+        }
+      }
+    };
+    auto store = [&](uint8_t* tile, const uint4 (&codes)[PIECES]) {
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const int idx = ct + kConverters * i;
+        const int row = idx / (8 * (D / 16)) * 8 + (idx & 7), at = (idx >> 3) % (D / 16) * 16;
+        const uint32_t w[4] = {codes[i].x ^ 0x80808080u, codes[i].y ^ 0x80808080u, codes[i].z ^ 0x80808080u,
+                               codes[i].w ^ 0x80808080u};
+        __half* to = reinterpret_cast<__half*>(tile) + tc::blk16(row, at, D);
+        *reinterpret_cast<uint4*>(to) = make_uint4(codes_to_f16(w[0], 0x4140), codes_to_f16(w[0], 0x4342),
+                                                   codes_to_f16(w[1], 0x4140), codes_to_f16(w[1], 0x4342));
+        *reinterpret_cast<uint4*>(to + 64) = make_uint4(codes_to_f16(w[2], 0x4140), codes_to_f16(w[2], 0x4342),
+                                                        codes_to_f16(w[3], 0x4140), codes_to_f16(w[3], 0x4342));
+      }
+    };
+    if (count1 > 0) load(0);
+    for (int j = 0; j < count1; ++j) {
+      const int stage = j % kStages;
+      if (j >= kStages && !tc::bar_wait(&kv_free[stage], (j / kStages - 1) & 1)) {
+        *failed = 1;
+        break;
+      }
+      uint8_t* tile = smem + stage * 2 * S::kOperand;
+      store(tile, kq);
+      store(tile + S::kOperand, vq);
+      if (ct < 4) {
+        meta[stage * 8 + ct] = sk;
+        meta[stage * 8 + 4 + ct] = sv;
+      }
+      tc::fence_async_smem();
+      tc::bar_arrive(&kv_full[stage]);
+      if (j + 1 < count1) load(j + 1);
+    }
+  } else if (lane == 0) {
+    constexpr uint32_t kIdS = tc::idesc_f16(128, kKeys), kIdO = tc::idesc_f16(128, D, true);
+    const int counts[2] = {both ? count0 : count1, both ? count1 : 0};
+    auto scores = [&](int h, int j) {
+      const uint8_t* k = smem + (j % kStages) * 2 * S::kOperand;
+      const uint32_t to = tmem + S::kS + h * kKeys;
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s)
+        tc::mma_ts_f16(to, tmem + h * S::kQ + 8 * s, tc::desc_kmajor16(k, D, s), kIdS, s > 0);
+      if constexpr (TERMS == 2) {
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+          if constexpr (S::kLowInSmem) {
+            const uint8_t* low = smem + S::kLow + h * kHalfRows * D * 2;
+            tc::mma_ss_f16(to, tc::desc_kmajor16(low, D, s), tc::desc_kmajor16(k, D, s), kIdS, 1);
+          } else {
+            tc::mma_ts_f16(to, tmem + h * S::kQ + D / 2 + 8 * s, tc::desc_kmajor16(k, D, s), kIdS, 1);
+          }
+        }
+      }
+    };
+    auto values = [&](int h, int j) {
+      const uint8_t* v = smem + (j % kStages) * 2 * S::kOperand + S::kOperand;
+      const uint32_t to = tmem + S::kO + h * D, p = tmem + S::kS + h * kKeys;
+#pragma unroll
+      for (int s = 0; s < kKeys / 16; ++s)
+        tc::mma_ts_f16(to, p + 8 * s, tc::desc_mn16(v, D, s), kIdO, j > 0 || s > 0);
+      if constexpr (TERMS == 2) {
+#pragma unroll
+        for (int s = 0; s < kKeys / 16; ++s) tc::mma_ts_f16(to, p + 32 + 8 * s, tc::desc_mn16(v, D, s), kIdO, 1);
+      }
+    };
+    bool ok = true;
+    int arrived[2] = {0, 0};  // phases of p_full waited for
+    auto wait_p = [&](int h) { return tc::bar_wait(&p_full[h], arrived[h]++ & 1); };
+    if (count1 > 0) {
+      ok = tc::bar_wait(&kv_full[0], 0);
+      for (int h = 0; h < 2 && ok; ++h)
+        if (counts[h] > 0) {
+          ok = wait_p(h);  // Q is in place
+          if (!ok) break;
+          tc::fence_after_sync();
+          scores(h, 0);
+          tc::commit(&s_full[h]);
+        }
+    }
+    for (int j = 0; j < count1 && ok; ++j) {
+      // the second half may go on after the first has ended
+      bool next = false;
+      for (int h = 0; h < 2 && ok; ++h) {
+        if (j < counts[h]) {
+          ok = wait_p(h);
+          if (!ok) break;
+          tc::fence_after_sync();
+          values(h, j);
+        }
+        if (h == 1 || !both) tc::commit(&kv_free[j % kStages]);
+        if (j + 1 < counts[h]) {
+          if (!next) ok = tc::bar_wait(&kv_full[(j + 1) % kStages], ((j + 1) / kStages) & 1);
+          next = true;
+          if (!ok) break;
+          tc::fence_after_sync();
+          scores(h, j + 1);
+        }
+        if (j < counts[h]) tc::commit(&s_full[h]);
+        if (!both) break;
+      }
+    }
+    if (!ok) *failed = 1;
+    // nothing is in flight when tensor memory is given back
+    tc::commit(drained);
+    if (!tc::bar_wait(drained, 0)) *failed = 1;
+  }
+  __syncwarp();
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 12) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem, 512);
+  }
+  if (threadIdx.x == 0 && *failed && q.status) atomicOr(q.status, kGaveUp);
+}
+
 // Joins the chunks of a unit's rows: one warp a row.
 template <class T, int D, int ROWS>
 __global__ void __launch_bounds__(256)
@@ -503,45 +947,55 @@ inline int sm_count() {
 }
 
 struct Plan {
+  bool tiles;          // the tile kernel, else the split kernel
   int blocks_per_seq;  // row blocks of a sequence
   size_t units;        // sequences times row blocks
   int chunks, chunk_tiles;
   size_t workspace;    // bytes
 };
 
-inline Plan make_plan(size_t batch, uint32_t kv_heads, uint32_t group, uint32_t width, uint32_t max_new,
+// More than 16 rows a sequence and key head on average go to the tile kernel.
+constexpr size_t kSplitMost = 16;
+
+inline Plan make_plan(size_t batch, size_t rows, uint32_t kv_heads, uint32_t group, uint32_t width, uint32_t max_new,
                       uint32_t max_tokens) {
   Plan p;
-  const size_t rows = (size_t)max_new * group;
-  require(rows <= (1u << 30), "too many new rows for one call");
-  p.blocks_per_seq = (int)((rows + kSplitRows - 1) / kSplitRows);
+  const size_t most_rows = (size_t)max_new * group;
+  require(most_rows <= (1u << 30), "too many new rows for one call");
+  p.tiles = rows * group > kSplitMost * batch;
+  const size_t unit_rows = p.tiles ? kTileRows : kSplitRows, keys = p.tiles ? kKeys : kTile;
+  p.blocks_per_seq = (int)((most_rows + unit_rows - 1) / unit_rows);
   p.units = batch * p.blocks_per_seq;
-  // Chunks for about three CTAs on every SM, none shorter than two tiles a warp.
-  const size_t want = (size_t)sm_count() * 3, have = std::max<size_t>(1, p.units * kv_heads);
-  const size_t tiles = std::max<size_t>(1, ((size_t)max_tokens + kTile - 1) / kTile);
-  const size_t most = (tiles + 2 * kSplitWarps - 1) / (2 * kSplitWarps);
-  const size_t chunks = std::max<size_t>(1, std::min(most, want / have));
+  // Chunks for one (tiles) or about three (split) CTAs on every SM, none
+  // shorter than eight tiles: two a warp of the split kernel.
+  const size_t want = (size_t)sm_count() * (p.tiles ? 1 : 3), have = std::max<size_t>(1, p.units * kv_heads);
+  const size_t tiles = std::max<size_t>(1, ((size_t)max_tokens + keys - 1) / keys);
+  const size_t chunks = std::max<size_t>(1, std::min((tiles + 7) / 8, want / have));
   p.chunk_tiles = (int)((tiles + chunks - 1) / chunks + kSplitWarps - 1) / kSplitWarps * kSplitWarps;
   p.chunks = (int)((tiles + p.chunk_tiles - 1) / p.chunk_tiles);
-  p.workspace = p.chunks > 1 ? p.units * kv_heads * p.chunks * kSplitRows * (width + 1) * sizeof(float) : 0;
+  p.workspace = p.chunks > 1 ? p.units * kv_heads * p.chunks * unit_rows * (width + 1) * sizeof(float) : 0;
   return p;
 }
 
-template <class T, int D>
-void launch_split(const View& c, const Batch& t, const Queries& q, const Plan& p, void* workspace, cudaStream_t st) {
+template <class T, int D, int ROWS>
+void launch_rows(const View& c, const Batch& t, const Queries& q, const Plan& p, void* workspace, cudaStream_t st) {
+  constexpr bool TILES = ROWS == kTileRows;
   const size_t slots = p.units * c.heads * p.chunks;
-  const Partials part{static_cast<float*>(workspace), static_cast<float*>(workspace) + slots * kSplitRows, p.chunks,
-                      p.chunk_tiles};
-  constexpr int bytes = SplitSmem<D>::kBytes;
-  auto kernel = attend_split<T, D>;
+  // outputs first: their vectors need the workspace's alignment
+  float* o = static_cast<float*>(workspace);
+  const Partials part{o + slots * ROWS * D, o, p.chunks, p.chunk_tiles};
+  constexpr int bytes = TILES ? TileShape<D, sizeof(T) == 4 ? 2 : 1>::kBytes : SplitSmem<D>::kBytes;
+  void (*kernel)(View, Batch, Queries, Partials, int);
+  if constexpr (TILES) kernel = attend_tiles<T, D>;
+  else kernel = attend_split<T, D>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   require(e == cudaSuccess, std::string("cache attention: ") + cudaGetErrorString(e), MB_ERR_CUDA);
-  kernel<<<dim3((unsigned)(p.units * p.chunks), (unsigned)c.heads), kSplitThreads, bytes, st>>>(
+  kernel<<<dim3((unsigned)(p.units * p.chunks), (unsigned)c.heads), TILES ? kTileThreads : kSplitThreads, bytes, st>>>(
       c, t, q, part, p.blocks_per_seq);
   launched("cache attention");
   if (p.chunks == 1) return;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)p.units, (unsigned)c.heads);
+  cfg.gridDim = dim3((unsigned)p.units, (unsigned)c.heads, ROWS / 8);
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
@@ -549,8 +1003,14 @@ void launch_split(const View& c, const Batch& t, const Queries& q, const Plan& p
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, join_chunks<T, D, kSplitRows>, c, t, q, part, p.blocks_per_seq);
+  e = cudaLaunchKernelEx(&cfg, join_chunks<T, D, ROWS>, c, t, q, part, p.blocks_per_seq);
   require(e == cudaSuccess, std::string("cache attention join: ") + cudaGetErrorString(e), MB_ERR_CUDA);
+}
+
+template <class T, int D>
+void launch(const View& c, const Batch& t, const Queries& q, const Plan& p, void* workspace, cudaStream_t st) {
+  if (p.tiles) launch_rows<T, D, kTileRows>(c, t, q, p, workspace, st);
+  else launch_rows<T, D, kSplitRows>(c, t, q, p, workspace, st);
 }
 
 }  // namespace cache
@@ -558,13 +1018,14 @@ void launch_split(const View& c, const Batch& t, const Queries& q, const Plan& p
 
 extern "C" {
 
-int mb_op_cache_attention_workspace(uint32_t batch, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,
+int mb_op_cache_attention_workspace(uint32_t batch, size_t rows, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,
                                     uint32_t max_new, uint32_t max_tokens, size_t* bytes) {
   using namespace mb::cache;
   return mb::guarded([&] {
     mb::need(bytes, "bytes");
     mb::require(kv_heads >= 1 && q_heads >= 1 && q_heads % kv_heads == 0, "kv_heads must divide q_heads");
-    *bytes = make_plan(batch, kv_heads, q_heads / kv_heads, (head_dim + 31) / 32 * 32, max_new, max_tokens).workspace;
+    *bytes = batch == 0 ? 0 : make_plan(batch, rows, kv_heads, q_heads / kv_heads, (head_dim + 31) / 32 * 32, max_new, max_tokens)
+                                 .workspace;
   });
 }
 
@@ -586,7 +1047,7 @@ int mb_op_cache_attention(const mb_kv_cache* cache, const mb_cache_rows* where, 
     mb::need(out, "out");
     const Queries qs{q, q_row_stride, q_head_stride, out, lse, (int)q_heads, (int)(q_heads / c.heads), (int)head_dim,
                      scale * mb::kLog2e, first, (int)max_new, d_status};
-    const Plan p = make_plan(t.count, c.heads, qs.group, c.width, max_new, max_tokens);
+    const Plan p = make_plan(t.count, t.rows, c.heads, qs.group, c.width, max_new, max_tokens);
     mb::require(p.units * p.chunks <= (size_t)INT_MAX, "too many row blocks for one call");
     mb::require(p.workspace == 0 || (workspace != nullptr && workspace_bytes >= p.workspace &&
                                      reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
@@ -597,10 +1058,10 @@ int mb_op_cache_attention(const mb_kv_cache* cache, const mb_cache_rows* where, 
       for (const void* x : {q, (const void*)out})
         mb::require(reinterpret_cast<uintptr_t>(x) % sizeof(T) == 0, "q and out must be aligned to their elements");
       switch (c.width) {
-        case 32: return launch_split<T, 32>(c, t, qs, p, workspace, st);
-        case 64: return launch_split<T, 64>(c, t, qs, p, workspace, st);
-        case 96: return launch_split<T, 96>(c, t, qs, p, workspace, st);
-        default: return launch_split<T, 128>(c, t, qs, p, workspace, st);
+        case 32: return launch<T, 32>(c, t, qs, p, workspace, st);
+        case 64: return launch<T, 64>(c, t, qs, p, workspace, st);
+        case 96: return launch<T, 96>(c, t, qs, p, workspace, st);
+        default: return launch<T, 128>(c, t, qs, p, workspace, st);
       }
     });
   });

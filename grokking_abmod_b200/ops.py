@@ -388,7 +388,7 @@ def cache_attention(q, cache: KvCache, table, lengths, offsets=None, *, first=No
     out = torch.empty((rows, heads, head_dim), dtype=q.dtype, device=q.device)
     lse = torch.empty((heads, rows), dtype=torch.float32, device=q.device)
     size = ctypes.c_size_t()
-    check(lib.mb_op_cache_attention_workspace(w.batch, heads, c.heads, head_dim, max_new, max_tokens,
+    check(lib.mb_op_cache_attention_workspace(w.batch, rows, heads, c.heads, head_dim, max_new, max_tokens,
                                               ctypes.byref(size)))
     work = torch.empty(size.value, dtype=torch.uint8, device=q.device) if size.value else None
     check(lib.mb_op_cache_attention(

@@ -358,8 +358,8 @@ int mb_op_cache_read(const mb_kv_cache* cache, const mb_cache_rows* where, uint3
  * about the largest length, by which long sequences are cut over the GPU (any
  * value is right).  workspace: 16-byte aligned, as many bytes as
  * mb_op_cache_attention_workspace says for the same sizes. */
-int mb_op_cache_attention_workspace(uint32_t batch, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,
-                                    uint32_t max_new, uint32_t max_tokens, size_t* bytes);
+int mb_op_cache_attention_workspace(uint32_t batch, size_t rows, uint32_t q_heads, uint32_t kv_heads,
+                                    uint32_t head_dim, uint32_t max_new, uint32_t max_tokens, size_t* bytes);
 int mb_op_cache_attention(const mb_kv_cache* cache, const mb_cache_rows* where, const int32_t* first, const void* q,
                           size_t q_row_stride, size_t q_head_stride, uint32_t q_heads, uint32_t head_dim,
                           uint32_t dtype, float scale, uint32_t max_new, uint32_t max_tokens, void* out, float* lse,
