@@ -463,8 +463,8 @@ __global__ void __launch_bounds__(kSplitThreads)
 //                   where a maximum has grown
 //   warps 8-11      converters: the tile's codes from global memory (loaded a
 //                   tile ahead), as FP16 into shared memory, once for both halves
-//   warp 12         issues the products: S = Q K^T and O += P V, the halves in
-//                   turn, so one half's products run under the other's softmax
+//   warps 12, 13    issue the products of a half each, S = Q K^T and O += P V:
+//                   one half's products run under the other's softmax
 //
 // Q, S (P over it) and O fill tensor memory, all products take A from there:
 // with A in shared memory its reads alone would take more than the products'
@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(kSplitThreads)
 constexpr int kKeys = 64;
 constexpr int kHalfRows = 128;
 constexpr int kTileRows = 2 * kHalfRows;
-constexpr int kTileThreads = 13 * 32;
+constexpr int kTileThreads = 14 * 32;
 constexpr int kConverters = 128;
 constexpr int kStages = 2;
 constexpr float kLazy = 4.f;
@@ -499,6 +499,20 @@ struct TileShape {
   static constexpr int kBars = kMeta + kStages * 32;
   static constexpr int kBytes = kBars + 128;
 };
+
+// D (tensor memory) (+)= A (tensor memory, or shared memory) * B (shared memory), FP16.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add));
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add));
+}
 
 // 64 columns of this thread's lane.
 __device__ __forceinline__ void tmem_ld64(uint32_t at, float (&v)[64]) {
@@ -551,20 +565,20 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* kv_free = bars + kStages;     // [stage] products -> converters
   uint64_t* s_full = bars + 2 * kStages;  // [half] products -> softmax
   uint64_t* p_full = s_full + 2;          // [half] softmax (and Q, once) -> products
-  uint64_t* drained = p_full + 2;
-  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drained + 1);
+  uint64_t* drained = p_full + 2;         // [half]
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drained + 2);
   int* failed = reinterpret_cast<int*>(tmem_at + 1);
   float* meta = reinterpret_cast<float*>(smem + S::kMeta);  // [stage][4 K scales, 4 V scales] of 16 tokens each
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       tc::bar_init(&kv_full[s], kConverters);
-      tc::bar_init(&kv_free[s], 1);
+      tc::bar_init(&kv_free[s], both ? 2 : 1);
     }
     for (int h = 0; h < 2; ++h) {
       tc::bar_init(&s_full[h], 1);
       tc::bar_init(&p_full[h], kHalfRows);
+      tc::bar_init(&drained[h], 1);
     }
-    tc::bar_init(drained, 1);
     *failed = 0;
   }
   tc::bar_init_fence();
@@ -591,23 +605,39 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     bool alive = true;
     if (count > 0) {
       const T* src = static_cast<const T*>(q.q) + (u.first_row + tok) * q.row_stride + (size_t)a * q.head_stride;
+      // 16-byte loads where every row is aligned for them
+      const bool vector = ((reinterpret_cast<uintptr_t>(q.q) | q.row_stride * sizeof(T) | q.head_stride * sizeof(T)) & 15) == 0 &&
+                          q.head_dim % Element<T>::kVec == 0;
+      auto chunk = [&](int c0, float (&x)[32]) {  // channels [c0, c0 + 32)
+        if (vector) {
+#pragma unroll
+          for (int i = 0; i < 32; i += Element<T>::kVec)
+            Element<T>::unpack(there && c0 + i < q.head_dim ? __ldg(reinterpret_cast<const uint4*>(src + c0 + i))
+                                                            : make_uint4(0u, 0u, 0u, 0u), x + i);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[i] = there && c0 + i < q.head_dim ? Element<T>::to(src[c0 + i]) : 0.f;
+        }
+      };
       float most = 0.f;
-      if (there)
-        for (int ch = 0; ch < q.head_dim; ++ch) most = fmaxf(most, fabsf(Element<T>::to(src[ch])));
+#pragma unroll
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        float x[32];
+        chunk(c0, x);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) most = fmaxf(most, fabsf(x[i]));
+      }
       const float up = tc::f16_scale(most);
       factor = q.scale_log2 / up;
       const float sign = factor < 0.f ? -up : up;  // scores are q.k times a factor that is not negative
       factor = fabsf(factor);
 #pragma unroll
       for (int c0 = 0; c0 < D; c0 += 32) {
+        float x[32];
+        chunk(c0, x);
         uint32_t hi[16], lo[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int ch = c0 + 2 * i;
-          const float x = there && ch < q.head_dim ? Element<T>::to(src[ch]) * sign : 0.f;
-          const float y = there && ch + 1 < q.head_dim ? Element<T>::to(src[ch + 1]) * sign : 0.f;
-          tc::split_f16x2(x, y, hi[i], lo[i]);
-        }
+        for (int i = 0; i < 16; ++i) tc::split_f16x2(x[2 * i] * sign, x[2 * i + 1] * sign, hi[i], lo[i]);
         __syncwarp();
         tc::tmem_st16u(at_q + c0 / 2, hi);
         if constexpr (S::kLowInSmem) {
@@ -816,77 +846,68 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if (j + 1 < count1) load(j + 1);
     }
   } else if (lane == 0) {
+    // Issuer of one half.  Descriptors are a base and constant steps: the
+    // fewer instructions between two products, the closer their issue gets
+    // to the tensor pipe's rate.
+    const int h = warp - 12;
+    const int count = h ? (both ? count1 : 0) : (both ? count0 : count1);
     constexpr uint32_t kIdS = tc::idesc_f16(128, kKeys), kIdO = tc::idesc_f16(128, D, true);
-    const int counts[2] = {both ? count0 : count1, both ? count1 : 0};
-    auto scores = [&](int h, int j) {
-      const uint8_t* k = smem + (j % kStages) * 2 * S::kOperand;
-      const uint32_t to = tmem + S::kS + h * kKeys;
+    const uint32_t at_q = tmem + h * S::kQ, at_s = tmem + S::kS + h * kKeys, at_o = tmem + S::kO + h * D;
+    const uint64_t k0 = tc::desc_kmajor16(smem, D, 0), v0 = tc::desc_mn16(smem + S::kOperand, D, 0);
+    const uint64_t low0 = tc::desc_kmajor16(smem + S::kLow + h * kHalfRows * D * 2, D, 0);
+    constexpr uint64_t kStep = 256 >> 4, vStep = D / 8 * 256 >> 4, kStage = 2 * S::kOperand >> 4;
+    auto scores = [&](int j) {
+      const uint64_t k = k0 + (j % kStages) * kStage;
 #pragma unroll
-      for (int s = 0; s < D / 16; ++s)
-        tc::mma_ts_f16(to, tmem + h * S::kQ + 8 * s, tc::desc_kmajor16(k, D, s), kIdS, s > 0);
+      for (int s = 0; s < D / 16; ++s) mma_ts(at_s, at_q + 8 * s, k + s * kStep, kIdS, s > 0);
       if constexpr (TERMS == 2) {
 #pragma unroll
         for (int s = 0; s < D / 16; ++s) {
-          if constexpr (S::kLowInSmem) {
-            const uint8_t* low = smem + S::kLow + h * kHalfRows * D * 2;
-            tc::mma_ss_f16(to, tc::desc_kmajor16(low, D, s), tc::desc_kmajor16(k, D, s), kIdS, 1);
-          } else {
-            tc::mma_ts_f16(to, tmem + h * S::kQ + D / 2 + 8 * s, tc::desc_kmajor16(k, D, s), kIdS, 1);
-          }
+          if constexpr (S::kLowInSmem) mma_ss(at_s, low0 + s * kStep, k + s * kStep, kIdS, true);
+          else mma_ts(at_s, at_q + D / 2 + 8 * s, k + s * kStep, kIdS, true);
         }
       }
     };
-    auto values = [&](int h, int j) {
-      const uint8_t* v = smem + (j % kStages) * 2 * S::kOperand + S::kOperand;
-      const uint32_t to = tmem + S::kO + h * D, p = tmem + S::kS + h * kKeys;
+    auto values = [&](int j) {
+      const uint64_t v = v0 + (j % kStages) * kStage;
 #pragma unroll
-      for (int s = 0; s < kKeys / 16; ++s)
-        tc::mma_ts_f16(to, p + 8 * s, tc::desc_mn16(v, D, s), kIdO, j > 0 || s > 0);
+      for (int s = 0; s < kKeys / 16; ++s) mma_ts(at_o, at_s + 8 * s, v + s * vStep, kIdO, j > 0 || s > 0);
       if constexpr (TERMS == 2) {
 #pragma unroll
-        for (int s = 0; s < kKeys / 16; ++s) tc::mma_ts_f16(to, p + 32 + 8 * s, tc::desc_mn16(v, D, s), kIdO, 1);
+        for (int s = 0; s < kKeys / 16; ++s) mma_ts(at_o, at_s + 32 + 8 * s, v + s * vStep, kIdO, true);
       }
     };
+    auto full = [&](int j) { return tc::bar_wait(&kv_full[j % kStages], (j / kStages) & 1); };
     bool ok = true;
-    int arrived[2] = {0, 0};  // phases of p_full waited for
-    auto wait_p = [&](int h) { return tc::bar_wait(&p_full[h], arrived[h]++ & 1); };
-    if (count1 > 0) {
-      ok = tc::bar_wait(&kv_full[0], 0);
-      for (int h = 0; h < 2 && ok; ++h)
-        if (counts[h] > 0) {
-          ok = wait_p(h);  // Q is in place
-          if (!ok) break;
-          tc::fence_after_sync();
-          scores(h, 0);
-          tc::commit(&s_full[h]);
-        }
-    }
-    for (int j = 0; j < count1 && ok; ++j) {
-      // the second half may go on after the first has ended
-      bool next = false;
-      for (int h = 0; h < 2 && ok; ++h) {
-        if (j < counts[h]) {
-          ok = wait_p(h);
-          if (!ok) break;
-          tc::fence_after_sync();
-          values(h, j);
-        }
-        if (h == 1 || !both) tc::commit(&kv_free[j % kStages]);
-        if (j + 1 < counts[h]) {
-          if (!next) ok = tc::bar_wait(&kv_full[(j + 1) % kStages], ((j + 1) / kStages) & 1);
-          next = true;
-          if (!ok) break;
-          tc::fence_after_sync();
-          scores(h, j + 1);
-        }
-        if (j < counts[h]) tc::commit(&s_full[h]);
-        if (!both) break;
+    if (count > 0) {
+      ok = full(0) && tc::bar_wait(&p_full[h], 0);  // Q is in place
+      if (ok) {
+        tc::fence_after_sync();
+        scores(0);
+        tc::commit(&s_full[h]);
       }
     }
+    for (int j = 0; j < count && ok; ++j) {
+      // the next tile is there long before the softmax is done
+      ok = (j + 1 == count || full(j + 1)) && tc::bar_wait(&p_full[h], (j + 1) & 1);
+      if (!ok) break;
+      tc::fence_after_sync();
+      values(j);
+      tc::commit(&kv_free[j % kStages]);
+      if (j + 1 < count) scores(j + 1);
+      tc::commit(&s_full[h]);
+    }
+    // the tiles that only the other half sees: released once they are full,
+    // so that no phase gets this half's arrival twice
+    if (both)
+      for (int j = count; j < count1 && ok; ++j) {
+        ok = full(j);
+        if (ok) tc::bar_arrive(&kv_free[j % kStages]);
+      }
     if (!ok) *failed = 1;
     // nothing is in flight when tensor memory is given back
-    tc::commit(drained);
-    if (!tc::bar_wait(drained, 0)) *failed = 1;
+    tc::commit(&drained[h]);
+    if (!tc::bar_wait(&drained[h], 0)) *failed = 1;
   }
   __syncwarp();
   tc::fence_before_sync();
