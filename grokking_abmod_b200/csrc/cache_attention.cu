@@ -463,8 +463,8 @@ __global__ void __launch_bounds__(kSplitThreads)
 //                   where a maximum has grown
 //   warps 8-11      converters: the tile's codes from global memory (loaded a
 //                   tile ahead), as FP16 into shared memory, once for both halves
-//   warps 12, 13    issue the products of a half each, S = Q K^T and O += P V:
-//                   one half's products run under the other's softmax
+//   warp 12         issues the products S = Q K^T and O += P V, the halves in
+//                   turn: one half's products run under the other's softmax
 //
 // Q, S (P over it) and O fill tensor memory, all products take A from there:
 // with A in shared memory its reads alone would take more than the products'
@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(kSplitThreads)
 constexpr int kKeys = 64;
 constexpr int kHalfRows = 128;
 constexpr int kTileRows = 2 * kHalfRows;
-constexpr int kTileThreads = 14 * 32;
+constexpr int kTileThreads = 13 * 32;
 constexpr int kConverters = 128;
 constexpr int kStages = 2;
 constexpr float kLazy = 4.f;
@@ -514,6 +514,13 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint3
       "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add));
 }
 
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+  return yes != 0;
+}
+
 // 64 columns of this thread's lane.
 __device__ __forceinline__ void tmem_ld64(uint32_t at, float (&v)[64]) {
   tc::tmem_ld32(at, v);
@@ -526,7 +533,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
   using S = TileShape<D, TERMS>;
   extern __shared__ __align__(128) uint8_t smem[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the shuffle makes the warp's number, and what follows from it, uniform
+  const int warp = __shfl_sync(kFull, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int chunk = blockIdx.x % part.chunks, head = blockIdx.y;
   // the last rows see the most: they go first
   const int block = blockIdx.x / part.chunks;
@@ -565,20 +573,20 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* kv_free = bars + kStages;     // [stage] products -> converters
   uint64_t* s_full = bars + 2 * kStages;  // [half] products -> softmax
   uint64_t* p_full = s_full + 2;          // [half] softmax (and Q, once) -> products
-  uint64_t* drained = p_full + 2;         // [half]
-  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drained + 2);
+  uint64_t* drained = p_full + 2;
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drained + 1);
   int* failed = reinterpret_cast<int*>(tmem_at + 1);
   float* meta = reinterpret_cast<float*>(smem + S::kMeta);  // [stage][4 K scales, 4 V scales] of 16 tokens each
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       tc::bar_init(&kv_full[s], kConverters);
-      tc::bar_init(&kv_free[s], both ? 2 : 1);
+      tc::bar_init(&kv_free[s], 1);
     }
     for (int h = 0; h < 2; ++h) {
       tc::bar_init(&s_full[h], 1);
       tc::bar_init(&p_full[h], kHalfRows);
-      tc::bar_init(&drained[h], 1);
     }
+    tc::bar_init(drained, 1);
     *failed = 0;
   }
   tc::bar_init_fence();
@@ -586,7 +594,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  const uint32_t tmem = *tmem_at;
+  const uint32_t tmem = __shfl_sync(kFull, *tmem_at, 0);
 
   if (warp < 8) {
     const int h = warp >> 2;
@@ -845,69 +853,78 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       tc::bar_arrive(&kv_full[stage]);
       if (j + 1 < count1) load(j + 1);
     }
-  } else if (lane == 0) {
-    // Issuer of one half.  Descriptors are a base and constant steps: the
-    // fewer instructions between two products, the closer their issue gets
-    // to the tensor pipe's rate.
-    const int h = warp - 12;
-    const int count = h ? (both ? count1 : 0) : (both ? count0 : count1);
+  } else {
+    // The whole warp waits, one lane issues: everything it works with is
+    // uniform, which keeps the instructions between two products few (from a
+    // single diverged lane a product took about 100 cycles to issue).  The
+    // halves take turns, a half's O += P V and next S in one go: with a warp
+    // for each half they fell into step, softmax and products both at once
+    // and neither over the other (3250 against 1900 cycles a tile).
+    const bool elected = elect_one();
+    const int counts[2] = {both ? count0 : count1, both ? count1 : 0};
     constexpr uint32_t kIdS = tc::idesc_f16(128, kKeys), kIdO = tc::idesc_f16(128, D, true);
-    const uint32_t at_q = tmem + h * S::kQ, at_s = tmem + S::kS + h * kKeys, at_o = tmem + S::kO + h * D;
     const uint64_t k0 = tc::desc_kmajor16(smem, D, 0), v0 = tc::desc_mn16(smem + S::kOperand, D, 0);
-    const uint64_t low0 = tc::desc_kmajor16(smem + S::kLow + h * kHalfRows * D * 2, D, 0);
+    const uint64_t low0 = tc::desc_kmajor16(smem + S::kLow, D, 0);
     constexpr uint64_t kStep = 256 >> 4, vStep = D / 8 * 256 >> 4, kStage = 2 * S::kOperand >> 4;
-    auto scores = [&](int j) {
+    constexpr uint64_t kLowHalf = kHalfRows * D * 2 >> 4;
+    auto scores = [&](int h, int j) {
       const uint64_t k = k0 + (j % kStages) * kStage;
+      const uint32_t to = tmem + S::kS + h * kKeys, q_at = tmem + h * S::kQ;
 #pragma unroll
-      for (int s = 0; s < D / 16; ++s) mma_ts(at_s, at_q + 8 * s, k + s * kStep, kIdS, s > 0);
+      for (int s = 0; s < D / 16; ++s) mma_ts(to, q_at + 8 * s, k + s * kStep, kIdS, s > 0);
       if constexpr (TERMS == 2) {
 #pragma unroll
         for (int s = 0; s < D / 16; ++s) {
-          if constexpr (S::kLowInSmem) mma_ss(at_s, low0 + s * kStep, k + s * kStep, kIdS, true);
-          else mma_ts(at_s, at_q + D / 2 + 8 * s, k + s * kStep, kIdS, true);
+          if constexpr (S::kLowInSmem) mma_ss(to, low0 + h * kLowHalf + s * kStep, k + s * kStep, kIdS, true);
+          else mma_ts(to, q_at + D / 2 + 8 * s, k + s * kStep, kIdS, true);
         }
       }
     };
-    auto values = [&](int j) {
+    auto values = [&](int h, int j) {
       const uint64_t v = v0 + (j % kStages) * kStage;
+      const uint32_t to = tmem + S::kO + h * D, p_at = tmem + S::kS + h * kKeys;
 #pragma unroll
-      for (int s = 0; s < kKeys / 16; ++s) mma_ts(at_o, at_s + 8 * s, v + s * vStep, kIdO, j > 0 || s > 0);
+      for (int s = 0; s < kKeys / 16; ++s) mma_ts(to, p_at + 8 * s, v + s * vStep, kIdO, j > 0 || s > 0);
       if constexpr (TERMS == 2) {
 #pragma unroll
-        for (int s = 0; s < kKeys / 16; ++s) mma_ts(at_o, at_s + 32 + 8 * s, v + s * vStep, kIdO, true);
+        for (int s = 0; s < kKeys / 16; ++s) mma_ts(to, p_at + 32 + 8 * s, v + s * vStep, kIdO, true);
       }
     };
     auto full = [&](int j) { return tc::bar_wait(&kv_full[j % kStages], (j / kStages) & 1); };
-    bool ok = true;
-    if (count > 0) {
-      ok = full(0) && tc::bar_wait(&p_full[h], 0);  // Q is in place
-      if (ok) {
-        tc::fence_after_sync();
-        scores(0);
+    bool ok = count1 == 0 || full(0);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (counts[h] == 0 || !__all_sync(kFull, ok)) continue;
+      ok = __all_sync(kFull, tc::bar_wait(&p_full[h], 0));  // Q is in place
+      tc::fence_after_sync();
+      if (ok && elected) {
+        scores(h, 0);
         tc::commit(&s_full[h]);
       }
+      __syncwarp();
     }
-    for (int j = 0; j < count && ok; ++j) {
+    for (int j = 0; j < count1 && ok; ++j) {
       // the next tile is there long before the softmax is done
-      ok = (j + 1 == count || full(j + 1)) && tc::bar_wait(&p_full[h], (j + 1) & 1);
-      if (!ok) break;
-      tc::fence_after_sync();
-      values(j);
-      tc::commit(&kv_free[j % kStages]);
-      if (j + 1 < count) scores(j + 1);
-      tc::commit(&s_full[h]);
-    }
-    // the tiles that only the other half sees: released once they are full,
-    // so that no phase gets this half's arrival twice
-    if (both)
-      for (int j = count; j < count1 && ok; ++j) {
-        ok = full(j);
-        if (ok) tc::bar_arrive(&kv_free[j % kStages]);
+      ok = __all_sync(kFull, j + 1 == count1 || full(j + 1));
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (j < counts[h] && ok) {
+          ok = __all_sync(kFull, tc::bar_wait(&p_full[h], (j + 1) & 1));
+          tc::fence_after_sync();
+          if (ok && elected) {
+            values(h, j);
+            if (h == (both ? 1 : 0)) tc::commit(&kv_free[j % kStages]);
+            if (j + 1 < counts[h]) scores(h, j + 1);
+            tc::commit(&s_full[h]);
+          }
+          __syncwarp();
+        }
       }
+    }
     if (!ok) *failed = 1;
     // nothing is in flight when tensor memory is given back
-    tc::commit(&drained[h]);
-    if (!tc::bar_wait(&drained[h], 0)) *failed = 1;
+    if (elected) tc::commit(drained);
+    if (!tc::bar_wait(drained, 0)) *failed = 1;
   }
   __syncwarp();
   tc::fence_before_sync();
