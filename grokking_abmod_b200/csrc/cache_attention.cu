@@ -521,12 +521,6 @@ __device__ __forceinline__ bool elect_one() {
   return yes != 0;
 }
 
-// 64 columns of this thread's lane.
-__device__ __forceinline__ void tmem_ld64(uint32_t at, float (&v)[64]) {
-  tc::tmem_ld32(at, v);
-  tc::tmem_ld32(at + 32, v + 32);
-}
-
 template <class T, int D>
 __global__ void __launch_bounds__(kTileThreads, 1)
     attend_tiles(View c, Batch t, Queries q, Partials part, int blocks_per_seq) {
@@ -672,8 +666,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         break;
       }
       tc::fence_after_sync();
-      float x[kKeys];
-      tmem_ld64(at_s, x);
       const float4 ks = *reinterpret_cast<const float4*>(meta + stage * 8);
       const float4 vs = *reinterpret_cast<const float4*>(meta + stage * 8 + 4);
       // not 0, so that a masked score stays -inf; NaN stays
@@ -682,22 +674,29 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       for (int g = 0; g < 4; ++g) fk[g] = fk[g] < 2e-38f ? 2e-38f : fk[g];
       const float sv[4] = {vs.x, vs.y, vs.z, vs.w};
       const int pos = (begin + j) * kKeys;
-      if (pos < u.lo || pos + kKeys - 1 > sure) {
-#pragma unroll
-        for (int i = 0; i < kKeys; ++i)
-          if (pos + i < u.lo || pos + i > limit) x[i] = -INFINITY;
-      }
+      const bool partial = pos < u.lo || pos + kKeys - 1 > sure;
+      // The scores are read twice, 32 columns at a time, once for their
+      // maximum and once for their exponentials: 64 at once spill.
       float mx = m;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        float a0 = x[16 * g], a1 = x[16 * g + 1];
+      for (int part32 = 0; part32 < 2; ++part32) {
+        float x[32];
+        tc::tmem_ld32(at_s + 32 * part32, x);
+        if (partial) {
 #pragma unroll
-        for (int i = 2; i < 16; i += 2) {
-          a0 = fmaxf(a0, x[16 * g + i]);
-          a1 = fmaxf(a1, x[16 * g + i + 1]);
+          for (int i = 0; i < 32; ++i)
+            if (pos + 32 * part32 + i < u.lo || pos + 32 * part32 + i > limit) x[i] = -INFINITY;
         }
-        a0 = fmaxf(a0, a1);
-        mx = fmaxf(mx, a0 * fk[g]);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          float a0 = x[16 * g], a1 = x[16 * g + 1];
+#pragma unroll
+          for (int i = 2; i < 16; i += 2) {
+            a0 = fmaxf(a0, x[16 * g + i]);
+            a1 = fmaxf(a1, x[16 * g + i + 1]);
+          }
+          mx = fmaxf(mx, fmaxf(a0, a1) * fk[2 * part32 + g]);
+        }
       }
       int top = ev;
 #pragma unroll
@@ -725,12 +724,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const float unit = power_of_two(-ev);
       float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+      for (int part32 = 0; part32 < 2; ++part32) {
+        float x[32];
+        tc::tmem_ld32(at_s + 32 * part32, x);
+        if (partial) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (pos + 32 * part32 + i < u.lo || pos + 32 * part32 + i > limit) x[i] = -INFINITY;
+        }
         uint32_t hi[16], lo[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int e = 32 * half + 2 * i, g = e / 16;
-          const float2 y = fma2(make_float2(x[e], x[e + 1]), splat2(fk[g]), nbase);
+          const int g = 2 * part32 + i / 8;
+          const float2 y = fma2(make_float2(x[2 * i], x[2 * i + 1]), splat2(fk[g]), nbase);
           const float2 p = make_float2(ex2_ftz(y.x), ex2_ftz(y.y));
           sum = add2(sum, p);
           const float2 w = mul2(p, splat2(sv[g] * unit * kProbScale));
@@ -741,8 +747,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             hi[i] = *reinterpret_cast<const uint32_t*>(&v);
           }
         }
-        tc::tmem_st16u(at_s + 16 * half, hi);
-        if constexpr (TERMS == 2) tc::tmem_st16u(at_s + 32 + 16 * half, lo);
+        // P of 32 tokens over their own scores' columns: hi in the first 16, lo behind
+        tc::tmem_st16u(at_s + 32 * part32, hi);
+        if constexpr (TERMS == 2) tc::tmem_st16u(at_s + 32 * part32 + 16, lo);
       }
       l += sum.x + sum.y;
       tc::tmem_st_wait();
@@ -884,10 +891,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const uint64_t v = v0 + (j % kStages) * kStage;
       const uint32_t to = tmem + S::kO + h * D, p_at = tmem + S::kS + h * kKeys;
 #pragma unroll
-      for (int s = 0; s < kKeys / 16; ++s) mma_ts(to, p_at + 8 * s, v + s * vStep, kIdO, j > 0 || s > 0);
-      if constexpr (TERMS == 2) {
-#pragma unroll
-        for (int s = 0; s < kKeys / 16; ++s) mma_ts(to, p_at + 32 + 8 * s, v + s * vStep, kIdO, true);
+      for (int s = 0; s < kKeys / 16; ++s) {
+        const uint32_t p_s = p_at + s / 2 * 32 + s % 2 * 8;  // 16 tokens
+        mma_ts(to, p_s, v + s * vStep, kIdO, j > 0 || s > 0);
+        if constexpr (TERMS == 2) mma_ts(to, p_s + 16, v + s * vStep, kIdO, true);
       }
     };
     auto full = [&](int j) { return tc::bar_wait(&kv_full[j % kStages], (j / kStages) & 1); };
