@@ -466,10 +466,10 @@ __global__ void __launch_bounds__(kSplitThreads)
 //   warp 12         issues the products S = Q K^T and O += P V, the halves in
 //                   turn: one half's products run under the other's softmax
 //
-// Q, S (P over it) and O fill tensor memory, all products take A from there:
-// with A in shared memory its reads alone would take more than the products'
-// time at 64 tokens.  K and V share one layout, rows = tokens: K-major for
-// S, MN-major for O.  Queries and probabilities of FP32 rows are FP16 pairs
+// Each half has two score buffers (P goes over S in place), so that the next
+// scores are there when a softmax ends and only softmax follows softmax in a
+// half's chain.  K and V share one layout, rows = tokens: K-major for S,
+// MN-major for O.  Queries and probabilities of FP32 rows are FP16 pairs
 // (two products), those of 16-bit rows one FP16 (bfloat16's 8 bits fit; a
 // probability's rounding to 11 bits is below the output's own).
 //
@@ -481,23 +481,25 @@ constexpr int kHalfRows = 128;
 constexpr int kTileRows = 2 * kHalfRows;
 constexpr int kTileThreads = 13 * 32;
 constexpr int kConverters = 128;
-constexpr int kStages = 2;
+constexpr int kStages = 3;
 constexpr float kLazy = 4.f;
 constexpr float kProbScale = 2048.f;
 
 template <int D, int TERMS>
 struct TileShape {
-  // FP32 rows 128 wide: their lo parts do not fit into tensor memory
-  static constexpr bool kLowInSmem = TERMS == 2 && D == 128;
-  static constexpr int kQ = kLowInSmem ? D / 2 : TERMS * D / 2;  // columns of a half's Q
-  static constexpr int kS = 2 * kQ;
-  static constexpr int kO = kS + 2 * kKeys;
+  // Two score buffers a half and O leave room for Q in tensor memory up to
+  // head width 64; wider heads read it from shared memory.
+  static constexpr bool kQInSmem = D > 64;
+  static constexpr int kQ = kQInSmem ? 0 : TERMS * D / 2;  // columns of a half's Q
+  static constexpr int kS = 2 * kQ;                        // [half][buffer]
+  static constexpr int kO = kS + 4 * kKeys;
   static_assert(kO + 2 * D <= 512, "tensor memory");
-  static constexpr int kOperand = kKeys * D * 2;  // bytes of a K or V tile
-  static constexpr int kLow = kStages * 2 * kOperand;
-  static constexpr int kMeta = kLow + (kLowInSmem ? 2 * kHalfRows * D * 2 : 0);
+  static constexpr int kOperand = kKeys * D * 2;           // bytes of a K or V tile
+  static constexpr int kQTile = kHalfRows * D * 2;         // bytes of a half's Q, a term
+  static constexpr int kQueries = kStages * 2 * kOperand;  // [half][term]
+  static constexpr int kMeta = kQueries + (kQInSmem ? 2 * TERMS * kQTile : 0);
   static constexpr int kBars = kMeta + kStages * 32;
-  static constexpr int kBytes = kBars + 128;
+  static constexpr int kBytes = kBars + 160;
 };
 
 // D (tensor memory) (+)= A (tensor memory, or shared memory) * B (shared memory), FP16.
@@ -565,9 +567,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
   uint64_t* kv_full = bars;               // [stage] converters -> products and softmax
   uint64_t* kv_free = bars + kStages;     // [stage] products -> converters
-  uint64_t* s_full = bars + 2 * kStages;  // [half] products -> softmax
-  uint64_t* p_full = s_full + 2;          // [half] softmax (and Q, once) -> products
-  uint64_t* drained = p_full + 2;
+  uint64_t* s_full = bars + 2 * kStages;  // [half][buffer] scores -> softmax
+  uint64_t* p_full = s_full + 4;          // [half][buffer] softmax -> products: a half may be two tiles ahead
+  uint64_t* q_full = p_full + 4;          // [half]
+  uint64_t* o_full = q_full + 2;          // [half] O += P V is done
+  uint64_t* drained = o_full + 2;
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drained + 1);
   int* failed = reinterpret_cast<int*>(tmem_at + 1);
   float* meta = reinterpret_cast<float*>(smem + S::kMeta);  // [stage][4 K scales, 4 V scales] of 16 tokens each
@@ -577,8 +581,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       tc::bar_init(&kv_free[s], 1);
     }
     for (int h = 0; h < 2; ++h) {
-      tc::bar_init(&s_full[h], 1);
-      tc::bar_init(&p_full[h], kHalfRows);
+      for (int k = 0; k < 2; ++k) {
+        tc::bar_init(&s_full[2 * h + k], 1);
+        tc::bar_init(&p_full[2 * h + k], kHalfRows);
+      }
+      tc::bar_init(&q_full[h], kHalfRows);
+      tc::bar_init(&o_full[h], 1);
     }
     tc::bar_init(drained, 1);
     *failed = 0;
@@ -595,7 +603,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const int count = h ? (both ? count1 : 0) : (both ? count0 : count1);
     const int r = h * kHalfRows + (warp & 3) * 32 + lane;  // row of the unit
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t at_q = lanes + h * S::kQ, at_s = lanes + S::kS + h * kKeys, at_o = lanes + S::kO + h * D;
+    const uint32_t at_q = lanes + h * S::kQ, at_o = lanes + S::kO + h * D;
     const bool there = r < u.rows;
     const int tok = (u.row0 + r) / q.group, a = head * q.group + (u.row0 + r) % q.group;
     const int limit = there ? old + tok : -1;
@@ -641,30 +649,32 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
         for (int i = 0; i < 16; ++i) tc::split_f16x2(x[2 * i] * sign, x[2 * i + 1] * sign, hi[i], lo[i]);
         __syncwarp();
-        tc::tmem_st16u(at_q + c0 / 2, hi);
-        if constexpr (S::kLowInSmem) {
-          __half* low = reinterpret_cast<__half*>(smem + S::kLow) + h * kHalfRows * D;
+        if constexpr (S::kQInSmem) {
+          __half* at = reinterpret_cast<__half*>(smem + S::kQueries + h * TERMS * S::kQTile);
 #pragma unroll
-          for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<uint4*>(low + tc::blk16(r & (kHalfRows - 1), c0 + 2 * i, D)) =
-                make_uint4(lo[i], lo[i + 1], lo[i + 2], lo[i + 3]);
-        } else if constexpr (TERMS == 2) {
-          tc::tmem_st16u(at_q + D / 2 + c0 / 2, lo);
+          for (int i = 0; i < 16; i += 4) {
+            const int e = tc::blk16(r & (kHalfRows - 1), c0 + 2 * i, D);
+            *reinterpret_cast<uint4*>(at + e) = make_uint4(hi[i], hi[i + 1], hi[i + 2], hi[i + 3]);
+            if constexpr (TERMS == 2)
+              *reinterpret_cast<uint4*>(at + S::kQTile / 2 + e) = make_uint4(lo[i], lo[i + 1], lo[i + 2], lo[i + 3]);
+          }
+        } else {
+          tc::tmem_st16u(at_q + c0 / 2, hi);
+          if constexpr (TERMS == 2) tc::tmem_st16u(at_q + D / 2 + c0 / 2, lo);
         }
       }
       tc::tmem_st_wait();
       tc::fence_async_smem();
       tc::fence_before_sync();
-      tc::bar_arrive(&p_full[h]);
+      tc::bar_arrive(&q_full[h]);
     }
     for (int j = 0; j < count; ++j) {
       const int stage = j % kStages;
       // both: the tile's scales (converters) and its scores (products)
-      alive = tc::bar_wait(&kv_full[stage], (j / kStages) & 1) && tc::bar_wait(&s_full[h], j & 1);
-      if (!__all_sync(kFull, alive)) {
-        alive = false;
-        break;
-      }
+      alive = __all_sync(kFull, tc::bar_wait(&kv_full[stage], (j / kStages) & 1) &&
+                                    tc::bar_wait(&s_full[2 * h + (j & 1)], (j >> 1) & 1));
+      if (!alive) break;
+      const uint32_t at_s = lanes + S::kS + (2 * h + (j & 1)) * kKeys;
       tc::fence_after_sync();
       const float4 ks = *reinterpret_cast<const float4*>(meta + stage * 8);
       const float4 vs = *reinterpret_cast<const float4*>(meta + stage * 8 + 4);
@@ -709,6 +719,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         m = mx;
         ev = top;
         if (j > 0) {
+          // the products before this tile's are in O
+          alive = __all_sync(kFull, tc::bar_wait(&o_full[h], (j - 1) & 1));
+          if (!alive) break;
+          tc::fence_after_sync();
 #pragma unroll
           for (int c0 = 0; c0 < D; c0 += 16) {
             float o[16];
@@ -754,9 +768,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       l += sum.x + sum.y;
       tc::tmem_st_wait();
       tc::fence_before_sync();
-      tc::bar_arrive(&p_full[h]);
+      tc::bar_arrive(&p_full[2 * h + (j & 1)]);
     }
-    if (count > 0 && alive) alive = __all_sync(kFull, tc::bar_wait(&s_full[h], count & 1));
+    // the scores of the last tile vouch for the products three tiles back: both
+    // later phases are waited for in order, a parity is exact for one only
+    if (count > 1 && alive) alive = __all_sync(kFull, tc::bar_wait(&o_full[h], (count - 2) & 1));
+    if (count > 0 && alive) alive = __all_sync(kFull, tc::bar_wait(&o_full[h], (count - 1) & 1));
     if (!alive) *failed = 1;
     tc::fence_after_sync();
     const float inverse = l == 0.f ? 0.f : power_of_two(ev) * (1.f / kProbScale) / l;
@@ -798,51 +815,63 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     constexpr int PIECES = D / 32;  // of K and of V, a thread and tile
     const int ct = threadIdx.x - 8 * 32;
     uint4 kq[PIECES], vq[PIECES];
-    float sk = 0.f, sv = 0.f;
+    int pages[PIECES], scale_page = -1;
+    float sk = 1.f, sv = 0.f;
+    auto row_of = [&](int i) { return (ct + kConverters * i) / (8 * (D / 16)) * 8 + (ct & 7); };
+    auto channel_of = [&](int i) { return ((ct + kConverters * i) >> 3) % (D / 16) * 16; };
+    // The page of a token: -1 out of the pool, -2 where no row sees the page;
+    // that is not looked up, its tokens are masked, as zeros.
+    auto look_up = [&](int pos) {
+      const int first_of_page = pos & ~(c.tokens - 1);
+      return first_of_page < u.hi && first_of_page + c.tokens > u.lo ? page_of(t, c, u.b, pos >> c.shift) : -2;
+    };
+    // Page numbers are read two tiles ahead and codes one, so that neither is waited for.
+    auto find = [&](int j) {
+      const int pos = (begin + j) * kKeys;
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) pages[i] = look_up(pos + row_of(i));
+      if (ct < 4) scale_page = look_up(pos + 16 * ct);
+    };
     auto load = [&](int j) {
       const int pos = (begin + j) * kKeys;
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
-        const int idx = ct + kConverters * i;
-        const int row = idx / (8 * (D / 16)) * 8 + (idx & 7), at = (idx >> 3) % (D / 16) * 16;
         kq[i] = vq[i] = make_uint4(0u, 0u, 0u, 0u);
-        const int first_of_page = (pos + row) & ~(c.tokens - 1);
-        // pages that no row sees are not looked up: their tokens are masked, as zeros
-        if (first_of_page < u.hi && first_of_page + c.tokens > u.lo) {
-          const int page = page_of(t, c, u.b, (pos + row) >> c.shift);
-          if (page >= 0) {
-            const size_t from = c.row(page, head, (pos + row) & (c.tokens - 1)) + at;
-            kq[i] = __ldg(reinterpret_cast<const uint4*>(c.k + from));
-            vq[i] = __ldg(reinterpret_cast<const uint4*>(c.v + from));
-          }
+        if (pages[i] >= 0) {
+          const size_t from = c.row(pages[i], head, (pos + row_of(i)) & (c.tokens - 1)) + channel_of(i);
+          kq[i] = __ldg(reinterpret_cast<const uint4*>(c.k + from));
+          vq[i] = __ldg(reinterpret_cast<const uint4*>(c.v + from));
         }
       }
       if (ct < 4) {
-        sk = sv = 0.f;
-        const int first_of_page = (pos + 16 * ct) & ~(c.tokens - 1);
-        if (first_of_page < u.hi && first_of_page + c.tokens > u.lo) {
-          const int page = page_of(t, c, u.b, (pos + 16 * ct) >> c.shift);
-          if (page < 0 && q.status) atomicOr(q.status, kBadPage);
-          sk = page < 0 ? NAN : __ldg(c.k_scale + c.scale_at(page, head));
-          sv = page < 0 ? NAN : __ldg(c.v_scale + c.scale_at(page, head));
+        sk = 1.f;
+        sv = 0.f;
+        if (scale_page >= 0) {
+          sk = __ldg(c.k_scale + c.scale_at(scale_page, head));
+          sv = __ldg(c.v_scale + c.scale_at(scale_page, head));
+        } else if (scale_page == -1) {
+          sk = sv = NAN;
+          if (q.status) atomicOr(q.status, kBadPage);
         }
       }
     };
     auto store = [&](uint8_t* tile, const uint4 (&codes)[PIECES]) {
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
-        const int idx = ct + kConverters * i;
-        const int row = idx / (8 * (D / 16)) * 8 + (idx & 7), at = (idx >> 3) % (D / 16) * 16;
         const uint32_t w[4] = {codes[i].x ^ 0x80808080u, codes[i].y ^ 0x80808080u, codes[i].z ^ 0x80808080u,
                                codes[i].w ^ 0x80808080u};
-        __half* to = reinterpret_cast<__half*>(tile) + tc::blk16(row, at, D);
+        __half* to = reinterpret_cast<__half*>(tile) + tc::blk16(row_of(i), channel_of(i), D);
         *reinterpret_cast<uint4*>(to) = make_uint4(codes_to_f16(w[0], 0x4140), codes_to_f16(w[0], 0x4342),
                                                    codes_to_f16(w[1], 0x4140), codes_to_f16(w[1], 0x4342));
         *reinterpret_cast<uint4*>(to + 64) = make_uint4(codes_to_f16(w[2], 0x4140), codes_to_f16(w[2], 0x4342),
                                                         codes_to_f16(w[3], 0x4140), codes_to_f16(w[3], 0x4342));
       }
     };
-    if (count1 > 0) load(0);
+    if (count1 > 0) {
+      find(0);
+      load(0);
+      if (count1 > 1) find(1);
+    }
     for (int j = 0; j < count1; ++j) {
       const int stage = j % kStages;
       if (j >= kStages && !tc::bar_wait(&kv_free[stage], (j / kStages - 1) & 1)) {
@@ -859,37 +888,37 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       tc::fence_async_smem();
       tc::bar_arrive(&kv_full[stage]);
       if (j + 1 < count1) load(j + 1);
+      if (j + 2 < count1) find(j + 2);
     }
   } else {
     // The whole warp waits, one lane issues: everything it works with is
     // uniform, which keeps the instructions between two products few (from a
     // single diverged lane a product took about 100 cycles to issue).  The
-    // halves take turns, a half's O += P V and next S in one go: with a warp
-    // for each half they fell into step, softmax and products both at once
-    // and neither over the other (3250 against 1900 cycles a tile).
+    // halves take turns.
     const bool elected = elect_one();
     const int counts[2] = {both ? count0 : count1, both ? count1 : 0};
     constexpr uint32_t kIdS = tc::idesc_f16(128, kKeys), kIdO = tc::idesc_f16(128, D, true);
     const uint64_t k0 = tc::desc_kmajor16(smem, D, 0), v0 = tc::desc_mn16(smem + S::kOperand, D, 0);
-    const uint64_t low0 = tc::desc_kmajor16(smem + S::kLow, D, 0);
+    const uint64_t q0 = tc::desc_kmajor16(smem + S::kQueries, D, 0);
     constexpr uint64_t kStep = 256 >> 4, vStep = D / 8 * 256 >> 4, kStage = 2 * S::kOperand >> 4;
-    constexpr uint64_t kLowHalf = kHalfRows * D * 2 >> 4;
     auto scores = [&](int h, int j) {
       const uint64_t k = k0 + (j % kStages) * kStage;
-      const uint32_t to = tmem + S::kS + h * kKeys, q_at = tmem + h * S::kQ;
+      const uint32_t to = tmem + S::kS + (2 * h + (j & 1)) * kKeys;
 #pragma unroll
-      for (int s = 0; s < D / 16; ++s) mma_ts(to, q_at + 8 * s, k + s * kStep, kIdS, s > 0);
-      if constexpr (TERMS == 2) {
+      for (int term = 0; term < TERMS; ++term) {
 #pragma unroll
         for (int s = 0; s < D / 16; ++s) {
-          if constexpr (S::kLowInSmem) mma_ss(to, low0 + h * kLowHalf + s * kStep, k + s * kStep, kIdS, true);
-          else mma_ts(to, q_at + D / 2 + 8 * s, k + s * kStep, kIdS, true);
+          const bool add = term > 0 || s > 0;
+          if constexpr (S::kQInSmem)
+            mma_ss(to, q0 + (h * TERMS + term) * (S::kQTile >> 4) + s * kStep, k + s * kStep, kIdS, add);
+          else
+            mma_ts(to, tmem + h * S::kQ + term * (D / 2) + 8 * s, k + s * kStep, kIdS, add);
         }
       }
     };
     auto values = [&](int h, int j) {
       const uint64_t v = v0 + (j % kStages) * kStage;
-      const uint32_t to = tmem + S::kO + h * D, p_at = tmem + S::kS + h * kKeys;
+      const uint32_t to = tmem + S::kO + h * D, p_at = tmem + S::kS + (2 * h + (j & 1)) * kKeys;
 #pragma unroll
       for (int s = 0; s < kKeys / 16; ++s) {
         const uint32_t p_s = p_at + s / 2 * 32 + s % 2 * 8;  // 16 tokens
@@ -898,34 +927,51 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
     };
     auto full = [&](int j) { return tc::bar_wait(&kv_full[j % kStages], (j / kStages) & 1); };
-    bool ok = count1 == 0 || full(0);
+    bool ok = true;
+    // the first two tiles' scores
+    for (int j = 0; j < 2 && j < count1 && ok; ++j) {
+      ok = __all_sync(kFull, full(j));
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (counts[h] == 0 || !__all_sync(kFull, ok)) continue;
-      ok = __all_sync(kFull, tc::bar_wait(&p_full[h], 0));  // Q is in place
+      for (int h = 0; h < 2; ++h) {
+        if (j >= counts[h] || !ok) continue;
+        if (j == 0) ok = __all_sync(kFull, tc::bar_wait(&q_full[h], 0));
+        tc::fence_after_sync();
+        if (ok && elected) {
+          scores(h, j);
+          tc::commit(&s_full[2 * h + j]);
+        }
+        __syncwarp();
+      }
+    }
+    // Scores of tile i go over the probabilities of tile i - 2: not before the
+    // products that read them are done (only products of one accumulator and
+    // shape are ordered among themselves).
+    auto next_scores = [&](int h, int i) {
+      if (i < 2 || i >= counts[h] || !ok) return;
+      ok = __all_sync(kFull, full(i) && tc::bar_wait(&o_full[h], i & 1));
       tc::fence_after_sync();
       if (ok && elected) {
-        scores(h, 0);
-        tc::commit(&s_full[h]);
+        scores(h, i);
+        tc::commit(&s_full[2 * h + (i & 1)]);
       }
       __syncwarp();
-    }
+    };
     for (int j = 0; j < count1 && ok; ++j) {
-      // the next tile is there long before the softmax is done
-      ok = __all_sync(kFull, j + 1 == count1 || full(j + 1));
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         if (j < counts[h] && ok) {
-          ok = __all_sync(kFull, tc::bar_wait(&p_full[h], (j + 1) & 1));
+          ok = __all_sync(kFull, tc::bar_wait(&p_full[2 * h + (j & 1)], (j >> 1) & 1));
           tc::fence_after_sync();
           if (ok && elected) {
             values(h, j);
+            tc::commit(&o_full[h]);
             if (h == (both ? 1 : 0)) tc::commit(&kv_free[j % kStages]);
-            if (j + 1 < counts[h]) scores(h, j + 1);
-            tc::commit(&s_full[h]);
           }
           __syncwarp();
         }
+        // the other half's scores: its last products were issued before these
+        if (h == 0) next_scores(1, j + 1);
+        else next_scores(0, j + 2);
       }
     }
     if (!ok) *failed = 1;
