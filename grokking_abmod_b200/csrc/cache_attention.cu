@@ -829,18 +829,21 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     auto find = [&](int j) {
       const int pos = (begin + j) * kKeys;
 #pragma unroll
-      for (int i = 0; i < PIECES; ++i) pages[i] = look_up(pos + row_of(i));
+      for (int i = 0; i < PIECES; ++i) pages[i] = i > 0 && c.tokens >= kKeys ? pages[0] : look_up(pos + row_of(i));
       if (ct < 4) scale_page = look_up(pos + 16 * ct);
     };
+    const size_t page_bytes = (size_t)c.heads * c.tokens * c.width;
+    const int8_t* k_head = c.k + (size_t)head * c.tokens * c.width;
+    const int8_t* v_head = c.v + (size_t)head * c.tokens * c.width;
     auto load = [&](int j) {
       const int pos = (begin + j) * kKeys;
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
         kq[i] = vq[i] = make_uint4(0u, 0u, 0u, 0u);
         if (pages[i] >= 0) {
-          const size_t from = c.row(pages[i], head, (pos + row_of(i)) & (c.tokens - 1)) + channel_of(i);
-          kq[i] = __ldg(reinterpret_cast<const uint4*>(c.k + from));
-          vq[i] = __ldg(reinterpret_cast<const uint4*>(c.v + from));
+          const size_t from = pages[i] * page_bytes + ((pos + row_of(i)) & (c.tokens - 1)) * c.width + channel_of(i);
+          kq[i] = __ldg(reinterpret_cast<const uint4*>(k_head + from));
+          vq[i] = __ldg(reinterpret_cast<const uint4*>(v_head + from));
         }
       }
       if (ct < 4) {
