@@ -499,7 +499,7 @@ struct TileShape {
   static constexpr int kQueries = kStages * 2 * kOperand;  // [half][term]
   static constexpr int kMeta = kQueries + (kQInSmem ? 2 * TERMS * kQTile : 0);
   static constexpr int kBars = kMeta + kStages * 32;
-  static constexpr int kBytes = kBars + 160;
+  static constexpr int kBytes = kBars + 192;
 };
 
 // D (tensor memory) (+)= A (tensor memory, or shared memory) * B (shared memory), FP16.
@@ -570,8 +570,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* s_full = bars + 2 * kStages;  // [half][buffer] scores -> softmax
   uint64_t* p_full = s_full + 4;          // [half][buffer] softmax -> products: a half may be two tiles ahead
   uint64_t* q_full = p_full + 4;          // [half]
-  uint64_t* o_full = q_full + 2;          // [half] O += P V is done
-  uint64_t* drained = o_full + 2;
+  uint64_t* o_full = q_full + 2;          // [half][tile & 1] O += P V is done
+  uint64_t* drained = o_full + 4;
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drained + 1);
   int* failed = reinterpret_cast<int*>(tmem_at + 1);
   float* meta = reinterpret_cast<float*>(smem + S::kMeta);  // [stage][4 K scales, 4 V scales] of 16 tokens each
@@ -582,11 +582,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
     for (int h = 0; h < 2; ++h) {
       for (int k = 0; k < 2; ++k) {
+        tc::bar_init(&o_full[2 * h + k], 1);
         tc::bar_init(&s_full[2 * h + k], 1);
         tc::bar_init(&p_full[2 * h + k], kHalfRows);
       }
       tc::bar_init(&q_full[h], kHalfRows);
-      tc::bar_init(&o_full[h], 1);
     }
     tc::bar_init(drained, 1);
     *failed = 0;
@@ -668,6 +668,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       tc::fence_before_sync();
       tc::bar_arrive(&q_full[h]);
     }
+    // The products of tile j.  A waiter may be a tile behind them or ahead, so
+    // each parity of tiles has a barrier: a wait is exact within one phase only.
+    auto o_done = [&](int j) { return tc::bar_wait(&o_full[2 * h + (j & 1)], (j >> 1) & 1); };
     for (int j = 0; j < count; ++j) {
       const int stage = j % kStages;
       // both: the tile's scales (converters) and its scores (products)
@@ -720,7 +723,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         ev = top;
         if (j > 0) {
           // the products before this tile's are in O
-          alive = __all_sync(kFull, tc::bar_wait(&o_full[h], (j - 1) & 1));
+          alive = __all_sync(kFull, o_done(j - 1));
           if (!alive) break;
           tc::fence_after_sync();
 #pragma unroll
@@ -770,10 +773,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       tc::fence_before_sync();
       tc::bar_arrive(&p_full[2 * h + (j & 1)]);
     }
-    // the scores of the last tile vouch for the products three tiles back: both
-    // later phases are waited for in order, a parity is exact for one only
-    if (count > 1 && alive) alive = __all_sync(kFull, tc::bar_wait(&o_full[h], (count - 2) & 1));
-    if (count > 0 && alive) alive = __all_sync(kFull, tc::bar_wait(&o_full[h], (count - 1) & 1));
+    if (count > 0 && alive) alive = __all_sync(kFull, o_done(count - 1));
     if (!alive) *failed = 1;
     tc::fence_after_sync();
     const float inverse = l == 0.f ? 0.f : power_of_two(ev) * (1.f / kProbScale) / l;
@@ -951,7 +951,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     // shape are ordered among themselves).
     auto next_scores = [&](int h, int i) {
       if (i < 2 || i >= counts[h] || !ok) return;
-      ok = __all_sync(kFull, full(i) && tc::bar_wait(&o_full[h], i & 1));
+      ok = __all_sync(kFull, full(i) && tc::bar_wait(&o_full[2 * h + (i & 1)], ((i - 2) >> 1) & 1));
       tc::fence_after_sync();
       if (ok && elected) {
         scores(h, i);
@@ -967,7 +967,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           tc::fence_after_sync();
           if (ok && elected) {
             values(h, j);
-            tc::commit(&o_full[h]);
+            tc::commit(&o_full[2 * h + (j & 1)]);
             if (h == (both ? 1 : 0)) tc::commit(&kv_free[j % kStages]);
           }
           __syncwarp();
