@@ -43,17 +43,6 @@ class AdamWC(ctypes.Structure):
         "learning_rate", "weight_decay", "beta1", "beta2", "epsilon")]
 
 
-class KvCacheC(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + \
-               [(n, ctypes.c_uint32) for n in ("pages", "heads", "page_tokens", "width")]
-
-
-class CacheRowsC(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_void_p) for n in ("table", "lengths", "offsets")] + \
-               [(n, ctypes.c_size_t) for n in ("table_stride", "rows")] + \
-               [(n, ctypes.c_uint32) for n in ("table_pages", "batch")]
-
-
 class MeshError(RuntimeError):
     """A nonzero status from the library, with its code and message."""
 
@@ -146,24 +135,14 @@ SIGNATURES = {
                       [ctypes.c_void_p] * 6),
     "mb_op_adamw": (ctypes.c_int, [ctypes.c_void_p] * 4 + [ctypes.c_size_t, ctypes.POINTER(AdamWC),
                                                            ctypes.c_uint32, ctypes.c_void_p]),
-    "mb_op_cache_write": (ctypes.c_int, [ctypes.POINTER(KvCacheC), ctypes.POINTER(CacheRowsC), ctypes.c_uint32] +
-                          [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_size_t] * 2 +
-                          [ctypes.c_uint32, ctypes.c_uint32, ctypes.c_void_p, ctypes.c_void_p]),
-    "mb_op_cache_read": (ctypes.c_int, [ctypes.POINTER(KvCacheC), ctypes.POINTER(CacheRowsC), ctypes.c_uint32,
-                                        ctypes.c_void_p, ctypes.c_uint32, ctypes.c_void_p, ctypes.c_void_p,
-                                        ctypes.c_uint32, ctypes.c_void_p, ctypes.c_void_p]),
+    # argument structures of the serving operators, packed by ops.py
+    "mb_op_cache_write": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
+    "mb_op_cache_read": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
     "mb_op_cache_attention_workspace": (ctypes.c_int, [ctypes.c_uint32, ctypes.c_size_t] + [ctypes.c_uint32] * 5 +
                                         [c_size_p]),
-    "mb_op_cache_attention": (ctypes.c_int, [ctypes.POINTER(KvCacheC), ctypes.POINTER(CacheRowsC), ctypes.c_void_p,
-                                             ctypes.c_void_p, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_uint32,
-                                             ctypes.c_uint32, ctypes.c_uint32, ctypes.c_float, ctypes.c_uint32,
-                                             ctypes.c_uint32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
-                                             ctypes.c_size_t, ctypes.c_void_p, ctypes.c_void_p]),
-    "mb_op_token_logprobs": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_uint32, ctypes.c_size_t, ctypes.c_size_t,
-                                            ctypes.c_uint32, ctypes.c_void_p, ctypes.c_uint32] +
-                             [ctypes.c_void_p] * 7),
-    "mb_op_token_logprobs_backward": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_uint32, ctypes.c_size_t,
-                                                     ctypes.c_size_t, ctypes.c_uint32] + [ctypes.c_void_p] * 8),
+    "mb_op_cache_attention": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
+    "mb_op_token_logprobs": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
+    "mb_op_token_logprobs_backward": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
     "mb_gpt_checkpoint_write": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(GptConfigC), c_u32_p, ctypes.c_size_t,
                                                c_float_p, ctypes.c_size_t]),
     "mb_gpt_checkpoint_read": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(GptConfigC), c_u32_p, c_size_p,

@@ -1032,14 +1032,6 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---------------------------------------------------------------- host side
-inline int sm_count() {
-  int dev = 0, sms = 1;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    throw Error(MB_ERR_CUDA, "no CUDA device");
-  return sms;
-}
-
 struct Plan {
   bool tiles;          // the tile kernel, else the split kernel
   int blocks_per_seq;  // row blocks of a sequence
@@ -1082,8 +1074,8 @@ void launch_rows(const View& c, const Batch& t, const Queries& q, const Plan& p,
   void (*kernel)(View, Batch, Queries, Partials, int);
   if constexpr (TILES) kernel = attend_tiles<T, D>;
   else kernel = attend_split<T, D>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  require(e == cudaSuccess, std::string("cache attention: ") + cudaGetErrorString(e), MB_ERR_CUDA);
+  static DeviceOnce once;  // one a kernel
+  once([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
   kernel<<<dim3((unsigned)(p.units * p.chunks), (unsigned)c.heads), TILES ? kTileThreads : kSplitThreads, bytes, st>>>(
       c, t, q, part, p.blocks_per_seq);
   launched("cache attention");
@@ -1097,7 +1089,7 @@ void launch_rows(const View& c, const Batch& t, const Queries& q, const Plan& p,
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, join_chunks<T, D, ROWS>, c, t, q, part, p.blocks_per_seq);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, join_chunks<T, D, ROWS>, c, t, q, part, p.blocks_per_seq);
   require(e == cudaSuccess, std::string("cache attention join: ") + cudaGetErrorString(e), MB_ERR_CUDA);
 }
 
@@ -1123,31 +1115,33 @@ int mb_op_cache_attention_workspace(uint32_t batch, size_t rows, uint32_t q_head
   });
 }
 
-int mb_op_cache_attention(const mb_kv_cache* cache, const mb_cache_rows* where, const int32_t* first, const void* q,
-                          size_t q_row_stride, size_t q_head_stride, uint32_t q_heads, uint32_t head_dim,
-                          uint32_t dtype, float scale, uint32_t max_new, uint32_t max_tokens, void* out, float* lse,
-                          void* workspace, size_t workspace_bytes, int* d_status, void* stream) {
+int mb_op_cache_attention(const mb_cache_attention_args* a, void* stream) {
   using namespace mb::cache;
   return mb::guarded([&] {
-    const View c = view_of(cache, head_dim);
-    const Batch t = batch_of(where, max_new);
+    mb::need(a, "args");
+    const View c = view_of(a->cache, a->head_dim);
+    const uint32_t q_heads = a->q_heads, max_new = a->max_new, max_tokens = a->max_tokens;
+    const Batch t = batch_of(a->where, max_new);
     mb::require(q_heads >= 1 && q_heads % c.heads == 0 && q_heads / c.heads <= 1024,
                 "the cache's heads must divide q_heads");
-    mb::require(std::isfinite(scale), "scale must be finite");
+    mb::require(std::isfinite(a->scale), "scale must be finite");
     mb::require(max_tokens <= (uint32_t)INT_MAX, "max_tokens must be below 2^31");
     if (t.rows == 0 || t.count == 0) return;
     mb::require(max_new >= 1, "max_new must be positive where there are rows");
+    const void* q = a->q;
+    void *out = a->out, *workspace = a->workspace;
+    const size_t workspace_bytes = a->workspace_bytes;
     mb::need(q, "q");
     mb::need(out, "out");
-    const Queries qs{q, q_row_stride, q_head_stride, out, lse, (int)q_heads, (int)(q_heads / c.heads), (int)head_dim,
-                     scale * mb::kLog2e, first, (int)max_new, d_status};
+    const Queries qs{q, a->q_row_stride, a->q_head_stride, out, a->lse, (int)q_heads, (int)(q_heads / c.heads),
+                     (int)a->head_dim, a->scale * mb::kLog2e, a->first, (int)max_new, a->d_status};
     const Plan p = make_plan(t.count, t.rows, c.heads, qs.group, c.width, max_new, max_tokens);
     mb::require(p.units * p.chunks <= (size_t)INT_MAX, "too many row blocks for one call");
     mb::require(p.workspace == 0 || (workspace != nullptr && workspace_bytes >= p.workspace &&
                                      reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
                 "workspace missing, too small or not 16-byte aligned");
     cudaStream_t st = (cudaStream_t)stream;
-    mb::with_dtype(dtype, [&](auto tag) {
+    mb::with_dtype(a->dtype, [&](auto tag) {
       using T = typename decltype(tag)::type;
       for (const void* x : {q, (const void*)out})
         mb::require(reinterpret_cast<uintptr_t>(x) % sizeof(T) == 0, "q and out must be aligned to their elements");

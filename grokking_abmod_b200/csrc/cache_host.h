@@ -9,8 +9,8 @@
 namespace mb {
 namespace cache {
 
-inline View view_of(const mb_kv_cache* c, uint32_t head_dim) {
-  need(c, "cache");
+inline View view_of(const mb_kv_cache& given, uint32_t head_dim) {
+  const mb_kv_cache* c = &given;
   need(c->k, "cache k");
   need(c->v, "cache v");
   need(c->k_scale, "cache k_scale");
@@ -32,8 +32,8 @@ inline View view_of(const mb_kv_cache* c, uint32_t head_dim) {
               (int)c->width};
 }
 
-inline Batch batch_of(const mb_cache_rows* r, uint32_t max_new) {
-  need(r, "rows");
+inline Batch batch_of(const mb_cache_rows& given, uint32_t max_new) {
+  const mb_cache_rows* r = &given;
   require(r->batch <= (1u << 24), "batch must be at most 2^24");
   require(r->rows <= (size_t)INT_MAX, "rows must be below 2^31");
   require(max_new <= (uint32_t)INT_MAX, "max_new must be below 2^31");

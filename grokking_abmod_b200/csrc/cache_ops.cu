@@ -235,22 +235,23 @@ Rows<T> make_rows(const void* p, size_t row_stride, size_t head_stride) {
 
 extern "C" {
 
-int mb_op_cache_write(const mb_kv_cache* cache, const mb_cache_rows* where, uint32_t head_dim, const void* k,
-                      size_t k_row_stride, size_t k_head_stride, const void* v, size_t v_row_stride,
-                      size_t v_head_stride, uint32_t dtype, uint32_t max_new, int* d_status, void* stream) {
+int mb_op_cache_write(const mb_cache_write_args* a, void* stream) {
   using namespace mb::cache;
   return mb::guarded([&] {
-    const View c = view_of(cache, head_dim);
-    const Batch t = batch_of(where, max_new);
+    mb::need(a, "args");
+    const View c = view_of(a->cache, a->head_dim);
+    const Batch t = batch_of(a->where, a->max_new);
+    const uint32_t max_new = a->max_new;
     if (t.rows == 0 || max_new == 0 || t.count == 0) return;
-    mb::need(k, "k");
-    mb::need(v, "v");
+    mb::need(a->k, "k");
+    mb::need(a->v, "v");
     const int page_slots = (int)(((size_t)max_new + c.tokens - 2) / c.tokens + 1);
     const size_t units = (size_t)t.count * page_slots * c.heads;
     cudaStream_t st = (cudaStream_t)stream;
-    mb::with_dtype(dtype, [&](auto tag) {
+    mb::with_dtype(a->dtype, [&](auto tag) {
       using T = typename decltype(tag)::type;
-      const Rows<T> kr = make_rows<T>(k, k_row_stride, k_head_stride), vr = make_rows<T>(v, v_row_stride, v_head_stride);
+      const Rows<T> kr = make_rows<T>(a->k, a->k_row_stride, a->k_head_stride);
+      const Rows<T> vr = make_rows<T>(a->v, a->v_row_stride, a->v_head_stride);
       // a warp where it can hold a page's new rows in registers, else a CTA
       const size_t vectors = std::min<size_t>(max_new, c.tokens) * c.width / mb::Element<T>::kVec;
       const bool warp = vectors <= 32 * kHeld;
@@ -258,26 +259,28 @@ int mb_op_cache_write(const mb_kv_cache* cache, const mb_cache_rows* where, uint
       mb::require(blocks <= (size_t)INT_MAX, "too many pages for one call");
       const dim3 grid((unsigned)blocks, 2);
       if (warp)
-        write_pages<T, 32><<<grid, kThreads, 0, st>>>(c, t, kr, vr, (int)head_dim, page_slots, d_status);
+        write_pages<T, 32><<<grid, kThreads, 0, st>>>(c, t, kr, vr, (int)a->head_dim, page_slots, a->d_status);
       else
-        write_pages<T, kThreads><<<grid, kThreads, 0, st>>>(c, t, kr, vr, (int)head_dim, page_slots, d_status);
+        write_pages<T, kThreads><<<grid, kThreads, 0, st>>>(c, t, kr, vr, (int)a->head_dim, page_slots, a->d_status);
       mb::launched("cache write");
     });
   });
 }
 
-int mb_op_cache_read(const mb_kv_cache* cache, const mb_cache_rows* where, uint32_t head_dim, const int32_t* first,
-                     uint32_t tokens, void* k_out, void* v_out, uint32_t dtype, int* d_status, void* stream) {
+int mb_op_cache_read(const mb_cache_read_args* a, void* stream) {
   using namespace mb::cache;
   return mb::guarded([&] {
-    const View c = view_of(cache, head_dim);
-    const Batch t = batch_of(where, 0);
+    mb::need(a, "args");
+    const uint32_t head_dim = a->head_dim, tokens = a->tokens;
+    const View c = view_of(a->cache, head_dim);
+    const Batch t = batch_of(a->where, 0);
     mb::require(tokens <= (1u << 30), "tokens must be at most 2^30");
     if (tokens == 0 || t.count == 0) return;
+    void *k_out = a->k_out, *v_out = a->v_out;
     mb::need(k_out, "k_out");
     mb::need(v_out, "v_out");
     cudaStream_t st = (cudaStream_t)stream;
-    mb::with_dtype(dtype, [&](auto tag) {
+    mb::with_dtype(a->dtype, [&](auto tag) {
       using T = typename decltype(tag)::type;
       constexpr int VEC = mb::Element<T>::kVec;
       for (const void* p : {(const void*)k_out, (const void*)v_out})
@@ -292,11 +295,11 @@ int mb_op_cache_read(const mb_kv_cache* cache, const mb_cache_rows* where, uint3
                   "too many tokens for one call");
       const dim3 grid((unsigned)(runs * t.count), (unsigned)((columns + here - 1) / here), 2);
       if (vector)
-        read_pages<T, VEC><<<grid, kThreads, 0, st>>>(c, t, first, (int)tokens, (int)head_dim, columns, here,
-                                                      (int)runs, (T*)k_out, (T*)v_out, d_status);
+        read_pages<T, VEC><<<grid, kThreads, 0, st>>>(c, t, a->first, (int)tokens, (int)head_dim, columns, here,
+                                                      (int)runs, (T*)k_out, (T*)v_out, a->d_status);
       else
-        read_pages<T, 1><<<grid, kThreads, 0, st>>>(c, t, first, (int)tokens, (int)head_dim, columns, here,
-                                                    (int)runs, (T*)k_out, (T*)v_out, d_status);
+        read_pages<T, 1><<<grid, kThreads, 0, st>>>(c, t, a->first, (int)tokens, (int)head_dim, columns, here,
+                                                    (int)runs, (T*)k_out, (T*)v_out, a->d_status);
       mb::launched("cache read");
     });
   });

@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "host.h"
 
 namespace mb {
@@ -96,6 +98,44 @@ void with_dtype(uint32_t dtype, F&& f) {
 }
 
 inline size_t dtype_bytes(uint32_t dtype) { return dtype == MB_F32 ? 4 : 2; }
+
+constexpr int kMaxDevices = 64;
+
+inline int current_device() {
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  require(e == cudaSuccess && dev < kMaxDevices, "no usable CUDA device", MB_ERR_CUDA);
+  return dev;
+}
+
+// SMs of the current device.
+inline int sm_count() {
+  static std::atomic<int> known[kMaxDevices];
+  const int dev = current_device();
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    const cudaError_t e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    require(e == cudaSuccess, "no usable CUDA device", MB_ERR_CUDA);
+    known[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+// A kernel attribute, set once on each device.
+class DeviceOnce {
+ public:
+  template <class F>
+  void operator()(F&& set) {
+    const uint64_t bit = 1ull << current_device();
+    if (done_.load(std::memory_order_acquire) & bit) return;
+    const cudaError_t e = set();
+    if (e != cudaSuccess) throw Error(MB_ERR_CUDA, std::string("kernel attribute: ") + cudaGetErrorString(e));
+    done_.fetch_or(bit, std::memory_order_release);
+  }
+
+ private:
+  std::atomic<uint64_t> done_{0};
+};
 
 inline void launched(const char* what) {
   const cudaError_t e = cudaGetLastError();

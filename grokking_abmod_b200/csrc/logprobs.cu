@@ -478,13 +478,6 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-inline int sm_count() {
-  int dev = 0, sms = 1;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    throw Error(MB_ERR_CUDA, "no CUDA device");
-  return sms;
-}
-
 // CTAs per row: enough rows fill the GPU with one each; few rows are cut into
 // up to 8 shares (the portable cluster size) of at least 4096 elements.
 inline unsigned row_shares(size_t rows, int vocab) {
@@ -540,59 +533,59 @@ void launch_forward(const T* x, size_t stride, size_t rows, uint32_t vocab, cons
 
 extern "C" {
 
-int mb_op_token_logprobs(const void* logits, uint32_t dtype, size_t row_stride, size_t rows, uint32_t vocab,
-                         const int32_t* tokens, uint32_t top, float* logprob, float* entropy, float* lse,
-                         float* top_logprob, int32_t* top_index, int* d_status, void* stream) {
+int mb_op_token_logprobs(const mb_token_logprobs_args* a, void* stream) {
   using namespace mb::logprobs;
   return mb::guarded([&] {
-    mb::need(logits, "logits");
-    mb::need(tokens, "tokens");
-    mb::need(logprob, "logprob");
-    mb::need(entropy, "entropy");
-    mb::need(lse, "lse");
-    shape(rows, vocab, row_stride);
-    mb::require(top <= (uint32_t)kMaxTop && top <= vocab, "top must be in 0..32 and at most vocab");
+    mb::need(a, "args");
+    const uint32_t top = a->top;
+    mb::need(a->logits, "logits");
+    mb::need(a->tokens, "tokens");
+    mb::need(a->logprob, "logprob");
+    mb::need(a->entropy, "entropy");
+    mb::need(a->lse, "lse");
+    shape(a->rows, a->vocab, a->row_stride);
+    mb::require(top <= (uint32_t)kMaxTop && top <= a->vocab, "top must be in 0..32 and at most vocab");
     if (top) {
-      mb::need(top_logprob, "top_logprob");
-      mb::need(top_index, "top_index");
+      mb::need(a->top_logprob, "top_logprob");
+      mb::need(a->top_index, "top_index");
     }
-    const Out o{logprob, entropy, lse, top_logprob, top_index, d_status};
-    cudaStream_t st = (cudaStream_t)stream;
-    mb::with_dtype(dtype, [&](auto tag) {
+    const Out o{a->logprob, a->entropy, a->lse, a->top_logprob, a->top_index, a->d_status};
+    mb::with_dtype(a->dtype, [&](auto tag) {
       using T = typename decltype(tag)::type;
-      aligned(logits, sizeof(T), "logits");
-      launch_forward<T>(static_cast<const T*>(logits), row_stride, rows, vocab, tokens, top, o, st);
+      aligned(a->logits, sizeof(T), "logits");
+      launch_forward<T>(static_cast<const T*>(a->logits), a->row_stride, a->rows, a->vocab, a->tokens, top, o,
+                        (cudaStream_t)stream);
       mb::launched("token log-probabilities");
     });
   });
 }
 
-int mb_op_token_logprobs_backward(const void* logits, uint32_t dtype, size_t row_stride, size_t rows, uint32_t vocab,
-                                  const int32_t* tokens, const float* lse, const float* entropy,
-                                  const float* dlogprob, const float* dentropy, void* dlogits, int* d_status,
-                                  void* stream) {
+int mb_op_token_logprobs_backward(const mb_token_logprobs_backward_args* a, void* stream) {
   using namespace mb::logprobs;
   return mb::guarded([&] {
-    mb::need(logits, "logits");
-    mb::need(tokens, "tokens");
-    mb::need(lse, "lse");
-    mb::need(dlogits, "dlogits");
-    if (dentropy) mb::need(entropy, "entropy");
-    shape(rows, vocab, row_stride);
-    const GradIn in{tokens, lse, entropy, dlogprob, dentropy, d_status};
+    mb::need(a, "args");
+    mb::need(a->logits, "logits");
+    mb::need(a->tokens, "tokens");
+    mb::need(a->lse, "lse");
+    mb::need(a->dlogits, "dlogits");
+    if (a->dentropy) mb::need(a->entropy, "entropy");
+    shape(a->rows, a->vocab, a->row_stride);
+    const GradIn in{a->tokens, a->lse, a->entropy, a->dlogprob, a->dentropy, a->d_status};
     cudaStream_t st = (cudaStream_t)stream;
-    mb::with_dtype(dtype, [&](auto tag) {
+    mb::with_dtype(a->dtype, [&](auto tag) {
       using T = typename decltype(tag)::type;
-      aligned(logits, sizeof(T), "logits");
-      aligned(dlogits, sizeof(T), "dlogits");
-      const T* x = static_cast<const T*>(logits);
-      T* d = static_cast<T*>(dlogits);
+      aligned(a->logits, sizeof(T), "logits");
+      aligned(a->dlogits, sizeof(T), "dlogits");
+      const T* x = static_cast<const T*>(a->logits);
+      T* d = static_cast<T*>(a->dlogits);
+      const size_t rows = a->rows;
+      const uint32_t vocab = a->vocab;
       if (vocab <= (uint32_t)kRowLanes) {
         const unsigned blocks = (unsigned)((rows + kWarps - 1) / kWarps);
-        backward_rows<T, 32><<<blocks, kThreads, 0, st>>>(x, row_stride, rows, (int)vocab, in, d);
+        backward_rows<T, 32><<<blocks, kThreads, 0, st>>>(x, a->row_stride, rows, (int)vocab, in, d);
       } else {
         backward_rows<T, kThreads><<<dim3((unsigned)rows, row_shares(rows, (int)vocab)), kThreads, 0, st>>>(
-            x, row_stride, rows, (int)vocab, in, d);
+            x, a->row_stride, rows, (int)vocab, in, d);
       }
       mb::launched("token log-probability gradient");
     });

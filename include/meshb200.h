@@ -339,15 +339,39 @@ typedef struct mb_cache_rows {
  * it.  An infinity or NaN makes the page and head's scale NaN until the
  * page's first token is written again.  max_new: at least the largest number
  * of new rows of a sequence. */
-int mb_op_cache_write(const mb_kv_cache* cache, const mb_cache_rows* where, uint32_t head_dim, const void* k,
-                      size_t k_row_stride, size_t k_head_stride, const void* v, size_t v_row_stride,
-                      size_t v_head_stride, uint32_t dtype, uint32_t max_new, int* d_status, void* stream);
+typedef struct mb_cache_write_args {
+  mb_kv_cache cache;
+  mb_cache_rows where;
+  const void* k;
+  const void* v;
+  size_t k_row_stride;
+  size_t k_head_stride;
+  size_t v_row_stride;
+  size_t v_head_stride;
+  int* d_status;
+  uint32_t head_dim;
+  uint32_t dtype;
+  uint32_t max_new;
+  uint32_t reserved;
+} mb_cache_write_args;
+int mb_op_cache_write(const mb_cache_write_args* args, void* stream);
 /* Reads positions first[b] .. first[b] + tokens - 1 (first NULL: from 0) of
  * every sequence: k_out, v_out [batch][tokens][heads][head_dim], 0 outside
- * 0 .. lengths[b] - 1, NaN for a page number out of range.  offsets and rows
- * are not used. */
-int mb_op_cache_read(const mb_kv_cache* cache, const mb_cache_rows* where, uint32_t head_dim, const int32_t* first,
-                     uint32_t tokens, void* k_out, void* v_out, uint32_t dtype, int* d_status, void* stream);
+ * 0 .. lengths[b] - 1, NaN for a page number out of range.  where's offsets
+ * and rows are not used. */
+typedef struct mb_cache_read_args {
+  mb_kv_cache cache;
+  mb_cache_rows where;
+  const int32_t* first;
+  void* k_out;
+  void* v_out;
+  int* d_status;
+  uint32_t head_dim;
+  uint32_t dtype;
+  uint32_t tokens;
+  uint32_t reserved;
+} mb_cache_read_args;
+int mb_op_cache_read(const mb_cache_read_args* args, void* stream);
 /* Attention of the new rows over their sequences' cached tokens (written
  * before, the new ones too): row i of n of sequence b sees positions
  * first[b] (NULL: 0) .. lengths[b] - n + i.  Query head a reads key head
@@ -356,14 +380,30 @@ int mb_op_cache_read(const mb_kv_cache* cache, const mb_cache_rows* where, uint3
  * by scale * log2(e).  A row that sees nothing gives 0 and -inf; rows of a
  * sequence whose numbers do not fit, and rows past max_new, NaN.  max_tokens:
  * about the largest length, by which long sequences are cut over the GPU (any
- * value is right).  workspace: 16-byte aligned, as many bytes as
- * mb_op_cache_attention_workspace says for the same sizes. */
+ * value is right).  workspace: 16-byte aligned, workspace_bytes at least what
+ * mb_op_cache_attention_workspace says for the same sizes on this device. */
+typedef struct mb_cache_attention_args {
+  mb_kv_cache cache;
+  mb_cache_rows where;
+  const int32_t* first;
+  const void* q;
+  void* out;
+  float* lse;
+  void* workspace;
+  int* d_status;
+  size_t q_row_stride;
+  size_t q_head_stride;
+  size_t workspace_bytes;
+  uint32_t q_heads;
+  uint32_t head_dim;
+  uint32_t dtype;
+  uint32_t max_new;
+  uint32_t max_tokens;
+  float scale;
+} mb_cache_attention_args;
 int mb_op_cache_attention_workspace(uint32_t batch, size_t rows, uint32_t q_heads, uint32_t kv_heads,
                                     uint32_t head_dim, uint32_t max_new, uint32_t max_tokens, size_t* bytes);
-int mb_op_cache_attention(const mb_kv_cache* cache, const mb_cache_rows* where, const int32_t* first, const void* q,
-                          size_t q_row_stride, size_t q_head_stride, uint32_t q_heads, uint32_t head_dim,
-                          uint32_t dtype, float scale, uint32_t max_new, uint32_t max_tokens, void* out, float* lse,
-                          void* workspace, size_t workspace_bytes, int* d_status, void* stream);
+int mb_op_cache_attention(const mb_cache_attention_args* args, void* stream);
 /* Per row of logits [rows][vocab] (rows row_stride elements apart): logprob =
  * ln softmax at tokens[row] (0 for -1, MB_IGNORE_TARGET), entropy in nats,
  * lse = ln sum e^x, and the `top` (0..32) most likely tokens by (logit
@@ -371,18 +411,43 @@ int mb_op_cache_attention(const mb_kv_cache* cache, const mb_cache_rows* where, 
  * top_index [rows][top].  Logits of -inf are masked tokens: probability 0.  A
  * row with nothing else gives logprob -inf, entropy 0, lse -inf.  A token
  * out of range gives NaN and status bit 2. */
-int mb_op_token_logprobs(const void* logits, uint32_t dtype, size_t row_stride, size_t rows, uint32_t vocab,
-                         const int32_t* tokens, uint32_t top, float* logprob, float* entropy, float* lse,
-                         float* top_logprob, int32_t* top_index, int* d_status, void* stream);
+typedef struct mb_token_logprobs_args {
+  const void* logits;
+  const int32_t* tokens;
+  float* logprob;
+  float* entropy;
+  float* lse;
+  float* top_logprob;
+  int32_t* top_index;
+  int* d_status;
+  size_t row_stride;
+  size_t rows;
+  uint32_t vocab;
+  uint32_t dtype;
+  uint32_t top;
+  uint32_t reserved;
+} mb_token_logprobs_args;
+int mb_op_token_logprobs(const mb_token_logprobs_args* args, void* stream);
 /* The gradient of sum(dlogprob . logprob + dentropy . entropy) with respect
  * to the logits, from the forward's lse and entropy: dlogits [rows][vocab] in
  * the type of the logits.  dlogprob or dentropy may be NULL (zeros); entropy
  * may be NULL with dentropy.  Ignored tokens take no part in dlogprob; rows
  * with nothing but masked tokens get 0. */
-int mb_op_token_logprobs_backward(const void* logits, uint32_t dtype, size_t row_stride, size_t rows, uint32_t vocab,
-                                  const int32_t* tokens, const float* lse, const float* entropy,
-                                  const float* dlogprob, const float* dentropy, void* dlogits, int* d_status,
-                                  void* stream);
+typedef struct mb_token_logprobs_backward_args {
+  const void* logits;
+  const int32_t* tokens;
+  const float* lse;
+  const float* entropy;
+  const float* dlogprob;
+  const float* dentropy;
+  void* dlogits;
+  int* d_status;
+  size_t row_stride;
+  size_t rows;
+  uint32_t vocab;
+  uint32_t dtype;
+} mb_token_logprobs_backward_args;
+int mb_op_token_logprobs_backward(const mb_token_logprobs_backward_args* args, void* stream);
 
 /* The same mesh stack backward without any allocation (no reference
  * counterpart: the reference always allocates its workspace).  For callers
