@@ -1,8 +1,8 @@
 // Log-probabilities of given tokens from rows of logits, with the rows'
 // entropy and their k most likely tokens, and the gradient of the first two.
 //
-//   m = max_j x_j, d_j = m - x_j, s = sum_j e^-d_j
-//   lse = m + ln s, logprob = x_t - lse, H = ln s + (sum_j e^-d_j d_j) / s
+//   m = max_j x_j, d_j = x_j - m, s = sum_j e^d_j
+//   lse = m + ln s, logprob = x_t - lse, H = ln s - (sum_j e^d_j d_j) / s
 //   dx_j = g (1[j = t] - p_j) - h p_j (ln p_j + H),  p_j = e^(x_j - lse)
 //
 // H is a sum of nonnegative terms, so nothing cancels where one token takes
@@ -11,15 +11,17 @@
 // maximum rises, and the triples are joined at the end in a fixed order.
 //
 // Top tokens order by (value descending, index ascending), a total order, so
-// ties go to the lowest index whatever the launch shape.  Values map to
-// integers in that order; a warp holds its candidates sorted, one a lane, and
-// a new element enters only if it beats the k-th best that any warp of its
-// CTA has so far - after the first elements of a row that is rare, and costs
-// one compare per 16 or 32 elements.
+// ties go to the lowest index whatever the launch shape.  The threads' maxima
+// are known when the sums are: at least k elements reach the k-th largest of
+// them, and few more do.  Only the threads whose maximum reaches it (k of
+// them) look at their elements again; what they find is sorted in registers.
+// Rows where too many elements tie there, or hold NaN or nothing but masked
+// tokens, go through a slower list that is right for any row.
 
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 #include "dtype.cuh"
@@ -33,12 +35,13 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kUnroll = 4;      // 16-byte vectors a thread has in flight
 constexpr int kRowLanes = 1024; // vocabularies up to here take one warp per row
+constexpr int kFewTop = 6;      // so many top tokens of a row in registers are picked one by one, more are sorted
 constexpr unsigned kFull = 0xFFFFFFFFu;
 
 using u64 = unsigned long long;
 
-// Running statistics in base-2 units: s = sum 2^-t, a = sum 2^-t t with
-// t = (m - x) log2 e.
+// Running statistics in base-2 units: s = sum 2^t, a = sum 2^t t with
+// t = (x - m) log2 e <= 0.
 struct Stats {
   float m, s, a;
 };
@@ -48,8 +51,8 @@ __device__ __forceinline__ Stats empty_stats() { return Stats{-INFINITY, 0.f, 0.
 // Moves the statistics to a maximum m >= s.m.
 __device__ __forceinline__ Stats rebase(Stats s, float m) {
   if (s.m == -INFINITY) return Stats{m, s.s, s.a};  // nothing counted (or only NaN terms)
-  const float t = (m - s.m) * kLog2e;
-  const float c = ex2_ftz(-t);
+  const float t = fmaxf((s.m - m) * kLog2e, -1e30f);
+  const float c = ex2_ftz(t);
   return Stats{m, s.s * c, c * fmaf(t, s.s, s.a)};
 }
 
@@ -62,14 +65,19 @@ __device__ __forceinline__ Stats join(Stats p, Stats q) {
   return Stats{m, p.s + q.s, p.a + q.a};
 }
 
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
+  return v;
+}
+
 __device__ __forceinline__ Stats warp_join(Stats v) {
+  const float m = warp_max(v.m);
+  if (m != -INFINITY) v = rebase(v, m);
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
-    Stats w;
-    w.m = __shfl_xor_sync(kFull, v.m, o);
-    w.s = __shfl_xor_sync(kFull, v.s, o);
-    w.a = __shfl_xor_sync(kFull, v.a, o);
-    v = join(v, w);
+    v.s += __shfl_xor_sync(kFull, v.s, o);
+    v.a += __shfl_xor_sync(kFull, v.a, o);
   }
   return v;
 }
@@ -79,16 +87,16 @@ template <int N>
 __device__ __forceinline__ void accumulate(Stats& st, const float (&x)[N], float mx) {
   if (mx > st.m) st = rebase(st, mx);
   // all of them -inf so far: differences from 0 keep the terms at 2^-inf = 0
-  const float m = st.m == -INFINITY ? 0.f : st.m;
-  const float2 mm = splat2(m), scale = splat2(kLog2e);
+  const float2 less = splat2(st.m == -INFINITY ? 0.f : -st.m), scale = splat2(kLog2e);
   float2 s = make_float2(0.f, 0.f), a = make_float2(0.f, 0.f);
 #pragma unroll
   for (int i = 0; i < N; i += 2) {
-    const float2 t = mul2(add2(mm, make_float2(-x[i], -x[i + 1])), scale);
-    const float2 e = make_float2(ex2_ftz(-t.x), ex2_ftz(-t.y));
+    const float2 t = mul2(add2(make_float2(x[i], x[i + 1]), less), scale);
+    const float2 e = make_float2(ex2_ftz(t.x), ex2_ftz(t.y));
     s = add2(s, e);
-    // a masked logit (-inf) has t = +inf and e = 0: its term is 0, not NaN
-    a = fma2(e, make_float2(fminf(t.x, 1e30f), fminf(t.y, 1e30f)), a);
+    // a masked logit (-inf, or the type's lowest) may have t = -inf and has
+    // e = 0: its term is 0, not NaN
+    a = fma2(e, make_float2(fmaxf(t.x, -1e30f), fmaxf(t.y, -1e30f)), a);
   }
   st.s += s.x + s.y;
   st.a += a.x + a.y;
@@ -132,6 +140,43 @@ __device__ __forceinline__ void offer(u64& mine, u64 key, u64 floor, int top, in
   }
 }
 
+// Sorting across a warp, largest in lane 0: a bitonic network.
+template <class K>
+__device__ __forceinline__ K merge_step(K v, int o, bool keep_larger) {
+  const K w = __shfl_xor_sync(kFull, v, o);
+  return (v > w) == keep_larger ? v : w;
+}
+template <class K>
+__device__ __forceinline__ K warp_sort(K v, int lane) {
+#pragma unroll
+  for (int k = 2; k <= 32; k *= 2)
+#pragma unroll
+    for (int o = k / 2; o; o /= 2) v = merge_step(v, o, ((lane & o) == 0) == ((lane & k) == 0));
+  return v;
+}
+// The 32 largest of two sorted lists; `reversed`: the other list's lane 31 - lane.
+template <class K>
+__device__ __forceinline__ K warp_merge(K v, K reversed, int lane) {
+  v = v > reversed ? v : reversed;  // a bitonic sequence
+#pragma unroll
+  for (int o = 16; o; o /= 2) v = merge_step(v, o, (lane & o) == 0);
+  return v;
+}
+// The same over sorted lists in shared memory, one a warp (n of them, a power
+// of two): the result is warp 0's.  The lists are in place and synchronised.
+template <class K>
+__device__ __forceinline__ K tree_merge(K (*lists)[32], int n, int warp, int lane) {
+  K v = warp < n ? lists[warp][lane] : 0;
+  for (n /= 2; n; n /= 2) {
+    if (warp < n) {
+      v = warp_merge(v, lists[warp + n][31 - lane], lane);
+      lists[warp][lane] = v;
+    }
+    __syncthreads();
+  }
+  return v;
+}
+
 struct Out {
   float *logprob, *entropy, *lse, *top_logprob;
   int* top_index;
@@ -148,7 +193,7 @@ __device__ __forceinline__ void finish(const Out& o, size_t row, const T* x, int
   const float lse = none ? -INFINITY : (st.m == -INFINITY ? st.s : st.m + log_s);
   if (lane == 0) {
     o.lse[row] = lse;
-    o.entropy[row] = none ? 0.f : log_s + st.a / st.s * kLn2;
+    o.entropy[row] = none ? 0.f : log_s - st.a / st.s * kLn2;
     const int t = tokens[row];
     float lp = 0.f;
     if (t != -1) {
@@ -168,13 +213,15 @@ __device__ __forceinline__ void finish(const Out& o, size_t row, const T* x, int
   }
 }
 
-// One warp per row, the whole row in registers (R elements a lane).
+// One warp per row, the whole row in registers (R elements a lane): small
+// vocabularies, where a row is less work than a CTA's joining.
 template <class T, int R>
 __global__ void __launch_bounds__(kThreads)
     forward_small(const T* __restrict__ logits, size_t stride, size_t rows, int vocab, const int* __restrict__ tokens,
                   int top, Out o) {
-  const int lane = threadIdx.x & 31;
-  const size_t row = (size_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  __shared__ u64 found[kWarps][64];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const size_t row = (size_t)blockIdx.x * kWarps + warp;
   if (row >= rows) return;
   const T* x = logits + row * stride;
   float v[R];
@@ -183,12 +230,51 @@ __global__ void __launch_bounds__(kThreads)
   float mx = v[0];
 #pragma unroll
   for (int r = 1; r < R; ++r) mx = fmaxf(mx, v[r]);
+  mx = warp_max(mx);
   Stats st = empty_stats();
   accumulate(st, v, mx);
-  st = warp_join(st);
+#pragma unroll
+  for (int i = 16; i; i >>= 1) {
+    st.s += __shfl_xor_sync(kFull, st.s, i);
+    st.a += __shfl_xor_sync(kFull, st.a, i);
+  }
   u64 mine = 0;
-  if (top) {
-    // k times: the largest key of all lanes, taken out of the lane it is in
+  if (top > kFewTop) {
+    u64 key[R], best = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      key[r] = lane + 32 * r < vocab ? top_key(v[r], lane + 32 * r) : 0;
+      best = key[r] > best ? key[r] : best;
+    }
+    if (R == 2) {
+      const u64 other = warp_sort(key[1], lane);
+      mine = warp_merge(warp_sort(key[0], lane), __shfl_sync(kFull, other, 31 - lane), lane);
+    } else {
+      // the k-th largest lane maximum (0 where fewer lanes hold elements) and what reaches it
+      const u64 least = __shfl_sync(kFull, warp_sort(best, lane), top - 1);
+      int count = 0;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const bool in = key[r] >= least && key[r] != 0;
+        const unsigned who = __ballot_sync(kFull, in);
+        const int at = count + __popc(who & ((1u << lane) - 1));
+        if (in && at < 64) found[warp][at] = key[r];
+        count += __popc(who);
+      }
+      __syncwarp();
+      if (count <= 64) {
+        mine = warp_sort(lane < count ? found[warp][lane] : 0ull, lane);
+        if (count > 32) {
+          const u64 other = warp_sort(lane + 32 < count ? found[warp][lane + 32] : 0ull, lane);
+          mine = warp_merge(mine, __shfl_sync(kFull, other, 31 - lane), lane);
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < R; ++r) offer(mine, key[r], 0, top, lane);
+      }
+    }
+  } else if (top) {
+    // few: the largest key of all lanes, taken out of the lane it is in, k times
     uint32_t best = 0, at = 0;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -238,79 +324,42 @@ __device__ __forceinline__ uint32_t remote_u32(const void* p, uint32_t rank) {
   return v;
 }
 
-// A thread's statistics and its warp's list, fed N elements a step.
-struct Running {
-  Stats st = empty_stats();
-  u64 mine = 0, floor = 0;  // keys at or below floor are out
-  bool first = true;
-  int lane, top;
-  u64* floor_key;  // the CTA's highest k-th best
-
-  // Element i of x is element at + (i / VEC) * apart + i % VEC of the row;
-  // those from `end` on are -inf and not of the row.
-  template <int VEC, int N>
-  __device__ __forceinline__ void step(const float (&x)[N], int at, int apart, int end) {
-    float mx = x[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) mx = fmaxf(mx, x[i]);
-    accumulate(st, x, mx);
-    if (!top) return;
-    const u64 shared = *(volatile u64*)floor_key;
-    if (shared > floor) floor = shared;
-    if (first) {
-      // k lanes hold an element at or above the k-th largest lane maximum,
-      // so nothing below that can be in the list
-      first = false;
-      u64 best = 0;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const u64 k = key<VEC>(x[i], i, at, apart, end);
-        if (k > best) best = k;
-      }
-      int above = 0;
-      for (int l = 0; l < 32; ++l) above += __shfl_sync(kFull, best, l) > best;
-      const unsigned kth = __ballot_sync(kFull, best != 0 && above == top - 1);
-      if (kth) {
-        const u64 k = __shfl_sync(kFull, best, __ffs(kth) - 1) - 1;
-        if (k > floor) floor = k;
-      }
-    }
-    const u64 last = __shfl_sync(kFull, mine, top - 1);
-    const uint32_t least = (uint32_t)((last > floor ? last : floor) >> 32);
-    // a maximum does not show NaN, the sum does
-    if (__any_sync(kFull, ordered(mx) >= least || st.s != st.s)) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) offer(mine, key<VEC>(x[i], i, at, apart, end), floor, top, lane);
-      if (lane == top - 1 && mine > floor) atomicMax(floor_key, mine);
-    }
-  }
-
-  template <int VEC>
-  static __device__ __forceinline__ u64 key(float x, int i, int at, int apart, int end) {
-    const int index = at + (i / VEC) * apart + i % VEC;
-    return index < end ? top_key(x, (uint32_t)index) : 0;
-  }
-};
-
-// One cluster per row, each CTA a contiguous share of it.  The ragged head
-// and tail around the 16-byte aligned body (odd vocabularies leave rows
-// unaligned) are one more step of single elements.
+// The largest of a 16-byte vector's elements.
 template <class T>
+__device__ __forceinline__ float vector_max(uint4 raw) {
+  if constexpr (sizeof(T) == 4) {
+    return fmaxf(fmaxf(__uint_as_float(raw.x), __uint_as_float(raw.y)),
+                 fmaxf(__uint_as_float(raw.z), __uint_as_float(raw.w)));
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const T2* h = reinterpret_cast<const T2*>(&raw);
+    const T2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(Element<T>::to(m.x), Element<T>::to(m.y));
+  }
+}
+
+// Rows of W warps each: 1 (kWarps rows a CTA), or kWarps with a cluster of
+// CTAs per row, each on a contiguous share of it.  The ragged head and tail
+// around the 16-byte aligned body (odd vocabularies leave rows unaligned) are
+// fewer than 2 VEC elements, one more for the group's first threads.
+template <class T, int W>
 __global__ void __launch_bounds__(kThreads)
-    forward_wide(const T* __restrict__ logits, size_t stride, int vocab, const int* __restrict__ tokens, int top,
-                 Out o) {
-  constexpr int VEC = Element<T>::kVec, N = kUnroll * VEC;
+    forward_wide(const T* __restrict__ logits, size_t stride, size_t rows, int vocab, const int* __restrict__ tokens,
+                 int top, Out o) {
+  constexpr int VEC = Element<T>::kVec, N = kUnroll * VEC, GROUP = 32 * W;
+  constexpr int kFound = W == 1 ? 64 : 32 * kWarps;
   __shared__ Stats warp_stats[kWarps];
-  __shared__ u64 lists[kWarps][kMaxTop];
-  __shared__ u64 floor_key;
-  __shared__ uint32_t cta_stats[3];
-  __shared__ uint32_t cta_list[2 * kMaxTop];
+  __shared__ u64 lists[kWarps][32];
+  __shared__ uint32_t maxima[kWarps][32];
+  __shared__ u64 found[W == 1 ? kWarps : 1][kFound];
+  __shared__ int counts[W == 1 ? kWarps : 1];
+  __shared__ uint32_t limit;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t rank = cluster_rank(), ranks = cluster_size();
-  const size_t row = blockIdx.x / ranks;
+  const int id = W == 1 ? lane : threadIdx.x, group = W == 1 ? warp : 0;
+  const uint32_t rank = W == 1 ? 0 : cluster_rank(), ranks = W == 1 ? 1 : cluster_size();
+  const size_t row = W == 1 ? (size_t)blockIdx.x * kWarps + warp : blockIdx.x / ranks;
+  if (W == 1 && row >= rows) return;
   const T* x = logits + row * stride;
-  if (threadIdx.x == 0) floor_key = 0;
-  __syncthreads();
 
   const int lead = (int)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(T));
   const int head = lead < vocab ? lead : vocab;
@@ -319,81 +368,135 @@ __global__ void __launch_bounds__(kThreads)
   const int share = (vectors + ranks - 1) / ranks;
   const int begin = min(vectors, (int)rank * share), end = min(vectors, begin + share);
   const uint4* body = reinterpret_cast<const uint4*>(x + head);
+  const int left = rank == 0 ? head + vocab - tail : 0;
+  const int left_at = id < head ? id : tail + id - head;
 
-  Running run;
-  run.lane = lane;
-  run.top = top;
-  run.floor_key = &floor_key;
-
-  // whole warps take part in every step (the list code votes)
-  for (int j = begin + warp * 32; j < end; j += kThreads * kUnroll) {
-    float v[N];
+  Stats st = empty_stats();
+  for (int j = begin + id; j < end; j += GROUP * kUnroll) {
     uint4 raw[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int at = j + lane + u * kThreads;
-      if (at < end) raw[u] = __ldg(body + at);
+    for (int u = 0; u < kUnroll; ++u)
+      if (j + u * GROUP < end) raw[u] = __ldg(body + j + u * GROUP);
+    if (j + (kUnroll - 1) * GROUP < end) {
+      float v[N], mx = vector_max<T>(raw[0]);
+#pragma unroll
+      for (int u = 1; u < kUnroll; ++u) mx = fmaxf(mx, vector_max<T>(raw[u]));
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) Element<T>::unpack(raw[u], v + u * VEC);
+      accumulate(st, v, mx);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (j + u * GROUP < end) {
+          float v[VEC];
+          Element<T>::unpack(raw[u], v);
+          accumulate(st, v, vector_max<T>(raw[u]));
+        }
     }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      if (j + lane + u * kThreads < end) {
-        Element<T>::unpack(raw[u], v + u * VEC);
-      } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[u * VEC + i] = -INFINITY;
-      }
-    }
-    run.step<VEC, N>(v, head + (j + lane) * VEC, kThreads * VEC, head + end * VEC);
   }
-  if (rank == 0 && warp == 0) {
-    // head + tail: fewer than 2 VEC elements, one a lane
-    const int left = head + vocab - tail;
-    const int at = lane < head ? lane : tail + lane - head;
-    float v[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = -INFINITY;
-    if (lane < left) v[0] = Element<T>::to(x[at]);
-    run.step<1, N>(v, at, 1, lane < left ? at + 1 : 0);
+  if (id < left) {
+    float v[2] = {Element<T>::to(x[left_at]), -INFINITY};
+    accumulate(st, v, v[0]);
   }
+  // this thread's largest element in the list's order; NaN, which a maximum
+  // does not show, above all
+  const uint32_t reach = st.s == st.s ? ordered(st.m) : 0xFFFFFFFFu;
 
-  Stats st = warp_join(run.st);
-  u64 mine = run.mine;
-  if (lane == 0) warp_stats[warp] = st;
-  if (lane < top) lists[warp][lane] = mine;
-  __syncthreads();
-  if (warp == 0) {
-    st = warp_stats[0];
-    for (int w = 1; w < kWarps; ++w) st = join(st, warp_stats[w]);
-    if (top)
-      for (int w = 1; w < kWarps; ++w) offer(mine, lane < top ? lists[w][lane] : 0, 0, top, lane);
-    if (ranks > 1) {
-      if (lane == 0) {
-        cta_stats[0] = __float_as_uint(st.m);
-        cta_stats[1] = __float_as_uint(st.s);
-        cta_stats[2] = __float_as_uint(st.a);
+  st = warp_join(st);
+  u64 mine = 0;
+  if (top) {
+    uint32_t sorted = warp_sort(reach, lane);
+    if (id == 0) counts[group] = 0;
+    if (W > 1) {
+      maxima[warp][lane] = sorted;
+      __syncthreads();
+      sorted = tree_merge(maxima, kWarps, warp, lane);
+      // NaN anywhere: no limit
+      const bool nan = __shfl_sync(kFull, sorted, 0) == 0xFFFFFFFFu;
+      if (warp == 0 && lane == top - 1) limit = nan ? 0 : sorted;
+      __syncthreads();
+    } else {
+      __syncwarp();
+    }
+    const uint32_t least = W > 1 ? limit : __shfl_sync(kFull, sorted, 0) == 0xFFFFFFFFu ? 0 : __shfl_sync(kFull, sorted, top - 1);
+    const bool plain = least > ordered(-INFINITY);
+    if (plain && reach >= least) {
+      auto take = [&](float v, int index) {
+        if (ordered(v) >= least) {
+          const int at = atomicAdd(&counts[group], 1);
+          if (at < kFound) found[group][at] = top_key(v, (uint32_t)index);
+        }
+      };
+      for (int j = begin + id; j < end; j += GROUP) {
+        const uint4 raw = __ldg(body + j);
+        if (ordered(vector_max<T>(raw)) < least) continue;
+        float v[VEC];
+        Element<T>::unpack(raw, v);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) take(v[i], head + j * VEC + i);
       }
-      cta_list[2 * lane] = (uint32_t)mine;
-      cta_list[2 * lane + 1] = (uint32_t)(mine >> 32);
+      if (id < left) take(Element<T>::to(x[left_at]), left_at);
+    }
+    if (W > 1) __syncthreads();
+    else __syncwarp();
+    const int count = counts[group];
+    if (plain && count >= top && count <= kFound) {
+      const u64* mine_at = found[group] + (W > 1 ? 32 * warp : 0);
+      const int here = W > 1 ? count - 32 * warp : count;
+      if (here > 0) mine = warp_sort(lane < here ? mine_at[lane] : 0ull, lane);
+      if (W == 1 && here > 32) {
+        const u64 other = warp_sort(lane + 32 < here ? mine_at[lane + 32] : 0ull, lane);
+        mine = warp_merge(mine, __shfl_sync(kFull, other, 31 - lane), lane);
+      }
+    } else {
+      // any row: a sorted list a warp, every element offered to it
+      for (int j = begin + (id & ~31); j < end; j += GROUP) {
+        const bool there = j + lane < end;
+        float v[VEC];
+        Element<T>::unpack(there ? __ldg(body + j + lane) : make_uint4(0u, 0u, 0u, 0u), v);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          offer(mine, there ? top_key(v[i], (uint32_t)(head + (j + lane) * VEC + i)) : 0ull, 0, top, lane);
+      }
+      if (id < 32)
+        offer(mine, id < left ? top_key(Element<T>::to(x[left_at]), (uint32_t)left_at) : 0ull, 0, top, lane);
     }
   }
-  if (ranks > 1) {
-    cluster_sync();
-    if (rank == 0 && warp == 0) {
-      for (uint32_t r = 1; r < ranks; ++r) {
-        Stats q;
-        q.m = __uint_as_float(remote_u32(&cta_stats[0], r));
-        q.s = __uint_as_float(remote_u32(&cta_stats[1], r));
-        q.a = __uint_as_float(remote_u32(&cta_stats[2], r));
-        st = join(st, q);
+  if (W > 1) {
+    if (lane == 0) warp_stats[warp] = st;
+    if (top) lists[warp][lane] = mine;
+    __syncthreads();
+    st = warp_stats[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) st = join(st, warp_stats[w]);
+    if (top) mine = tree_merge(lists, kWarps, warp, lane);
+    if (ranks > 1) {
+      // the cluster's first CTA reads the others' results, a warp each
+      __syncthreads();
+      if (threadIdx.x == 0) warp_stats[0] = st;
+      cluster_sync();
+      Stats q = empty_stats();
+      u64 theirs = 0;
+      if (rank == 0 && warp < (int)ranks) {
+        q.m = __uint_as_float(remote_u32(&warp_stats[0].m, warp));
+        q.s = __uint_as_float(remote_u32(&warp_stats[0].s, warp));
+        q.a = __uint_as_float(remote_u32(&warp_stats[0].a, warp));
         if (top) {
-          const u64 lo = remote_u32(&cta_list[2 * lane], r), hi = remote_u32(&cta_list[2 * lane + 1], r);
-          offer(mine, lane < top ? (hi << 32) | lo : 0, 0, top, lane);
+          const uint32_t* at = reinterpret_cast<const uint32_t*>(&lists[0][lane]);
+          theirs = (u64)remote_u32(at + 1, warp) << 32 | remote_u32(at, warp);
         }
       }
+      cluster_sync();  // read before any of it is written again
+      if (rank != 0) return;
+      if (lane == 0) warp_stats[warp] = q;
+      lists[warp][lane] = theirs;
+      __syncthreads();
+      st = warp_stats[0];
+      for (uint32_t r = 1; r < ranks; ++r) st = join(st, warp_stats[r]);
+      if (top) mine = tree_merge(lists, (int)ranks, warp, lane);
     }
-    cluster_sync();  // the lists stay in place until they have been read
   }
-  if (rank == 0 && warp == 0) finish(o, row, x, vocab, tokens, top, st, mine, lane);
+  if (W == 1 || warp == 0) finish(o, row, x, vocab, tokens, top, st, mine, lane);
 }
 
 // ---------------------------------------------------------------- gradient
@@ -509,9 +612,11 @@ void launch_forward(const T* x, size_t stride, size_t rows, uint32_t vocab, cons
                     const Out& o, cudaStream_t st) {
   if (vocab <= 64) return launch_small<T, 2>(x, stride, rows, vocab, tokens, top, o, st);
   if (vocab <= 128) return launch_small<T, 4>(x, stride, rows, vocab, tokens, top, o, st);
-  if (vocab <= 256) return launch_small<T, 8>(x, stride, rows, vocab, tokens, top, o, st);
-  if (vocab <= 512) return launch_small<T, 16>(x, stride, rows, vocab, tokens, top, o, st);
-  if (vocab <= (uint32_t)kRowLanes) return launch_small<T, 32>(x, stride, rows, vocab, tokens, top, o, st);
+  if (vocab <= (uint32_t)kRowLanes) {
+    forward_wide<T, 1><<<(unsigned)((rows + kWarps - 1) / kWarps), kThreads, 0, st>>>(x, stride, rows, (int)vocab,
+                                                                                     tokens, (int)top, o);
+    return;
+  }
   const unsigned shares = row_shares(rows, (int)vocab);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * shares));
@@ -524,7 +629,7 @@ void launch_forward(const T* x, size_t stride, size_t rows, uint32_t vocab, cons
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, forward_wide<T>, x, stride, (int)vocab, tokens, (int)top, o);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, forward_wide<T, kWarps>, x, stride, rows, (int)vocab, tokens, (int)top, o);
   require(e == cudaSuccess, std::string("token log-probabilities: ") + cudaGetErrorString(e), MB_ERR_CUDA);
 }
 
