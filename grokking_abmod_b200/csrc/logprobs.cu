@@ -34,6 +34,7 @@ constexpr int kMaxTop = 32;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kUnroll = 4;      // 16-byte vectors a thread has in flight
+constexpr int kAgain = 4;       // the same where it looks for top tokens
 constexpr int kRowLanes = 1024; // vocabularies up to here take one warp per row
 constexpr int kFewTop = 6;      // so many top tokens of a row in registers are picked one by one, more are sorted
 constexpr unsigned kFull = 0xFFFFFFFFu;
@@ -162,6 +163,15 @@ __device__ __forceinline__ K warp_merge(K v, K reversed, int lane) {
   for (int o = 16; o; o /= 2) v = merge_step(v, o, (lane & o) == 0);
   return v;
 }
+// The 32 largest of n keys in shared memory, sorted.
+__device__ __forceinline__ u64 sort_found(const u64* at, int n, int lane) {
+  u64 v = warp_sort(lane < n ? at[lane] : 0ull, lane);
+  for (int b = 32; b < n; b += 32) {
+    const u64 other = warp_sort(b + lane < n ? at[b + lane] : 0ull, lane);
+    v = warp_merge(v, __shfl_sync(kFull, other, 31 - lane), lane);
+  }
+  return v;
+}
 // The same over sorted lists in shared memory, one a warp (n of them, a power
 // of two): the result is warp 0's.  The lists are in place and synchronised.
 template <class K>
@@ -219,7 +229,7 @@ template <class T, int R>
 __global__ void __launch_bounds__(kThreads)
     forward_small(const T* __restrict__ logits, size_t stride, size_t rows, int vocab, const int* __restrict__ tokens,
                   int top, Out o) {
-  __shared__ u64 found[kWarps][64];
+  __shared__ u64 found[kWarps][32 * R];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const size_t row = (size_t)blockIdx.x * kWarps + warp;
   if (row >= rows) return;
@@ -258,20 +268,11 @@ __global__ void __launch_bounds__(kThreads)
         const bool in = key[r] >= least && key[r] != 0;
         const unsigned who = __ballot_sync(kFull, in);
         const int at = count + __popc(who & ((1u << lane) - 1));
-        if (in && at < 64) found[warp][at] = key[r];
+        if (in) found[warp][at] = key[r];
         count += __popc(who);
       }
       __syncwarp();
-      if (count <= 64) {
-        mine = warp_sort(lane < count ? found[warp][lane] : 0ull, lane);
-        if (count > 32) {
-          const u64 other = warp_sort(lane + 32 < count ? found[warp][lane + 32] : 0ull, lane);
-          mine = warp_merge(mine, __shfl_sync(kFull, other, 31 - lane), lane);
-        }
-      } else {
-#pragma unroll
-        for (int r = 0; r < R; ++r) offer(mine, key[r], 0, top, lane);
-      }
+      mine = sort_found(found[warp], count, lane);
     }
   } else if (top) {
     // few: the largest key of all lanes, taken out of the lane it is in, k times
@@ -342,12 +343,12 @@ __device__ __forceinline__ float vector_max(uint4 raw) {
 // CTAs per row, each on a contiguous share of it.  The ragged head and tail
 // around the 16-byte aligned body (odd vocabularies leave rows unaligned) are
 // fewer than 2 VEC elements, one more for the group's first threads.
-template <class T, int W>
+template <class T, int W, bool TOP>
 __global__ void __launch_bounds__(kThreads)
     forward_wide(const T* __restrict__ logits, size_t stride, size_t rows, int vocab, const int* __restrict__ tokens,
                  int top, Out o) {
   constexpr int VEC = Element<T>::kVec, N = kUnroll * VEC, GROUP = 32 * W;
-  constexpr int kFound = W == 1 ? 64 : 32 * kWarps;
+  constexpr int kFound = 256;  // candidates of a group
   __shared__ Stats warp_stats[kWarps];
   __shared__ u64 lists[kWarps][32];
   __shared__ uint32_t maxima[kWarps][32];
@@ -404,13 +405,19 @@ __global__ void __launch_bounds__(kThreads)
 
   st = warp_join(st);
   u64 mine = 0;
-  if (top) {
-    uint32_t sorted = warp_sort(reach, lane);
+  if constexpr (TOP) {
+    // of one top token only the largest is needed
+    uint32_t sorted = top > 1 ? warp_sort(reach, lane) : __reduce_max_sync(kFull, reach);
     if (id == 0) counts[group] = 0;
     if (W > 1) {
       maxima[warp][lane] = sorted;
       __syncthreads();
-      sorted = tree_merge(maxima, kWarps, warp, lane);
+      if (top > 1) {
+        sorted = tree_merge(maxima, kWarps, warp, lane);
+      } else {
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) sorted = max(sorted, maxima[w][0]);
+      }
       // NaN anywhere: no limit
       const bool nan = __shfl_sync(kFull, sorted, 0) == 0xFFFFFFFFu;
       if (warp == 0 && lane == top - 1) limit = nan ? 0 : sorted;
@@ -427,13 +434,23 @@ __global__ void __launch_bounds__(kThreads)
           if (at < kFound) found[group][at] = top_key(v, (uint32_t)index);
         }
       };
-      for (int j = begin + id; j < end; j += GROUP) {
-        const uint4 raw = __ldg(body + j);
-        if (ordered(vector_max<T>(raw)) < least) continue;
-        float v[VEC];
-        Element<T>::unpack(raw, v);
+      for (int j = begin + id; j < end; j += GROUP * kAgain) {
+        uint4 raw[kAgain];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) take(v[i], head + j * VEC + i);
+        for (int u = 0; u < kAgain; ++u)
+          if (j + u * GROUP < end) raw[u] = __ldg(body + j + u * GROUP);
+        unsigned hits = 0;
+#pragma unroll
+        for (int u = 0; u < kAgain; ++u)
+          if (j + u * GROUP < end && ordered(vector_max<T>(raw[u])) >= least) hits |= 1u << u;
+        while (hits) {
+          const int at = j + (__ffs(hits) - 1) * GROUP;
+          hits &= hits - 1;
+          float v[VEC];
+          Element<T>::unpack(__ldg(body + at), v);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) take(v[i], head + at * VEC + i);
+        }
       }
       if (id < left) take(Element<T>::to(x[left_at]), left_at);
     }
@@ -441,13 +458,8 @@ __global__ void __launch_bounds__(kThreads)
     else __syncwarp();
     const int count = counts[group];
     if (plain && count >= top && count <= kFound) {
-      const u64* mine_at = found[group] + (W > 1 ? 32 * warp : 0);
-      const int here = W > 1 ? count - 32 * warp : count;
-      if (here > 0) mine = warp_sort(lane < here ? mine_at[lane] : 0ull, lane);
-      if (W == 1 && here > 32) {
-        const u64 other = warp_sort(lane + 32 < here ? mine_at[lane + 32] : 0ull, lane);
-        mine = warp_merge(mine, __shfl_sync(kFull, other, 31 - lane), lane);
-      }
+      if (W == 1) mine = sort_found(found[group], count, lane);
+      else if (32 * warp < count) mine = sort_found(found[group] + 32 * warp, min(32, count - 32 * warp), lane);
     } else {
       // any row: a sorted list a warp, every element offered to it
       for (int j = begin + (id & ~31); j < end; j += GROUP) {
@@ -464,12 +476,12 @@ __global__ void __launch_bounds__(kThreads)
   }
   if (W > 1) {
     if (lane == 0) warp_stats[warp] = st;
-    if (top) lists[warp][lane] = mine;
+    if (TOP) lists[warp][lane] = mine;
     __syncthreads();
     st = warp_stats[0];
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) st = join(st, warp_stats[w]);
-    if (top) mine = tree_merge(lists, kWarps, warp, lane);
+    if (TOP) mine = tree_merge(lists, kWarps, warp, lane);
     if (ranks > 1) {
       // the cluster's first CTA reads the others' results, a warp each
       __syncthreads();
@@ -481,7 +493,7 @@ __global__ void __launch_bounds__(kThreads)
         q.m = __uint_as_float(remote_u32(&warp_stats[0].m, warp));
         q.s = __uint_as_float(remote_u32(&warp_stats[0].s, warp));
         q.a = __uint_as_float(remote_u32(&warp_stats[0].a, warp));
-        if (top) {
+        if (TOP) {
           const uint32_t* at = reinterpret_cast<const uint32_t*>(&lists[0][lane]);
           theirs = (u64)remote_u32(at + 1, warp) << 32 | remote_u32(at, warp);
         }
@@ -493,10 +505,10 @@ __global__ void __launch_bounds__(kThreads)
       __syncthreads();
       st = warp_stats[0];
       for (uint32_t r = 1; r < ranks; ++r) st = join(st, warp_stats[r]);
-      if (top) mine = tree_merge(lists, (int)ranks, warp, lane);
+      if (TOP) mine = tree_merge(lists, (int)ranks, warp, lane);
     }
   }
-  if (W == 1 || warp == 0) finish(o, row, x, vocab, tokens, top, st, mine, lane);
+  if (W == 1 || warp == 0) finish(o, row, x, vocab, tokens, TOP ? top : 0, st, mine, lane);
 }
 
 // ---------------------------------------------------------------- gradient
@@ -607,14 +619,12 @@ void launch_small(const T* x, size_t stride, size_t rows, uint32_t vocab, const 
                                                                                     tokens, (int)top, o);
 }
 
-template <class T>
-void launch_forward(const T* x, size_t stride, size_t rows, uint32_t vocab, const int* tokens, uint32_t top,
-                    const Out& o, cudaStream_t st) {
-  if (vocab <= 64) return launch_small<T, 2>(x, stride, rows, vocab, tokens, top, o, st);
-  if (vocab <= 128) return launch_small<T, 4>(x, stride, rows, vocab, tokens, top, o, st);
+template <class T, bool TOP>
+void launch_wide(const T* x, size_t stride, size_t rows, uint32_t vocab, const int* tokens, uint32_t top, const Out& o,
+                 cudaStream_t st) {
   if (vocab <= (uint32_t)kRowLanes) {
-    forward_wide<T, 1><<<(unsigned)((rows + kWarps - 1) / kWarps), kThreads, 0, st>>>(x, stride, rows, (int)vocab,
-                                                                                     tokens, (int)top, o);
+    forward_wide<T, 1, TOP><<<(unsigned)((rows + kWarps - 1) / kWarps), kThreads, 0, st>>>(
+        x, stride, rows, (int)vocab, tokens, (int)top, o);
     return;
   }
   const unsigned shares = row_shares(rows, (int)vocab);
@@ -629,8 +639,18 @@ void launch_forward(const T* x, size_t stride, size_t rows, uint32_t vocab, cons
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, forward_wide<T, kWarps>, x, stride, rows, (int)vocab, tokens, (int)top, o);
+  const cudaError_t e =
+      cudaLaunchKernelEx(&cfg, forward_wide<T, kWarps, TOP>, x, stride, rows, (int)vocab, tokens, (int)top, o);
   require(e == cudaSuccess, std::string("token log-probabilities: ") + cudaGetErrorString(e), MB_ERR_CUDA);
+}
+
+template <class T>
+void launch_forward(const T* x, size_t stride, size_t rows, uint32_t vocab, const int* tokens, uint32_t top,
+                    const Out& o, cudaStream_t st) {
+  if (vocab <= 64) return launch_small<T, 2>(x, stride, rows, vocab, tokens, top, o, st);
+  if (vocab <= 128) return launch_small<T, 4>(x, stride, rows, vocab, tokens, top, o, st);
+  if (top) launch_wide<T, true>(x, stride, rows, vocab, tokens, top, o, st);
+  else launch_wide<T, false>(x, stride, rows, vocab, tokens, 0, o, st);
 }
 
 }  // namespace logprobs
