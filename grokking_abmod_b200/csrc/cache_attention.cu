@@ -39,7 +39,6 @@ constexpr int kTile = 32;        // tokens a warp takes at a time
 constexpr int kSplitWarps = 4;
 constexpr int kSplitThreads = kSplitWarps * 32;
 constexpr int kSplitRows = 8;    // query rows of a unit
-constexpr int kSplitStages = 3;  // tiles a warp has in flight
 
 struct Queries {
   const void* q;
@@ -64,11 +63,16 @@ struct Partials {
 
 template <int D>
 struct SplitSmem {
+  // Tiles a warp has in its ring, and CTAs of an SM that registers and shared
+  // memory then allow: the warps that wait on latencies count more than a
+  // deeper ring (128 wide, 131071 tokens: 292 us with 3 stages and 2 CTAs).
+  static constexpr int kStages = D > 64 ? 2 : 3;
+  static constexpr int kResident = D > 64 ? 3 : D > 32 ? 4 : 5;
   static constexpr int kTileBytes = kTile * D;
-  static constexpr int kWarpBytes = kSplitStages * 2 * kTileBytes;
+  static constexpr int kWarpBytes = kStages * 2 * kTileBytes;
   static constexpr int kBars = kSplitWarps * kWarpBytes;
-  static constexpr int kMeta = kBars + kSplitWarps * kSplitStages * 8;          // scales of each stage
-  static constexpr int kJoin = kMeta + kSplitWarps * kSplitStages * 16;         // m, l, exponent per warp and row
+  static constexpr int kMeta = kBars + kSplitWarps * kStages * 8;          // scales of each stage
+  static constexpr int kJoin = kMeta + kSplitWarps * kStages * 16;         // m, l, exponent per warp and row
   static constexpr int kBytes = kJoin + kSplitWarps * kSplitRows * 12 + 16;
 };
 
@@ -167,9 +171,10 @@ __device__ __forceinline__ void refuse_rows(const Batch& t, const Queries& q, in
 }
 
 template <class T, int D>
-__global__ void __launch_bounds__(kSplitThreads)
+__global__ void __launch_bounds__(kSplitThreads, SplitSmem<D>::kResident)
     attend_split(View c, Batch t, Queries q, Partials part, int blocks_per_seq) {
   using S = SplitSmem<D>;
+  constexpr int STAGES = S::kStages;
   constexpr int KW = D / 16;  // words of a K row that a thread reads: one K step of 16 channels each
   constexpr int VW = D / 32;  // words of a V row
   extern __shared__ __align__(128) uint8_t smem[];
@@ -200,12 +205,12 @@ __global__ void __launch_bounds__(kSplitThreads)
   }
 
   int8_t* ring = reinterpret_cast<int8_t*>(smem) + warp * S::kWarpBytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars) + warp * kSplitStages;
-  float4* meta = reinterpret_cast<float4*>(smem + S::kMeta) + warp * kSplitStages;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars) + warp * STAGES;
+  float4* meta = reinterpret_cast<float4*>(smem + S::kMeta) + warp * STAGES;
   float* join = reinterpret_cast<float*>(smem + S::kJoin);
   int* gave_up = reinterpret_cast<int*>(smem + S::kJoin + kSplitWarps * kSplitRows * 12);
   if (lane == 0)
-    for (int s = 0; s < kSplitStages; ++s) tc::bar_init(&bars[s], 1);
+    for (int s = 0; s < STAGES; ++s) tc::bar_init(&bars[s], 1);
   tc::bar_init_fence();
   if (threadIdx.x == 0) *gave_up = 0;
   __syncthreads();
@@ -241,7 +246,7 @@ __global__ void __launch_bounds__(kSplitThreads)
     if (bad && q.status) atomicOr(q.status, kBadPage);
   };
   auto issue = [&](int n) {
-    const int s = n % kSplitStages, from = n & 31;
+    const int s = n % STAGES, from = n & 31;
     const int p0 = __shfl_sync(kFull, page0, from), p1 = __shfl_sync(kFull, page1, from);
     const float4 m = make_float4(__shfl_sync(kFull, ks0, from), __shfl_sync(kFull, ks1, from),
                                  __shfl_sync(kFull, vs0, from), __shfl_sync(kFull, vs1, from));
@@ -265,7 +270,7 @@ __global__ void __launch_bounds__(kSplitThreads)
 
   look_up(0);
   int issued = 0;
-  for (; issued < kSplitStages - 1 && issued < mine; ++issued) issue(issued);
+  for (; issued < STAGES - 1 && issued < mine; ++issued) issue(issued);
 
   // This lane's query row (g): hi parts as operand row g, lo parts as g + 8.
   uint32_t qh[KW][2], ql[KW][2];
@@ -309,11 +314,11 @@ __global__ void __launch_bounds__(kSplitThreads)
       if ((issued & 31) == 0) look_up(issued);
       issue(issued++);
     }
-    const int s = n % kSplitStages;
-    if (!__all_sync(kFull, tc::bar_wait(&bars[s], (n / kSplitStages) & 1))) {
+    const int s = n % STAGES;
+    if (!__all_sync(kFull, tc::bar_wait(&bars[s], (n / STAGES) & 1))) {
       *gave_up = 1;
       // the copies behind it may still land: none is left when the CTA ends
-      for (int k = n + 1; k < issued; ++k) tc::bar_wait(&bars[k % kSplitStages], (k / kSplitStages) & 1);
+      for (int k = n + 1; k < issued; ++k) tc::bar_wait(&bars[k % STAGES], (k / STAGES) & 1);
       break;
     }
     const float4 sc = meta[s];
@@ -992,41 +997,66 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   if (threadIdx.x == 0 && *failed && q.status) atomicOr(q.status, kGaveUp);
 }
 
-// Joins the chunks of a unit's rows: one warp a row.
-template <class T, int D, int ROWS>
+// Joins the chunks of a unit's rows.  WARPS warps share a row's chunks: 8 for
+// the few rows of the split kernel, whose chunks may be hundreds, 1 for tiles.
+template <class T, int D, int ROWS, int WARPS>
 __global__ void __launch_bounds__(256)
     join_chunks(View c, Batch t, Queries q, Partials part, int blocks_per_seq) {
+  constexpr int C = D / 32;
+  __shared__ float sums[8], values[8][D];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int head = blockIdx.y, z = blockIdx.x;
-  const int r = blockIdx.z * 8 + (threadIdx.x >> 5);
+  const int r = WARPS == 1 ? blockIdx.z * 8 + warp : blockIdx.z;
   const Unit u = unit_of<ROWS>(c, t, q, z, blocks_per_seq);
   if (u.bad || r >= u.rows) return;
   const size_t slot = ((size_t)z * c.heads + head) * part.chunks;
+  const float* lse = part.lse + slot * ROWS + r;
   float top = -INFINITY;
-  for (int i = lane; i < part.chunks; i += 32) top = fmaxf(top, part.lse[(slot + i) * ROWS + r]);
+  for (int i = lane; i < part.chunks; i += 32) top = fmaxf(top, lse[(size_t)i * ROWS]);
 #pragma unroll
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
   const float base = top == -INFINITY ? 0.f : top;
-  float sum = 0.f, value[D / 32];
+  float sum = 0.f, value[C];
 #pragma unroll
-  for (int k = 0; k < D / 32; ++k) value[k] = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < part.chunks; ++i) {
-    const float x = part.lse[(slot + i) * ROWS + r];
-    if (x == -INFINITY) continue;  // saw nothing: its outputs were not written
-    const float f = ex2_ftz(x - base);
-    sum += f;
-    const float* po = part.o + ((slot + i) * ROWS + r) * D;
+  for (int k = 0; k < C; ++k) value[k] = 0.f;
+  constexpr int AHEAD = 4;
+  for (int i = WARPS == 1 ? 0 : warp; i < part.chunks; i += WARPS * AHEAD) {
+    float f[AHEAD], x[AHEAD][C];
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) value[k] = fmaf(f, po[lane + 32 * k], value[k]);
+    for (int e = 0; e < AHEAD; ++e) {
+      const int at = i + e * WARPS;
+      const float s = at < part.chunks ? lse[(size_t)at * ROWS] : -INFINITY;
+      f[e] = s == -INFINITY ? 0.f : ex2_ftz(s - base);  // saw nothing: its outputs were not written
+      const float* po = part.o + ((slot + at) * ROWS + r) * D;
+#pragma unroll
+      for (int k = 0; k < C; ++k) x[e][k] = s == -INFINITY ? 0.f : po[lane + 32 * k];
+    }
+#pragma unroll
+    for (int e = 0; e < AHEAD; ++e) {
+      sum += f[e];
+#pragma unroll
+      for (int k = 0; k < C; ++k) value[k] = fmaf(f[e], x[e][k], value[k]);
+    }
+  }
+  if (WARPS > 1) {
+    if (lane == 0) sums[warp] = sum;
+#pragma unroll
+    for (int k = 0; k < C; ++k) values[warp][lane + 32 * k] = value[k];
+    __syncthreads();
+    if (warp > 0) return;
+    for (int w = 1; w < WARPS; ++w) {
+      sum += sums[w];
+#pragma unroll
+      for (int k = 0; k < C; ++k) value[k] += values[w][lane + 32 * k];
+    }
   }
   const int row = u.row0 + r;
   const size_t at = u.first_row + row / q.group;
   const int a = head * q.group + row % q.group;
   T* out = static_cast<T*>(q.out) + (at * q.heads + a) * q.head_dim;
 #pragma unroll
-  for (int k = 0; k < D / 32; ++k)
+  for (int k = 0; k < C; ++k)
     if (lane + 32 * k < q.head_dim) out[lane + 32 * k] = Element<T>::from(sum == 0.f ? 0.f : value[k] / sum);
   if (lane == 0 && q.lse) q.lse[(size_t)a * t.rows + at] = sum == 0.f ? -INFINITY : base + log2f(sum);
 }
@@ -1052,11 +1082,15 @@ inline Plan make_plan(size_t batch, size_t rows, uint32_t kv_heads, uint32_t gro
   const size_t unit_rows = p.tiles ? kTileRows : kSplitRows, keys = p.tiles ? kKeys : kTile;
   p.blocks_per_seq = (int)((most_rows + unit_rows - 1) / unit_rows);
   p.units = batch * p.blocks_per_seq;
-  // Chunks for one (tiles) or about three (split) CTAs on every SM, none
-  // shorter than eight tiles: two a warp of the split kernel.
-  const size_t want = (size_t)sm_count() * (p.tiles ? 1 : 3), have = std::max<size_t>(1, p.units * kv_heads);
+  // Chunks for the CTAs that the GPU holds at a time, none shorter than eight
+  // tiles (two a warp of the split kernel).  Long sequences are cut further, as
+  // long as a chunk keeps 128 tiles: unequal lengths and ends even out.
+  const int resident = p.tiles ? 1 : width > 64 ? 3 : width > 32 ? 4 : 5;
+  const size_t slots = (size_t)sm_count() * resident, have = std::max<size_t>(1, p.units * kv_heads);
   const size_t tiles = std::max<size_t>(1, ((size_t)max_tokens + keys - 1) / keys);
-  const size_t chunks = std::max<size_t>(1, std::min((tiles + 7) / 8, want / have));
+  size_t chunks = std::max<size_t>(1, std::min((tiles + 7) / 8, slots / have));
+  for (int waves = 2; waves <= 4; ++waves)
+    if (tiles * have >= slots * waves * 128) chunks = std::max(chunks, slots * waves / have);
   p.chunk_tiles = (int)((tiles + chunks - 1) / chunks + kSplitWarps - 1) / kSplitWarps * kSplitWarps;
   p.chunks = (int)((tiles + p.chunk_tiles - 1) / p.chunk_tiles);
   p.workspace = p.chunks > 1 ? p.units * kv_heads * p.chunks * unit_rows * (width + 1) * sizeof(float) : 0;
@@ -1081,7 +1115,7 @@ void launch_rows(const View& c, const Batch& t, const Queries& q, const Plan& p,
   launched("cache attention");
   if (p.chunks == 1) return;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)p.units, (unsigned)c.heads, ROWS / 8);
+  cfg.gridDim = dim3((unsigned)p.units, (unsigned)c.heads, TILES ? ROWS / 8 : ROWS);
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
@@ -1089,7 +1123,7 @@ void launch_rows(const View& c, const Batch& t, const Queries& q, const Plan& p,
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, join_chunks<T, D, ROWS>, c, t, q, part, p.blocks_per_seq);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, join_chunks<T, D, ROWS, TILES ? 1 : 8>, c, t, q, part, p.blocks_per_seq);
   require(e == cudaSuccess, std::string("cache attention join: ") + cudaGetErrorString(e), MB_ERR_CUDA);
 }
 
