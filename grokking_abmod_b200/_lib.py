@@ -138,7 +138,7 @@ SIGNATURES = {
     # argument structures of the serving operators, packed by ops.py
     "mb_op_cache_write": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
     "mb_op_cache_read": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
-    "mb_op_cache_attention_workspace": (ctypes.c_int, [ctypes.c_uint32, ctypes.c_size_t] + [ctypes.c_uint32] * 5 +
+    "mb_op_cache_attention_workspace": (ctypes.c_int, [ctypes.c_uint32, ctypes.c_size_t] + [ctypes.c_uint32] * 6 +
                                         [c_size_p]),
     "mb_op_cache_attention": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
     "mb_op_token_logprobs": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),

@@ -15,13 +15,16 @@
 // two: q by its row's largest magnitude, p times 2^14, which keeps the
 // smallest kept part 2^-39 of the row's largest probability.
 //
-// The split kernel serves rows that share a key head and are few: 8 at a
-// time, one tile of 32 tokens after the other, bound by the bytes of the
-// cache.  The 8 rows' hi parts are rows 0-7 and their lo parts rows 8-15 of
-// the 16-row operand, so the second term costs nothing.  Every warp runs its
-// own ring of bulk copies and its own running softmax (no barrier between
-// warps until the end); the four warps' results, and the chunks that a long
-// sequence is cut into, are joined by their maxima in a fixed order.
+// The split kernel serves rows that share a key head and are few, one tile of
+// 32 tokens after the other, bound by the bytes of the cache.  The tensor
+// core's operand has 16 rows: 8 query rows' hi parts are its rows 0-7 and
+// their lo parts its rows 8-15, so the second term costs nothing; of 16-bit
+// rows, which need no second term (bfloat16's 8 bits fit into FP16, and a
+// probability's rounding to 11 bits is below the output's own), up to 16 are
+// served at once.  Every warp runs its own ring of bulk copies and its own
+// running softmax (no barrier between warps until the end); the four warps'
+// results, and the chunks that a long sequence is cut into, are joined by
+// their maxima in a fixed order.
 
 #include <algorithm>
 #include <cmath>
@@ -38,7 +41,6 @@ constexpr unsigned kFull = 0xFFFFFFFFu;
 constexpr int kTile = 32;        // tokens a warp takes at a time
 constexpr int kSplitWarps = 4;
 constexpr int kSplitThreads = kSplitWarps * 32;
-constexpr int kSplitRows = 8;    // query rows of a unit
 
 struct Queries {
   const void* q;
@@ -61,7 +63,7 @@ struct Partials {
   int chunk_tiles;  // tiles of a chunk; the last one takes what is left
 };
 
-template <int D>
+template <int D, int ROWS>
 struct SplitSmem {
   // Tiles a warp has in its ring, and CTAs of an SM that registers and shared
   // memory then allow: the warps that wait on latencies count more than a
@@ -73,7 +75,7 @@ struct SplitSmem {
   static constexpr int kBars = kSplitWarps * kWarpBytes;
   static constexpr int kMeta = kBars + kSplitWarps * kStages * 8;          // scales of each stage
   static constexpr int kJoin = kMeta + kSplitWarps * kStages * 16;         // m, l, exponent per warp and row
-  static constexpr int kBytes = kJoin + kSplitWarps * kSplitRows * 12 + 16;
+  static constexpr int kBytes = kJoin + kSplitWarps * ROWS * 12 + 16;
 };
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -170,10 +172,13 @@ __device__ __forceinline__ void refuse_rows(const Batch& t, const Queries& q, in
   }
 }
 
-template <class T, int D>
-__global__ void __launch_bounds__(kSplitThreads, SplitSmem<D>::kResident)
+template <class T, int D, int ROWS>
+__global__ void __launch_bounds__(kSplitThreads, SplitSmem<D, ROWS>::kResident)
     attend_split(View c, Batch t, Queries q, Partials part, int blocks_per_seq) {
-  using S = SplitSmem<D>;
+  using S = SplitSmem<D, ROWS>;
+  // 8 rows in two terms, or 16 in one: a lane has rows g (and g + 8), NB of them
+  static_assert(ROWS == 8 || (ROWS == 16 && sizeof(T) == 2), "rows");
+  constexpr int NB = ROWS / 8;
   constexpr int STAGES = S::kStages;
   constexpr int KW = D / 16;  // words of a K row that a thread reads: one K step of 16 channels each
   constexpr int VW = D / 32;  // words of a V row
@@ -181,7 +186,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D>::kResident)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, tq = lane & 3;
   const int chunk = blockIdx.x % part.chunks, head = blockIdx.y, z = blockIdx.x / part.chunks;
-  const Unit u = unit_of<kSplitRows>(c, t, q, z, blocks_per_seq);
+  const Unit u = unit_of<ROWS>(c, t, q, z, blocks_per_seq);
   const bool last_block = z % blocks_per_seq == blocks_per_seq - 1;
 
   if (u.bad) {
@@ -189,8 +194,8 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D>::kResident)
       refuse_rows<T>(t, q, head, u, 0, kSplitThreads);
       if (q.status && threadIdx.x == 0) atomicOr(q.status, span_of(t, c, u.b).flags);
     }
-  } else if (last_block && chunk == 0 && (long long)u.fresh * q.group > u.row0 + kSplitRows) {
-    refuse_rows<T>(t, q, head, u, u.row0 + kSplitRows, kSplitThreads);
+  } else if (last_block && chunk == 0 && (long long)u.fresh * q.group > u.row0 + ROWS) {
+    refuse_rows<T>(t, q, head, u, u.row0 + ROWS, kSplitThreads);
     if (q.status && threadIdx.x == 0) atomicOr(q.status, kBadRows);
   }
   if (u.bad || u.rows <= 0) return;
@@ -200,7 +205,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D>::kResident)
   const int end = chunk == part.chunks - 1 ? tile_hi : min(tile_hi, begin + part.chunk_tiles);
   const size_t slot = ((size_t)z * c.heads + head) * part.chunks + chunk;
   if (begin >= end && part.chunks > 1) {
-    if (threadIdx.x < kSplitRows) part.lse[slot * kSplitRows + threadIdx.x] = -INFINITY;
+    if (threadIdx.x < ROWS) part.lse[slot * ROWS + threadIdx.x] = -INFINITY;
     return;
   }
 
@@ -208,7 +213,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D>::kResident)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars) + warp * STAGES;
   float4* meta = reinterpret_cast<float4*>(smem + S::kMeta) + warp * STAGES;
   float* join = reinterpret_cast<float*>(smem + S::kJoin);
-  int* gave_up = reinterpret_cast<int*>(smem + S::kJoin + kSplitWarps * kSplitRows * 12);
+  int* gave_up = reinterpret_cast<int*>(smem + S::kJoin + kSplitWarps * ROWS * 12);
   if (lane == 0)
     for (int s = 0; s < STAGES; ++s) tc::bar_init(&bars[s], 1);
   tc::bar_init_fence();
@@ -248,10 +253,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D>::kResident)
   auto issue = [&](int n) {
     const int s = n % STAGES, from = n & 31;
     const int p0 = __shfl_sync(kFull, page0, from), p1 = __shfl_sync(kFull, page1, from);
-    const float4 m = make_float4(__shfl_sync(kFull, ks0, from), __shfl_sync(kFull, ks1, from),
-                                 __shfl_sync(kFull, vs0, from), __shfl_sync(kFull, vs1, from));
     if (lane == 0) {
-      meta[s] = m;
       int8_t* k_at = ring + s * 2 * S::kTileBytes;
       int8_t* v_at = k_at + S::kTileBytes;
       const int inside = ((begin + warp + n * kSplitWarps) * kTile) & (c.tokens - 1);
@@ -266,21 +268,27 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D>::kResident)
         tc::bulk_g2s(v_at + bytes, c.v + c.row(p1, head, 0), bytes, &bars[s]);
       }
     }
+    // behind the copies: the scales' loads may still be on their way
+    const float4 m = make_float4(__shfl_sync(kFull, ks0, from), __shfl_sync(kFull, ks1, from),
+                                 __shfl_sync(kFull, vs0, from), __shfl_sync(kFull, vs1, from));
+    if (lane == 0) meta[s] = m;
   };
 
   look_up(0);
   int issued = 0;
   for (; issued < STAGES - 1 && issued < mine; ++issued) issue(issued);
 
-  // This lane's query row (g): hi parts as operand row g, lo parts as g + 8.
-  uint32_t qh[KW][2], ql[KW][2];
-  float row_factor;
-  int limit;  // last position the row sees
-  {
-    const int r = u.row0 + g;
-    const bool there = g < u.rows;
+  // This lane's query rows: hi parts as operand rows g; as rows g + 8 their
+  // lo parts, or row g + 8.
+  uint32_t qf[KW][4];
+  float row_factor[NB];
+  int limit[NB];  // last position the row sees
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int r = u.row0 + 8 * nb + g;
+    const bool there = 8 * nb + g < u.rows;
     const int tok = r / q.group, a = head * q.group + r % q.group;
-    limit = there ? u.length - u.fresh + tok : -1;
+    limit[nb] = there ? u.length - u.fresh + tok : -1;
     const T* src = static_cast<const T*>(q.q) + (u.first_row + tok) * q.row_stride + (size_t)a * q.head_stride;
     float x[KW][4];
     float most = 0.f;
@@ -296,8 +304,12 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D>::kResident)
 #pragma unroll
     for (int w = 0; w < KW; ++w)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) tc::split_f16x2(x[w][2 * e] * up, x[w][2 * e + 1] * up, qh[w][e], ql[w][e]);
-    row_factor = q.scale_log2 / up;
+      for (int e = 0; e < 2; ++e) {
+        uint32_t lo;
+        tc::split_f16x2(x[w][2 * e] * up, x[w][2 * e + 1] * up, qf[w][2 * e + nb], lo);
+        if (NB == 1) qf[w][2 * e + 1] = lo;
+      }
+    row_factor[nb] = q.scale_log2 / up;
   }
   const int sure = u.length - u.fresh + u.row0 / q.group;  // the last position that every row sees
 
@@ -306,7 +318,12 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D>::kResident)
   for (int i = 0; i < D / 8; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-  float m = -INFINITY, l = 0.f;
+  float m[NB], l[NB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    m[nb] = -INFINITY;
+    l[nb] = 0.f;
+  }
   int ev = -126;  // o carries 2^(14 - ev)
 
   for (int n = 0; n < mine; ++n) {
@@ -326,7 +343,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D>::kResident)
     const int8_t* vt = kt + S::kTileBytes;
     const int pos = (begin + warp + n * kSplitWarps) * kTile;
 
-    float x[4][2];
+    float x[4][2 * NB];  // [8 tokens][row, token 2 tq + e]
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       uint32_t w[KW];
@@ -335,51 +352,69 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D>::kResident)
 #pragma unroll
       for (int k = 0; k < KW; ++k) {
         const uint32_t biased = w[k] ^ 0x80808080u;
-        mma16816(acc, qh[k][0], ql[k][0], qh[k][1], ql[k][1], codes_to_f16(biased, 0x4140),
+        mma16816(acc, qf[k][0], qf[k][1], qf[k][2], qf[k][3], codes_to_f16(biased, 0x4140),
                  codes_to_f16(biased, 0x4342));
       }
-      const float f = (j < 2 ? sc.x : sc.y) * row_factor;
-      x[j][0] = (acc[0] + acc[2]) * f;
-      x[j][1] = (acc[1] + acc[3]) * f;
+      const float scale = j < 2 ? sc.x : sc.y;
+      if constexpr (NB == 1) {
+        x[j][0] = (acc[0] + acc[2]) * (scale * row_factor[0]);
+        x[j][1] = (acc[1] + acc[3]) * (scale * row_factor[0]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[j][e] = acc[e] * (scale * row_factor[e / 2]);
+      }
     }
     if (pos < u.lo || pos + kTile - 1 > sure) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int at = pos + 8 * j + 2 * tq + e;
-          if (at < u.lo || at > limit) x[j][e] = -INFINITY;
+        for (int e = 0; e < 2 * NB; ++e) {
+          const int at = pos + 8 * j + 2 * tq + (e & 1);
+          if (at < u.lo || at > limit[e / 2]) x[j][e] = -INFINITY;
         }
     }
-    float mx = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1])),
-                     fmaxf(fmaxf(x[2][0], x[2][1]), fmaxf(x[3][0], x[3][1])));
-    mx = fmaxf(m, quad_max(mx));
-    const float base = mx == -INFINITY ? 0.f : mx;
-    const float shrink = ex2_ftz(m - base);
-    m = mx;
     // V's exponent: o is kept relative to the largest V scale so far
     int top = ev;
     if (sc.z == sc.z) top = max(top, exponent_of(sc.z));
     if (sc.w == sc.w) top = max(top, exponent_of(sc.w));
-    float change = shrink;
-    if (top != ev) change *= power_of_two(max(ev - top, -126));
+    const float lower = top != ev ? power_of_two(max(ev - top, -126)) : 1.f;
     ev = top;
-    l *= shrink;
-    if (__any_sync(kFull, change != 1.0f)) {
+    float base[NB], change[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      float mx = fmaxf(x[0][2 * nb], x[0][2 * nb + 1]);
+#pragma unroll
+      for (int j = 1; j < 4; ++j) mx = fmaxf(mx, fmaxf(x[j][2 * nb], x[j][2 * nb + 1]));
+      mx = fmaxf(m[nb], quad_max(mx));
+      base[nb] = mx == -INFINITY ? 0.f : mx;
+      const float shrink = ex2_ftz(m[nb] - base[nb]);
+      m[nb] = mx;
+      l[nb] *= shrink;
+      change[nb] = shrink * lower;
+    }
+    if (__any_sync(kFull, change[0] != 1.0f || change[NB - 1] != 1.0f)) {
 #pragma unroll
       for (int i = 0; i < D / 8; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][e] *= change;
+        for (int e = 0; e < 4; ++e) o[i][e] *= change[NB == 1 ? 0 : e / 2];
     }
     const float unit = power_of_two(-ev);
     const float f0 = sc.z * unit * 16384.f, f1 = sc.w * unit * 16384.f;
-    uint32_t ph[4], pl[4];
+    uint32_t pf[4][2];  // [8 tokens][operand rows g, g + 8]
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float p0 = ex2_ftz(x[j][0] - base), p1 = ex2_ftz(x[j][1] - base);
-      l += p0 + p1;
       const float f = j < 2 ? f0 : f1;
-      tc::split_f16x2(p0 * f, p1 * f, ph[j], pl[j]);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const float p0 = ex2_ftz(x[j][2 * nb] - base[nb]), p1 = ex2_ftz(x[j][2 * nb + 1] - base[nb]);
+        l[nb] += p0 + p1;
+        if constexpr (NB == 1) {
+          tc::split_f16x2(p0 * f, p1 * f, pf[j][0], pf[j][1]);
+        } else {
+          const __half2 h = __floats2half2_rn(p0 * f, p1 * f);
+          pf[j][nb] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+      }
     }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -396,13 +431,13 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D>::kResident)
         // bytes of the two rows side by side: channels 0, 1 and 2, 3
         const uint32_t ab0 = __byte_perm(a, b, 0x5140), ab1 = __byte_perm(a, b, 0x7362);
         const uint32_t de0 = __byte_perm(d, e, 0x5140), de1 = __byte_perm(d, e, 0x7362);
-        mma16816(o[4 * w + 0], ph[2 * k], pl[2 * k], ph[2 * k + 1], pl[2 * k + 1], codes_to_f16(ab0, 0x4140),
+        mma16816(o[4 * w + 0], pf[2 * k][0], pf[2 * k][1], pf[2 * k + 1][0], pf[2 * k + 1][1], codes_to_f16(ab0, 0x4140),
                  codes_to_f16(de0, 0x4140));
-        mma16816(o[4 * w + 1], ph[2 * k], pl[2 * k], ph[2 * k + 1], pl[2 * k + 1], codes_to_f16(ab0, 0x4342),
+        mma16816(o[4 * w + 1], pf[2 * k][0], pf[2 * k][1], pf[2 * k + 1][0], pf[2 * k + 1][1], codes_to_f16(ab0, 0x4342),
                  codes_to_f16(de0, 0x4342));
-        mma16816(o[4 * w + 2], ph[2 * k], pl[2 * k], ph[2 * k + 1], pl[2 * k + 1], codes_to_f16(ab1, 0x4140),
+        mma16816(o[4 * w + 2], pf[2 * k][0], pf[2 * k][1], pf[2 * k + 1][0], pf[2 * k + 1][1], codes_to_f16(ab1, 0x4140),
                  codes_to_f16(de1, 0x4140));
-        mma16816(o[4 * w + 3], ph[2 * k], pl[2 * k], ph[2 * k + 1], pl[2 * k + 1], codes_to_f16(ab1, 0x4342),
+        mma16816(o[4 * w + 3], pf[2 * k][0], pf[2 * k][1], pf[2 * k + 1][0], pf[2 * k + 1][1], codes_to_f16(ab1, 0x4342),
                  codes_to_f16(de1, 0x4342));
       }
     }
@@ -410,20 +445,31 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D>::kResident)
   }
 
   // The four warps' results side by side; every copy issued has landed.
-  l = quad_sum(l);
-  if (tq == 0) {
-    float* w = join + (warp * kSplitRows + g) * 3;
-    w[0] = m;
-    w[1] = l;
-    w[2] = power_of_two(ev);
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const float sum = quad_sum(l[nb]);
+    if (tq == 0) {
+      float* w = join + (warp * ROWS + 8 * nb + g) * 3;
+      w[0] = m[nb];
+      w[1] = sum;
+      w[2] = power_of_two(ev);
+    }
   }
   __syncwarp();
-  float* mine_o = reinterpret_cast<float*>(ring);  // [8][D]
+  float* mine_o = reinterpret_cast<float*>(ring);  // [ROWS][D]
 #pragma unroll
   for (int i = 0; i < D / 8; ++i) {
     // n-tile i, column n is channel n D/8 + i
-    mine_o[g * D + (2 * tq) * (D / 8) + i] = o[i][0] + o[i][2];
-    mine_o[g * D + (2 * tq + 1) * (D / 8) + i] = o[i][1] + o[i][3];
+    float* at = mine_o + g * D + 2 * tq * (D / 8) + i;
+    if constexpr (NB == 1) {
+      at[0] = o[i][0] + o[i][2];
+      at[D / 8] = o[i][1] + o[i][3];
+    } else {
+      at[0] = o[i][0];
+      at[D / 8] = o[i][1];
+      at[8 * D] = o[i][2];
+      at[8 * D + D / 8] = o[i][3];
+    }
   }
   __syncthreads();
   const bool failed = *gave_up != 0;
@@ -432,12 +478,12 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D>::kResident)
     const int r = e / D, ch = e % D;
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kSplitWarps; ++w) top = fmaxf(top, join[(w * kSplitRows + r) * 3]);
+    for (int w = 0; w < kSplitWarps; ++w) top = fmaxf(top, join[(w * ROWS + r) * 3]);
     const float base = top == -INFINITY ? 0.f : top;
     float sum = 0.f, value = 0.f;
 #pragma unroll
     for (int w = 0; w < kSplitWarps; ++w) {
-      const float* jw = join + (w * kSplitRows + r) * 3;
+      const float* jw = join + (w * ROWS + r) * 3;
       const float f = ex2_ftz(jw[0] - base);
       const float ow = reinterpret_cast<const float*>(smem + w * S::kWarpBytes)[e];
       sum = fmaf(jw[1], f, sum);
@@ -447,8 +493,8 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D>::kResident)
     value = sum == 0.f ? 0.f : value / sum;
     if (failed) lse = value = NAN;
     if (part.chunks > 1) {
-      part.o[(slot * kSplitRows + r) * D + ch] = value;
-      if (ch == 0) part.lse[slot * kSplitRows + r] = lse;
+      part.o[(slot * ROWS + r) * D + ch] = value;
+      if (ch == 0) part.lse[slot * ROWS + r] = lse;
     } else {
       const int row = u.row0 + r;
       const size_t at = u.first_row + row / q.group;
@@ -1063,7 +1109,7 @@ __global__ void __launch_bounds__(256)
 
 // ---------------------------------------------------------------- host side
 struct Plan {
-  bool tiles;          // the tile kernel, else the split kernel
+  int unit_rows;       // kTileRows: the tile kernel, else the split kernel with 8 or 16
   int blocks_per_seq;  // row blocks of a sequence
   size_t units;        // sequences times row blocks
   int chunks, chunk_tiles;
@@ -1074,18 +1120,19 @@ struct Plan {
 constexpr size_t kSplitMost = 16;
 
 inline Plan make_plan(size_t batch, size_t rows, uint32_t kv_heads, uint32_t group, uint32_t width, uint32_t max_new,
-                      uint32_t max_tokens) {
+                      uint32_t max_tokens, uint32_t dtype) {
   Plan p;
   const size_t most_rows = (size_t)max_new * group;
   require(most_rows <= (1u << 30), "too many new rows for one call");
-  p.tiles = rows * group > kSplitMost * batch;
-  const size_t unit_rows = p.tiles ? kTileRows : kSplitRows, keys = p.tiles ? kKeys : kTile;
+  const bool use_tiles = rows * group > kSplitMost * batch;
+  p.unit_rows = use_tiles ? kTileRows : dtype != MB_F32 && most_rows > 8 ? 16 : 8;
+  const size_t unit_rows = p.unit_rows, keys = use_tiles ? kKeys : kTile;
   p.blocks_per_seq = (int)((most_rows + unit_rows - 1) / unit_rows);
   p.units = batch * p.blocks_per_seq;
   // Chunks for the CTAs that the GPU holds at a time, none shorter than eight
   // tiles (two a warp of the split kernel).  Long sequences are cut further, as
   // long as a chunk keeps 128 tiles: unequal lengths and ends even out.
-  const int resident = p.tiles ? 1 : width > 64 ? 3 : width > 32 ? 4 : 5;
+  const int resident = use_tiles ? 1 : width > 64 ? 3 : width > 32 ? 4 : 5;
   const size_t slots = (size_t)sm_count() * resident, have = std::max<size_t>(1, p.units * kv_heads);
   const size_t tiles = std::max<size_t>(1, ((size_t)max_tokens + keys - 1) / keys);
   size_t chunks = std::max<size_t>(1, std::min((tiles + 7) / 8, slots / have));
@@ -1104,10 +1151,10 @@ void launch_rows(const View& c, const Batch& t, const Queries& q, const Plan& p,
   // outputs first: their vectors need the workspace's alignment
   float* o = static_cast<float*>(workspace);
   const Partials part{o + slots * ROWS * D, o, p.chunks, p.chunk_tiles};
-  constexpr int bytes = TILES ? TileShape<D, sizeof(T) == 4 ? 2 : 1>::kBytes : SplitSmem<D>::kBytes;
+  constexpr int bytes = TILES ? TileShape<D, sizeof(T) == 4 ? 2 : 1>::kBytes : SplitSmem<D, TILES ? 8 : ROWS>::kBytes;
   void (*kernel)(View, Batch, Queries, Partials, int);
   if constexpr (TILES) kernel = attend_tiles<T, D>;
-  else kernel = attend_split<T, D>;
+  else kernel = attend_split<T, D, ROWS>;
   static DeviceOnce once;  // one a kernel
   once([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
   kernel<<<dim3((unsigned)(p.units * p.chunks), (unsigned)c.heads), TILES ? kTileThreads : kSplitThreads, bytes, st>>>(
@@ -1129,8 +1176,10 @@ void launch_rows(const View& c, const Batch& t, const Queries& q, const Plan& p,
 
 template <class T, int D>
 void launch(const View& c, const Batch& t, const Queries& q, const Plan& p, void* workspace, cudaStream_t st) {
-  if (p.tiles) launch_rows<T, D, kTileRows>(c, t, q, p, workspace, st);
-  else launch_rows<T, D, kSplitRows>(c, t, q, p, workspace, st);
+  if (p.unit_rows == kTileRows) return launch_rows<T, D, kTileRows>(c, t, q, p, workspace, st);
+  if constexpr (sizeof(T) == 2)
+    if (p.unit_rows == 16) return launch_rows<T, D, 16>(c, t, q, p, workspace, st);
+  launch_rows<T, D, 8>(c, t, q, p, workspace, st);
 }
 
 }  // namespace cache
@@ -1139,13 +1188,13 @@ void launch(const View& c, const Batch& t, const Queries& q, const Plan& p, void
 extern "C" {
 
 int mb_op_cache_attention_workspace(uint32_t batch, size_t rows, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,
-                                    uint32_t max_new, uint32_t max_tokens, size_t* bytes) {
+                                    uint32_t dtype, uint32_t max_new, uint32_t max_tokens, size_t* bytes) {
   using namespace mb::cache;
   return mb::guarded([&] {
     mb::need(bytes, "bytes");
     mb::require(kv_heads >= 1 && q_heads >= 1 && q_heads % kv_heads == 0, "kv_heads must divide q_heads");
-    *bytes = batch == 0 ? 0 : make_plan(batch, rows, kv_heads, q_heads / kv_heads, (head_dim + 31) / 32 * 32, max_new, max_tokens)
-                                 .workspace;
+    const uint32_t width = (head_dim + 31) / 32 * 32;
+    *bytes = batch == 0 ? 0 : make_plan(batch, rows, kv_heads, q_heads / kv_heads, width, max_new, max_tokens, dtype).workspace;
   });
 }
 
@@ -1169,7 +1218,7 @@ int mb_op_cache_attention(const mb_cache_attention_args* a, void* stream) {
     mb::need(out, "out");
     const Queries qs{q, a->q_row_stride, a->q_head_stride, out, a->lse, (int)q_heads, (int)(q_heads / c.heads),
                      (int)a->head_dim, a->scale * mb::kLog2e, a->first, (int)max_new, a->d_status};
-    const Plan p = make_plan(t.count, t.rows, c.heads, qs.group, c.width, max_new, max_tokens);
+    const Plan p = make_plan(t.count, t.rows, c.heads, qs.group, c.width, max_new, max_tokens, a->dtype);
     mb::require(p.units * p.chunks <= (size_t)INT_MAX, "too many row blocks for one call");
     mb::require(p.workspace == 0 || (workspace != nullptr && workspace_bytes >= p.workspace &&
                                      reinterpret_cast<uintptr_t>(workspace) % 16 == 0),

@@ -434,7 +434,7 @@ def cache_attention(q, cache: KvCache, table, lengths, offsets=None, *, first=No
     stream = _current(device)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((heads, rows), dtype=torch.float32, device=q.device)
-    size = _attention_workspace(device, batch, rows, heads, kv_heads, head_dim, max_new, max_tokens)
+    size = _attention_workspace(device, batch, rows, heads, kv_heads, head_dim, code, max_new, max_tokens)
     work = torch.empty(size, dtype=torch.uint8, device=q.device).data_ptr() if size else 0
     args = _ATTENTION.pack(*fields, at, at_q, out.data_ptr(), lse.data_ptr(), work,
                            _int32(status, "status", (1,), device), row, head, size, heads, head_dim, code, max_new,

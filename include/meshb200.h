@@ -402,7 +402,8 @@ typedef struct mb_cache_attention_args {
   float scale;
 } mb_cache_attention_args;
 int mb_op_cache_attention_workspace(uint32_t batch, size_t rows, uint32_t q_heads, uint32_t kv_heads,
-                                    uint32_t head_dim, uint32_t max_new, uint32_t max_tokens, size_t* bytes);
+                                    uint32_t head_dim, uint32_t dtype, uint32_t max_new, uint32_t max_tokens,
+                                    size_t* bytes);
 int mb_op_cache_attention(const mb_cache_attention_args* args, void* stream);
 /* Per row of logits [rows][vocab] (rows row_stride elements apart): logprob =
  * ln softmax at tokens[row] (0 for -1, MB_IGNORE_TARGET), entropy in nats,
