@@ -135,14 +135,14 @@ SIGNATURES = {
                       [ctypes.c_void_p] * 6),
     "mb_op_adamw": (ctypes.c_int, [ctypes.c_void_p] * 4 + [ctypes.c_size_t, ctypes.POINTER(AdamWC),
                                                            ctypes.c_uint32, ctypes.c_void_p]),
-    # argument structures of the serving operators, packed by ops.py
-    "mb_op_cache_write": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
-    "mb_op_cache_read": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
+    # the serving operators take argument structures; ops.py calls them through the compiled binding
+    "mb_op_cache_write": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "mb_op_cache_read": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "mb_op_cache_attention_workspace": (ctypes.c_int, [ctypes.c_uint32, ctypes.c_size_t] + [ctypes.c_uint32] * 6 +
                                         [c_size_p]),
-    "mb_op_cache_attention": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
-    "mb_op_token_logprobs": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
-    "mb_op_token_logprobs_backward": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
+    "mb_op_cache_attention": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "mb_op_token_logprobs": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "mb_op_token_logprobs_backward": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "mb_gpt_checkpoint_write": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(GptConfigC), c_u32_p, ctypes.c_size_t,
                                                c_float_p, ctypes.c_size_t]),
     "mb_gpt_checkpoint_read": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(GptConfigC), c_u32_p, c_size_p,

@@ -1,4 +1,5 @@
-"""Builds ``libmeshb200.so`` (sm_100a) in-tree with nvcc.
+"""Builds ``libmeshb200.so`` (sm_100a) in-tree with nvcc, and ``_serving``, the
+Python binding of its serving operators, with the host compiler.
 
 Usage: ``python -m grokking_abmod_b200.build`` (or ``build()`` from Python).
 The library exports the C ABI declared in ``include/meshb200.h``.
@@ -7,11 +8,13 @@ The library exports the C ABI declared in ``include/meshb200.h``.
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmeshb200.so")
+BINDING = os.path.join(HERE, "_serving.so")
 
 SOURCES = ["gpt_model.cu", "mesh_ops.cu", "gemm_tc.cu", "simple_model.cu", "config.cpp", "data.cpp",
            "simple_config.cpp", "checkpoint.cpp", "cache_ops.cu", "cache_attention.cu", "logprobs.cu"]
@@ -25,32 +28,60 @@ def _nvcc():
     raise RuntimeError("nvcc not found")
 
 
-def _stale():
-    if not os.path.exists(LIB):
+def _older(target, deps):
+    if not os.path.exists(target):
         return True
-    t = os.path.getmtime(LIB)
-    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)]
-    deps.append(os.path.join(ROOT, "include", "meshb200.h"))
+    t = os.path.getmtime(target)
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-def build(force: bool = False, verbose: bool = False) -> str:
-    """Compiles the library if any source is newer than it; returns its path."""
-    if not force and not _stale():
-        return LIB
-    tmp = LIB + ".tmp"
-    cmd = [_nvcc(), "-std=c++17", "-O3", "-lineinfo", "--threads", "0", *ARCH, "-shared", "-Xcompiler",
-           "-fPIC,-ffp-contract=off",
-           "-I", os.path.join(ROOT, "include"), "-o", tmp]
-    cmd += [os.path.join(CSRC, s) for s in SOURCES]
-    cmd += ["-ldl"]
+def _stale():
+    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f != "binding.cpp"]
+    deps.append(os.path.join(ROOT, "include", "meshb200.h"))
+    return _older(LIB, deps)
+
+
+def _run(cmd, target, verbose):
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
-    os.replace(tmp, LIB)
+        raise RuntimeError(f"{os.path.basename(cmd[0])} failed:\n" + res.stdout + res.stderr)
+    os.replace(target + ".tmp", target)
+
+
+def build(force: bool = False, verbose: bool = False) -> str:
+    """Compiles the library and the binding if any source is newer than them;
+    returns the library's path."""
+    if force or _stale():
+        cmd = [_nvcc(), "-std=c++17", "-O3", "-lineinfo", "--threads", "0", *ARCH, "-shared", "-Xcompiler",
+               "-fPIC,-ffp-contract=off",
+               "-I", os.path.join(ROOT, "include"), "-o", LIB + ".tmp"]
+        cmd += [os.path.join(CSRC, s) for s in SOURCES]
+        cmd += ["-ldl"]
+        _run(cmd, LIB, verbose)
+    build_binding(force, verbose)
     return LIB
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> str:
+    """Compiles ``_serving.so`` against the installed torch and the library
+    (found beside it at run time) if it is older than its sources."""
+    source, header = os.path.join(CSRC, "binding.cpp"), os.path.join(ROOT, "include", "meshb200.h")
+    if not force and not _older(BINDING, [source, header]):
+        return BINDING
+    import torch
+    home = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", os.path.join(ROOT, "include"), "-I", os.path.join(home, "include"),
+           "-I", os.path.join(home, "include", "torch", "csrc", "api", "include"),
+           "-I", os.path.join(cuda, "include"), "-I", sysconfig.get_paths()["include"],
+           source, "-o", BINDING + ".tmp", "-L", HERE, "-l:libmeshb200.so", "-Wl,-rpath,$ORIGIN",
+           "-L", os.path.join(home, "lib"), "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+    _run(cmd, BINDING, verbose)
+    return BINDING
 
 
 if __name__ == "__main__":

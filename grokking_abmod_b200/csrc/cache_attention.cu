@@ -1170,8 +1170,8 @@ void launch_rows(const View& c, const Batch& t, const Queries& q, const Plan& p,
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, join_chunks<T, D, ROWS, TILES ? 1 : 8>, c, t, q, part, p.blocks_per_seq);
-  require(e == cudaSuccess, std::string("cache attention join: ") + cudaGetErrorString(e), MB_ERR_CUDA);
+  launched("cache attention join",
+           cudaLaunchKernelEx(&cfg, join_chunks<T, D, ROWS, TILES ? 1 : 8>, c, t, q, part, p.blocks_per_seq));
 }
 
 template <class T, int D>
@@ -1227,7 +1227,7 @@ int mb_op_cache_attention(const mb_cache_attention_args* a, void* stream) {
     mb::with_dtype(a->dtype, [&](auto tag) {
       using T = typename decltype(tag)::type;
       for (const void* x : {q, (const void*)out})
-        mb::require(reinterpret_cast<uintptr_t>(x) % sizeof(T) == 0, "q and out must be aligned to their elements");
+        mb::aligned_to(x, sizeof(T), "q and out must be aligned to their elements");
       switch (c.width) {
         case 32: return launch<T, 32>(c, t, qs, p, workspace, st);
         case 64: return launch<T, 64>(c, t, qs, p, workspace, st);

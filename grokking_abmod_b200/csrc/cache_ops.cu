@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(kThreads)
 template <class T>
 Rows<T> make_rows(const void* p, size_t row_stride, size_t head_stride) {
   constexpr size_t VEC = Element<T>::kVec;
-  require(reinterpret_cast<uintptr_t>(p) % sizeof(T) == 0, "rows must be aligned to their elements");
+  aligned_to(p, sizeof(T), "rows must be aligned to their elements");
   return Rows<T>{static_cast<const T*>(p), row_stride, head_stride,
                  reinterpret_cast<uintptr_t>(p) % 16 == 0 && row_stride % VEC == 0 && head_stride % VEC == 0};
 }
@@ -284,7 +284,7 @@ int mb_op_cache_read(const mb_cache_read_args* a, void* stream) {
       using T = typename decltype(tag)::type;
       constexpr int VEC = mb::Element<T>::kVec;
       for (const void* p : {(const void*)k_out, (const void*)v_out})
-        mb::require(reinterpret_cast<uintptr_t>(p) % sizeof(T) == 0, "outputs must be aligned to their elements");
+        mb::aligned_to(p, sizeof(T), "outputs must be aligned to their elements");
       const bool vector = head_dim % VEC == 0 && reinterpret_cast<uintptr_t>(k_out) % 16 == 0 &&
                           reinterpret_cast<uintptr_t>(v_out) % 16 == 0;
       const int columns = c.heads * (int)(head_dim / (vector ? VEC : 1));

@@ -97,7 +97,9 @@ void with_dtype(uint32_t dtype, F&& f) {
   throw Error(MB_ERR_INVALID, "dtype must be MB_F32, MB_BF16 or MB_F16");
 }
 
-inline size_t dtype_bytes(uint32_t dtype) { return dtype == MB_F32 ? 4 : 2; }
+inline void aligned_to(const void* p, size_t bytes, const char* message) {
+  require(reinterpret_cast<uintptr_t>(p) % bytes == 0, message);
+}
 
 constexpr int kMaxDevices = 64;
 
@@ -137,8 +139,7 @@ class DeviceOnce {
   std::atomic<uint64_t> done_{0};
 };
 
-inline void launched(const char* what) {
-  const cudaError_t e = cudaGetLastError();
+inline void launched(const char* what, cudaError_t e = cudaGetLastError()) {
   if (e != cudaSuccess) throw Error(MB_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
 }
 

@@ -27,7 +27,9 @@ inline void require(bool ok, const char* message, int code = MB_ERR_INVALID) {
   if (!ok) throw Error(code, message);
 }
 
-inline void need(const void* p, const char* what) { require(p != nullptr, std::string(what) + " must not be null"); }
+inline void need(const void* p, const char* what) {
+  if (p == nullptr) throw Error(MB_ERR_INVALID, std::string(what) + " must not be null");
+}
 
 // The calling thread's last status and message (read by mb_last_error).
 void set_last_error(int code, const char* message);

@@ -608,10 +608,6 @@ inline void shape(size_t rows, uint32_t vocab, size_t stride) {
   require(stride >= vocab || rows == 1, "the row stride must be at least vocab");
 }
 
-inline void aligned(const void* p, size_t bytes, const char* what) {
-  require((reinterpret_cast<uintptr_t>(p) % bytes) == 0, std::string(what) + " must be aligned to its elements");
-}
-
 template <class T, int R>
 void launch_small(const T* x, size_t stride, size_t rows, uint32_t vocab, const int* tokens, uint32_t top, const Out& o,
                   cudaStream_t st) {
@@ -639,9 +635,8 @@ void launch_wide(const T* x, size_t stride, size_t rows, uint32_t vocab, const i
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e =
-      cudaLaunchKernelEx(&cfg, forward_wide<T, kWarps, TOP>, x, stride, rows, (int)vocab, tokens, (int)top, o);
-  require(e == cudaSuccess, std::string("token log-probabilities: ") + cudaGetErrorString(e), MB_ERR_CUDA);
+  launched("token log-probabilities",
+           cudaLaunchKernelEx(&cfg, forward_wide<T, kWarps, TOP>, x, stride, rows, (int)vocab, tokens, (int)top, o));
 }
 
 template <class T>
@@ -677,7 +672,7 @@ int mb_op_token_logprobs(const mb_token_logprobs_args* a, void* stream) {
     const Out o{a->logprob, a->entropy, a->lse, a->top_logprob, a->top_index, a->d_status};
     mb::with_dtype(a->dtype, [&](auto tag) {
       using T = typename decltype(tag)::type;
-      aligned(a->logits, sizeof(T), "logits");
+      mb::aligned_to(a->logits, sizeof(T), "logits must be aligned to their elements");
       launch_forward<T>(static_cast<const T*>(a->logits), a->row_stride, a->rows, a->vocab, a->tokens, top, o,
                         (cudaStream_t)stream);
       mb::launched("token log-probabilities");
@@ -699,8 +694,8 @@ int mb_op_token_logprobs_backward(const mb_token_logprobs_backward_args* a, void
     cudaStream_t st = (cudaStream_t)stream;
     mb::with_dtype(a->dtype, [&](auto tag) {
       using T = typename decltype(tag)::type;
-      aligned(a->logits, sizeof(T), "logits");
-      aligned(a->dlogits, sizeof(T), "dlogits");
+      mb::aligned_to(a->logits, sizeof(T), "logits must be aligned to their elements");
+      mb::aligned_to(a->dlogits, sizeof(T), "dlogits must be aligned to their elements");
       const T* x = static_cast<const T*>(a->logits);
       T* d = static_cast<T*>(a->dlogits);
       const size_t rows = a->rows;

@@ -19,8 +19,6 @@ with ``check_status`` when convenient.
 
 import ctypes
 import functools
-import math
-import struct
 from typing import NamedTuple
 
 from . import _lib
@@ -218,32 +216,14 @@ class TokenLogprobs(NamedTuple):
 
 
 @functools.cache
-def _torch():
-    import torch
-    return torch
+def _binding():
+    """The compiled binding (csrc/binding.cpp), which checks the tensors and
+    calls the library; built with it."""
+    _lib.load()
+    import torch  # noqa: F401  (its libraries first)
 
-
-@functools.cache
-def _dtypes():
-    torch = _torch()
-    return {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # MB_F32, MB_BF16, MB_F16
-
-
-def _dtype(dtype, name):
-    code = _dtypes().get(dtype)
-    if code is None:
-        raise ValueError(f"{name} must be float32, bfloat16 or float16")
-    return code
-
-
-# The C argument structures (include/meshb200.h); every one begins with a
-# cache and the rows' places where the operator has them.
-_CACHE_WHERE = "4P4I3P2N2I"
-_WRITE = struct.Struct(_CACHE_WHERE + "2P4NP4I")
-_READ = struct.Struct(_CACHE_WHERE + "4P4I")
-_ATTENTION = struct.Struct(_CACHE_WHERE + "6P3N5If")
-_LOGPROBS = struct.Struct("8P2N4I")
-_LOGPROBS_BACKWARD = struct.Struct("8P2N2I")
+    from . import _serving
+    return _serving
 
 
 def new_kv_cache(pages: int, heads: int, head_dim: int, page_tokens: int = 32, device="cuda") -> KvCache:
@@ -273,88 +253,6 @@ def check_status(status) -> None:
         raise RuntimeError("; ".join(text for bit, text in _STATUS_BITS if code & bit) or f"device status {code}")
 
 
-def _cache_where(cache, table, lengths, offsets, rows):
-    """(fields of the cache and of the rows' places, device index)."""
-    torch = _torch()
-    k, v, ks, vs = cache
-    shape, device = k.shape, k.get_device()
-    i8, f32, i32 = torch.int8, torch.float32, torch.int32
-    if len(shape) != 4 or v.shape != shape or not (
-            k.dtype is i8 and v.dtype is i8 and k.is_contiguous() and v.is_contiguous()):
-        raise ValueError("cache.k and cache.v must be contiguous int8 tensors [pages][heads][page_tokens][width]")
-    pages, heads, tokens, width = shape
-    scales = shape[:2]
-    if not (ks.shape == scales and vs.shape == scales and ks.dtype is f32 and vs.dtype is f32
-            and ks.is_contiguous() and vs.is_contiguous()):
-        raise ValueError("cache.k_scale and cache.v_scale must be contiguous float32 tensors [pages][heads]")
-    if table.dtype is not i32 or table.ndim != 2:
-        raise ValueError("table must be an int32 tensor [batch][pages]")
-    batch, per = table.shape
-    stride, step = table.stride()
-    if step != 1 and per > 1:
-        raise ValueError("table must have adjacent page numbers")
-    if batch <= 1:
-        stride = per
-    if lengths.dtype is not i32 or lengths.shape != (batch,) or not lengths.is_contiguous():
-        raise ValueError("lengths must be a contiguous int32 tensor [batch]")
-    if offsets is None:
-        at = 0
-    elif offsets.dtype is not i32 or offsets.shape != (batch + 1,) or not offsets.is_contiguous():
-        raise ValueError("offsets must be a contiguous int32 tensor [batch + 1]")
-    else:
-        at = offsets.data_ptr()
-        if offsets.get_device() != device:
-            raise ValueError("the operands must be on one CUDA device")
-    if device < 0 or not (v.get_device() == ks.get_device() == vs.get_device() == table.get_device()
-                          == lengths.get_device() == device):
-        raise ValueError("the operands must be on one CUDA device")
-    return (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages, heads, tokens, width,
-            table.data_ptr(), lengths.data_ptr(), at, stride, rows, per, batch), device
-
-
-def _int32(t, name, shape, device):
-    """The address of an optional int32 tensor."""
-    if t is None:
-        return 0
-    if not (t.dtype is _torch().int32 and t.get_device() == device and t.shape == shape and t.is_contiguous()):
-        raise ValueError(f"{name} must be a contiguous int32 tensor {list(shape)} on the operands' device")
-    return t.data_ptr()
-
-
-def _rows3(t, name, device):
-    """(address, row stride, head stride) of [rows][heads][head_dim] rows."""
-    row, head, channel = t.stride()
-    if channel != 1 and t.shape[2] > 1:
-        raise ValueError(f"{name} must have adjacent channels")
-    if row < 0 or head < 0:
-        raise ValueError(f"{name} must not have negative strides")
-    if t.get_device() != device:
-        raise ValueError(f"{name} must be on the cache's device")
-    return t.data_ptr(), row, head
-
-
-def _sizes(*values):
-    for v in values:
-        if not 0 <= v < 1 << 32:
-            raise ValueError("sizes must be in 0..2^32-1")
-
-
-def _current(device):
-    """The current stream's handle; the operands must be on the current device."""
-    torch = _torch()
-    if device != torch.cuda.current_device():
-        raise ValueError("operands must be on the current CUDA device")
-    return torch._C._cuda_getCurrentRawStream(device)
-
-
-@functools.lru_cache(maxsize=4096)
-def _attention_workspace(device, *sizes):
-    """Bytes that an attention of these sizes needs on this device."""
-    n = ctypes.c_size_t()
-    check(_lib.load().mb_op_cache_attention_workspace(*sizes, ctypes.byref(n)))
-    return n.value
-
-
 def cache_write(cache: KvCache, k, v, table, lengths, offsets=None, *, max_new: int = None, status=None) -> None:
     """Quantises the new rows k, v [rows][heads][head_dim] into their pages.
 
@@ -363,20 +261,7 @@ def cache_write(cache: KvCache, k, v, table, lengths, offsets=None, *, max_new: 
     offsets[b] .. offsets[b+1] are sequence b's newest (``offsets`` None: row b
     is).  ``max_new``: at least the largest number of new rows of a sequence
     (default: 1 without offsets, else all rows)."""
-    if k.ndim != 3 or v.shape != k.shape or v.dtype is not k.dtype:
-        raise ValueError("k and v must be [rows][heads][head_dim] of one shape and type")
-    rows, heads, head_dim = k.shape
-    if heads != cache[0].shape[1]:
-        raise ValueError("k and v must have the cache's heads")
-    if max_new is None:
-        max_new = rows if offsets is not None else 1
-    fields, device = _cache_where(cache, table, lengths, offsets, rows)
-    at_k, k_row, k_head = _rows3(k, "k", device)
-    at_v, v_row, v_head = _rows3(v, "v", device)
-    _sizes(max_new)
-    args = _WRITE.pack(*fields, at_k, at_v, k_row, k_head, v_row, v_head, _int32(status, "status", (1,), device),
-                       head_dim, _dtype(k.dtype, "k"), max_new, 0)
-    check(_lib.load().mb_op_cache_write(args, _current(device)))
+    check(_binding().cache_write(*cache, table, lengths, offsets, k, v, max_new, status))
 
 
 def cache_read(cache: KvCache, table, lengths, tokens: int, *, first=None, head_dim: int = None, dtype=None,
@@ -385,23 +270,8 @@ def cache_read(cache: KvCache, table, lengths, tokens: int, *, first=None, head_
     first[b] + tokens - 1 (``first`` None: from 0) of each sequence, zeros
     past its length.  ``head_dim`` defaults to the cache's width, ``dtype`` to
     float32."""
-    torch = _torch()
-    batch = table.shape[0]
-    fields, device = _cache_where(cache, table, lengths, None, batch)
-    heads, width = fields[5], fields[7]
-    head_dim = width if head_dim is None else head_dim
-    dtype = torch.float32 if dtype is None else dtype
-    code = _dtype(dtype, "dtype")
-    _sizes(tokens, head_dim)
-    at = _int32(first, "first", (batch,), device)
-    stream = _current(device)
-    shape = (batch, tokens, heads, head_dim)
-    k = torch.empty(shape, dtype=dtype, device=cache[0].device)
-    v = torch.empty_like(k)
-    args = _READ.pack(*fields, at, k.data_ptr(), v.data_ptr(), _int32(status, "status", (1,), device), head_dim, code,
-                      tokens, 0)
-    check(_lib.load().mb_op_cache_read(args, stream))
-    return k, v
+    r = _binding().cache_read(*cache, table, lengths, tokens, first, head_dim, dtype, status)
+    return r if r.__class__ is tuple else check(r)
 
 
 def cache_attention(q, cache: KvCache, table, lengths, offsets=None, *, first=None, scale: float = None,
@@ -417,42 +287,8 @@ def cache_attention(q, cache: KvCache, table, lengths, offsets=None, *, first=No
     table, lengths, offsets, max_new as in ``cache_write``; ``scale`` defaults
     to 1 / sqrt(head_dim); ``max_tokens``, about the largest length, is how
     long sequences are cut over the GPU (default: what the table can hold)."""
-    torch = _torch()
-    if q.ndim != 3:
-        raise ValueError("q must be [rows][q_heads][head_dim]")
-    rows, heads, head_dim = q.shape
-    fields, device = _cache_where(cache, table, lengths, offsets, rows)
-    at_q, row, head = _rows3(q, "q", device)
-    code = _dtype(q.dtype, "q")
-    kv_heads, batch = fields[5], fields[14]
-    if max_new is None:
-        max_new = rows if offsets is not None else 1
-    if max_tokens is None:
-        max_tokens = min(fields[13] * fields[6], (1 << 31) - 1)
-    _sizes(max_new, max_tokens)
-    at = _int32(first, "first", (batch,), device)
-    stream = _current(device)
-    out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse = torch.empty((heads, rows), dtype=torch.float32, device=q.device)
-    size = _attention_workspace(device, batch, rows, heads, kv_heads, head_dim, code, max_new, max_tokens)
-    work = torch.empty(size, dtype=torch.uint8, device=q.device).data_ptr() if size else 0
-    args = _ATTENTION.pack(*fields, at, at_q, out.data_ptr(), lse.data_ptr(), work,
-                           _int32(status, "status", (1,), device), row, head, size, heads, head_dim, code, max_new,
-                           max_tokens, 1.0 / math.sqrt(head_dim) if scale is None else scale)
-    check(_lib.load().mb_op_cache_attention(args, stream))
-    return out, lse
-
-
-def _logit_rows(logits):
-    """(address, row stride, rows, vocab, type, device) of logits."""
-    if logits.ndim != 2:
-        raise ValueError("logits must be [rows][vocab]")
-    rows, vocab = logits.shape
-    row, column = logits.stride()
-    device = logits.get_device()
-    if device < 0 or (column != 1 and vocab > 1) or row < 0:
-        raise ValueError("logits must be a CUDA tensor [rows][vocab] with adjacent columns")
-    return logits.data_ptr(), row if rows > 1 else vocab, rows, vocab, _dtype(logits.dtype, "logits"), device
+    r = _binding().cache_attention(*cache, table, lengths, offsets, q, first, scale, max_new, max_tokens, status)
+    return r if r.__class__ is tuple else check(r)
 
 
 def token_logprobs(logits, tokens, top: int = 0, *, status=None) -> TokenLogprobs:
@@ -460,43 +296,13 @@ def token_logprobs(logits, tokens, top: int = 0, *, status=None) -> TokenLogprob
     of IGNORE_TARGET, gives 0), entropies, and the ``top`` (0..32) most likely
     tokens of each row of ``logits`` [rows][vocab], ties to the lowest index.
     -inf masks a token; a row of masked tokens gives -inf and entropy 0."""
-    torch = _torch()
-    at, stride, rows, vocab, code, device = _logit_rows(logits)
-    _sizes(vocab, top)
-    at_tokens = _int32(tokens, "tokens", (rows,), device)
-    word = _int32(status, "status", (1,), device)
-    stream = _current(device)
-    # one allocation: logprob, entropy, lse, then the top log-probabilities and their indices
-    room = torch.empty(rows * (3 + 2 * top), dtype=torch.float32, device=logits.device)
-    logprob, entropy, lse, best, index = room.split((rows, rows, rows, rows * top, rows * top))
-    if rows:
-        to = room.data_ptr()
-        args = _LOGPROBS.pack(at, at_tokens, to, to + 4 * rows, to + 8 * rows, to + 12 * rows,
-                              to + (12 + 4 * top) * rows, word, stride, rows, vocab, code, top, 0)
-        check(_lib.load().mb_op_token_logprobs(args, stream))
-    return TokenLogprobs(logprob, entropy, lse, best.view(rows, top), index.view(torch.int32).view(rows, top))
+    r = _binding().token_logprobs(logits, tokens, top, status)
+    return TokenLogprobs._make(r) if r.__class__ is tuple else check(r)
 
 
 def token_logprobs_backward(logits, tokens, lse, entropy, dlogprob=None, dentropy=None, *, status=None):
     """dlogits of sum(dlogprob * logprob + dentropy * entropy), in the type of
     the logits, from the forward's ``lse`` and ``entropy``; dlogprob or
     dentropy None: zeros."""
-    torch = _torch()
-    at, stride, rows, vocab, code, device = _logit_rows(logits)
-    _sizes(vocab)
-    at_tokens = _int32(tokens, "tokens", (rows,), device)
-    given = []
-    for t, name in ((lse, "lse"), (entropy, "entropy"), (dlogprob, "dlogprob"), (dentropy, "dentropy")):
-        if t is None:
-            given.append(0)
-        elif t.dtype is torch.float32 and t.shape == (rows,) and t.get_device() == device and t.is_contiguous():
-            given.append(t.data_ptr())
-        else:
-            raise ValueError(f"{name} must be a contiguous float32 tensor [rows] on the logits' device")
-    word = _int32(status, "status", (1,), device)
-    stream = _current(device)
-    d = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
-    if rows:
-        args = _LOGPROBS_BACKWARD.pack(at, at_tokens, *given, d.data_ptr(), word, stride, rows, vocab, code)
-        check(_lib.load().mb_op_token_logprobs_backward(args, stream))
-    return d
+    r = _binding().token_logprobs_backward(logits, tokens, lse, entropy, dlogprob, dentropy, status)
+    return r if r.__class__ is not int else check(r)
