@@ -13,7 +13,6 @@ namespace mb {
 namespace cache {
 
 constexpr int kThreads = 256;
-constexpr int kHeld = 8;  // 16-byte input vectors a thread holds between the reduction and the store
 
 template <class T>
 struct Rows {
@@ -66,20 +65,22 @@ __device__ __forceinline__ void store_codes(int8_t* at, uint4 raw, float inverse
   }
 }
 
-// A group of G threads (32: a warp, kThreads: the CTA) writes one page of one
-// head, of K (blockIdx.y 0) or V (1).
-template <class T, int G>
-__global__ void __launch_bounds__(kThreads)
-    write_pages(View c, Batch t, Rows<T> k, Rows<T> v, int head_dim, int page_slots, int* status) {
-  constexpr int VEC = Element<T>::kVec;
+// A group of G threads (32: a warp, else the CTA) writes one page of one head,
+// of K and of V.  A thread holds up to HELD 16-byte vectors of each between
+// the reduction and the store; the two tensors' loads go out together, since
+// what a group waits for is mostly the chain length -> page -> rows.
+template <class T, int G, int HELD>
+__global__ void __launch_bounds__(G == 32 ? 128 : G)
+    write_pages(View c, Batch t, Rows<T> k, Rows<T> v, int head_dim, int page_slots, unsigned units, int* status) {
+  constexpr int VEC = Element<T>::kVec, GROUPS = G == 32 ? 4 : 1;
   const int id = threadIdx.x % G;
-  const size_t unit = (size_t)blockIdx.x * (kThreads / G) + threadIdx.x / G;
-  const int head = (int)(unit % c.heads);
-  const size_t rest = unit / c.heads;
-  const int b = (int)(rest / page_slots), slot_page = (int)(rest % page_slots);
-  if (b >= t.count) return;
+  const unsigned unit = blockIdx.x * GROUPS + threadIdx.x / G;
+  if (unit >= units) return;
+  const unsigned rest = unit / (unsigned)c.heads;
+  const int head = (int)(unit - rest * c.heads);
+  const int b = (int)(rest / (unsigned)page_slots), slot_page = (int)(rest - (unsigned)b * page_slots);
   const Span s = span_of(t, c, b);
-  const bool report = status != nullptr && id == 0 && head == 0 && blockIdx.y == 0;
+  const bool report = status != nullptr && id == 0 && head == 0;
   if (report && slot_page == 0) {
     // pages past the announced number of new rows are not visited
     const bool missed = s.fresh && ((s.length - s.fresh) >> c.shift) + page_slots <= (s.length - 1) >> c.shift;
@@ -97,73 +98,96 @@ __global__ void __launch_bounds__(kThreads)
     if (report) atomicOr(status, kBadPage);
     return;
   }
-  const Rows<T>& in = blockIdx.y ? v : k;
-  int8_t* codes = (blockIdx.y ? c.v : c.k) + c.row(page, head, 0);
-  float* scale_at = (blockIdx.y ? c.v_scale : c.k_scale) + c.scale_at(page, head);
-  const float before = from > lo ? *scale_at : 0.f;
-
+  float* scale_at[2] = {c.k_scale + c.scale_at(page, head), c.v_scale + c.scale_at(page, head)};
+  float before[2] = {0.f, 0.f};
+  if (from > lo) {
+    before[0] = *scale_at[0];
+    before[1] = *scale_at[1];
+  }
   const int per_row = c.width / VEC;  // width is a multiple of 32
   const int chunks = (to - from) * per_row;
   const size_t row0 = s.row + (from - old);
-  uint4 raw[kHeld];
-  uint32_t most = 0;
-  const bool held = chunks <= G * kHeld;
-  for (int base = 0; base < chunks; base += G * kHeld) {
+  uint4 raw[2][HELD];
+  uint32_t most[2] = {0, 0};
+  auto load = [&](int base) {
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
+    for (int i = 0; i < HELD; ++i) {
       const int e = base + i * G + id;
       if (e < chunks) {
-        const int r = e / per_row;
-        raw[i] = load_chunk(in, row0 + r, head, (e - r * per_row) * VEC, head_dim);
+        const int r = e / per_row, ch = (e - r * per_row) * VEC;
+        raw[0][i] = load_chunk(k, row0 + r, head, ch, head_dim);
+        raw[1][i] = load_chunk(v, row0 + r, head, ch, head_dim);
       }
     }
+  };
+  for (int base = 0; base < chunks; base += G * HELD) {
+    load(base);
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i)
-      if (base + i * G + id < chunks) most = max(most, magnitude<T>(raw[i]));
+    for (int i = 0; i < HELD; ++i)
+      if (base + i * G + id < chunks) {
+        most[0] = max(most[0], magnitude<T>(raw[0][i]));
+        most[1] = max(most[1], magnitude<T>(raw[1][i]));
+      }
   }
-  most = __reduce_max_sync(0xFFFFFFFFu, most);
+  // before every group's store of a scale below: all its threads have read it
+  most[0] = __reduce_max_sync(0xFFFFFFFFu, most[0]);
+  most[1] = __reduce_max_sync(0xFFFFFFFFu, most[1]);
   if constexpr (G > 32) {
-    __shared__ uint32_t parts[G / 32];
-    if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = most;
+    __shared__ uint2 parts[G / 32];
+    if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = make_uint2(most[0], most[1]);
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < G / 32; ++w) most = max(most, parts[w]);
-  }
-  float scale = scale_for(most);
-  if (from > lo) {
-    // the page's earlier tokens: the scale never shrinks, NaN stays
-    if (before != before || before > scale) scale = before;
-    if (scale != before) {
-      const float ratio = before / scale;
-      uint32_t* w = reinterpret_cast<uint32_t*>(codes);
-      for (int e = id; e < (from - lo) * (c.width / 4); e += G) {
-        const uint32_t q = w[e];
-        w[e] = pack_codes(rintf((float)(int8_t)q * ratio), rintf((float)(int8_t)(q >> 8) * ratio),
-                          rintf((float)(int8_t)(q >> 16) * ratio), rintf((float)(int8_t)(q >> 24) * ratio));
-      }
+    for (int w = 0; w < G / 32; ++w) {
+      most[0] = max(most[0], parts[w].x);
+      most[1] = max(most[1], parts[w].y);
     }
   }
-  // the group read `before` before this store: in lockstep for a warp, behind
-  // the barrier above for a CTA
-  if (id == 0) *scale_at = scale;
-  const float inverse = 1.0f / scale;
-  codes += (size_t)(from - lo) * c.width;
-  for (int base = 0; base < chunks; base += G * kHeld) {
+  float inverse[2];
+  const size_t page_at = c.row(page, head, 0);
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
+  for (int which = 0; which < 2; ++which) {
+    float scale = scale_for(most[which]);
+    if (from > lo) {
+      // the page's earlier tokens: the scale never shrinks, NaN stays
+      const float was = before[which];
+      if (was != was || was > scale) scale = was;
+      if (scale != was) {
+        const float ratio = was / scale;
+        uint32_t* w = reinterpret_cast<uint32_t*>((which ? c.v : c.k) + page_at);
+        for (int e = id; e < (from - lo) * (c.width / 4); e += G) {
+          const uint32_t q = w[e];
+          w[e] = pack_codes(rintf((float)(int8_t)q * ratio), rintf((float)(int8_t)(q >> 8) * ratio),
+                            rintf((float)(int8_t)(q >> 16) * ratio), rintf((float)(int8_t)(q >> 24) * ratio));
+        }
+      }
+    }
+    if (id == 0) *scale_at[which] = scale;
+    inverse[which] = 1.0f / scale;
+  }
+  const size_t at = page_at + (size_t)(from - lo) * c.width;
+  const bool held = chunks <= G * HELD;
+  for (int base = 0; base < chunks; base += G * HELD) {
+    if (!held) load(base);
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
       const int e = base + i * G + id;
       if (e < chunks) {
-        if (!held) {
-          const int r = e / per_row;
-          raw[i] = load_chunk(in, row0 + r, head, (e - r * per_row) * VEC, head_dim);
-        }
-        store_codes<T>(codes + (size_t)e * VEC, raw[i], inverse);
+        store_codes<T>(c.k + at + (size_t)e * VEC, raw[0][i], inverse[0]);
+        store_codes<T>(c.v + at + (size_t)e * VEC, raw[1][i], inverse[1]);
       }
     }
   }
 }
 
-constexpr int kReadTokens = 4;  // tokens a thread has in flight
+template <class T, int G, int HELD>
+void launch_write(const View& c, const Batch& t, const Rows<T>& k, const Rows<T>& v, int head_dim, int page_slots,
+                  unsigned units, int* status, cudaStream_t st) {
+  constexpr unsigned GROUPS = G == 32 ? 4 : 1;
+  write_pages<T, G, HELD><<<(units + GROUPS - 1) / GROUPS, G == 32 ? 128 : G, 0, st>>>(c, t, k, v, head_dim, page_slots,
+                                                                                     units, status);
+}
+
+constexpr int kReadTokens = 8;  // tokens a thread has in flight
 
 // out [batch][tokens][heads][head_dim]: blockIdx.x a run of tokens of one
 // sequence, blockIdx.y a run of columns (head, chunk), blockIdx.z K or V.
@@ -218,7 +242,7 @@ __global__ void __launch_bounds__(kThreads)
     for (int e = 0; e < CHUNK; ++e)
       x[e] = (float)(int8_t)((e < 4 ? q[u].x : q[u].y) >> (8 * (e & 3))) * scale[u];
     if constexpr (CHUNK == 1) *o = Element<T>::from(x[0]);
-    else *reinterpret_cast<uint4*>(o) = Element<T>::pack(x);
+    else __stcs(reinterpret_cast<uint4*>(o), Element<T>::pack(x));  // not read again here
   }
 }
 
@@ -247,21 +271,20 @@ int mb_op_cache_write(const mb_cache_write_args* a, void* stream) {
     mb::need(a->v, "v");
     const int page_slots = (int)(((size_t)max_new + c.tokens - 2) / c.tokens + 1);
     const size_t units = (size_t)t.count * page_slots * c.heads;
-    cudaStream_t st = (cudaStream_t)stream;
+    mb::require(units <= (size_t)INT_MAX, "too many pages for one call");
     mb::with_dtype(a->dtype, [&](auto tag) {
       using T = typename decltype(tag)::type;
       const Rows<T> kr = make_rows<T>(a->k, a->k_row_stride, a->k_head_stride);
       const Rows<T> vr = make_rows<T>(a->v, a->v_row_stride, a->v_head_stride);
-      // a warp where it can hold a page's new rows in registers, else a CTA
+      // as few threads as hold a page's new rows in registers
       const size_t vectors = std::min<size_t>(max_new, c.tokens) * c.width / mb::Element<T>::kVec;
-      const bool warp = vectors <= 32 * kHeld;
-      const size_t blocks = warp ? (units + kThreads / 32 - 1) / (kThreads / 32) : units;
-      mb::require(blocks <= (size_t)INT_MAX, "too many pages for one call");
-      const dim3 grid((unsigned)blocks, 2);
-      if (warp)
-        write_pages<T, 32><<<grid, kThreads, 0, st>>>(c, t, kr, vr, (int)a->head_dim, page_slots, a->d_status);
-      else
-        write_pages<T, kThreads><<<grid, kThreads, 0, st>>>(c, t, kr, vr, (int)a->head_dim, page_slots, a->d_status);
+      const int hd = (int)a->head_dim;
+      const unsigned n = (unsigned)units;
+      const cudaStream_t st = (cudaStream_t)stream;
+      if (vectors <= 32 * 4) launch_write<T, 32, 4>(c, t, kr, vr, hd, page_slots, n, a->d_status, st);
+      else if (vectors <= 128 * 4) launch_write<T, 128, 4>(c, t, kr, vr, hd, page_slots, n, a->d_status, st);
+      else if (vectors <= 256 * 4) launch_write<T, 256, 4>(c, t, kr, vr, hd, page_slots, n, a->d_status, st);
+      else launch_write<T, 256, 8>(c, t, kr, vr, hd, page_slots, n, a->d_status, st);
       mb::launched("cache write");
     });
   });
