@@ -15,8 +15,9 @@
 // are known when the sums are: at least k elements reach the k-th largest of
 // them, and few more do.  Only the threads whose maximum reaches it (k of
 // them) look at their elements again; what they find is sorted in registers.
-// Rows where too many elements tie there, or hold NaN or nothing but masked
-// tokens, go through a slower list that is right for any row.
+// Where fewer than k elements are not masked, the first masked ones follow
+// them.  Rows where too many elements tie at the k-th, or with NaN, go through
+// a slower list that is right for any row.
 
 #include <algorithm>
 #include <climits>
@@ -110,6 +111,7 @@ __device__ __forceinline__ uint32_t ordered(float x) {
   if (x != x) return 0xFFFFFFFFu;
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
+constexpr uint32_t kUnmasked = 0x00800000u;  // the key above that of -inf: of the lowest finite value
 __device__ __forceinline__ float unordered(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k);
 }
@@ -193,29 +195,31 @@ struct Out {
   int* status;
 };
 
+// A row's statistics; t its token, valid: inside the vocabulary, xt its logit.
+// Returns lse.
+__device__ __forceinline__ float store_row(const Out& o, size_t row, Stats st, int t, bool valid, float xt) {
+  const bool none = st.m == -INFINITY && st.s == 0.f;  // every token masked
+  const float log_s = logf(st.s);
+  const float lse = none ? -INFINITY : (st.m == -INFINITY ? st.s : st.m + log_s);
+  o.lse[row] = lse;
+  o.entropy[row] = none ? 0.f : log_s - st.a / st.s * kLn2;
+  if (t != -1 && !valid && o.status) atomicOr(o.status, 2);
+  o.logprob[row] = t == -1 ? 0.f : !valid ? NAN : none ? -INFINITY : xt - lse;
+  return lse;
+}
+
 // Writes a row's results; one warp, with the joined statistics in every lane
 // and the list in its lanes.
 template <class T>
 __device__ __forceinline__ void finish(const Out& o, size_t row, const T* x, int vocab, const int* tokens, int top,
                                        Stats st, u64 mine, int lane) {
-  const bool none = st.m == -INFINITY && st.s == 0.f;  // every token masked
-  const float log_s = logf(st.s);
-  const float lse = none ? -INFINITY : (st.m == -INFINITY ? st.s : st.m + log_s);
+  float lse = 0.f;
   if (lane == 0) {
-    o.lse[row] = lse;
-    o.entropy[row] = none ? 0.f : log_s - st.a / st.s * kLn2;
     const int t = tokens[row];
-    float lp = 0.f;
-    if (t != -1) {
-      if ((unsigned)t < (unsigned)vocab) {
-        lp = none ? -INFINITY : Element<T>::to(x[t]) - lse;
-      } else {
-        lp = NAN;
-        if (o.status) atomicOr(o.status, 2);
-      }
-    }
-    o.logprob[row] = lp;
+    const bool valid = (unsigned)t < (unsigned)vocab;
+    lse = store_row(o, row, st, t, valid, valid ? Element<T>::to(x[t]) : 0.f);
   }
+  lse = __shfl_sync(kFull, lse, 0);
   if (lane < top) {
     const float v = unordered((uint32_t)(mine >> 32));
     o.top_logprob[row * top + lane] = v == -INFINITY ? v : v - lse;
@@ -325,6 +329,38 @@ __device__ __forceinline__ uint32_t remote_u32(const void* p, uint32_t rank) {
   return v;
 }
 
+// Eight lanes per row, R elements a lane, without top tokens: the smallest
+// vocabularies are all latency, and four rows a warp share it.
+template <class T, int R>
+__global__ void __launch_bounds__(kThreads)
+    forward_narrow(const T* __restrict__ logits, size_t stride, size_t rows, int vocab, const int* __restrict__ tokens,
+                   Out o) {
+  constexpr int G = 8;
+  const int id = threadIdx.x % G;
+  const size_t at = (size_t)blockIdx.x * (kThreads / G) + threadIdx.x / G;
+  const size_t row = at < rows ? at : rows - 1;  // whole warps shuffle; rows past the last are not stored
+  const T* x = logits + row * stride;
+  const int t = tokens[row];
+  const bool valid = (unsigned)t < (unsigned)vocab;
+  const float xt = valid ? Element<T>::to(x[t]) : 0.f;
+  float v[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) v[r] = id + G * r < vocab ? Element<T>::to(x[id + G * r]) : -INFINITY;
+  float mx = v[0];
+#pragma unroll
+  for (int r = 1; r < R; ++r) mx = fmaxf(mx, v[r]);
+#pragma unroll
+  for (int i = G / 2; i; i >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, i));
+  Stats st = empty_stats();
+  accumulate(st, v, mx);
+#pragma unroll
+  for (int i = G / 2; i; i >>= 1) {
+    st.s += __shfl_xor_sync(kFull, st.s, i);
+    st.a += __shfl_xor_sync(kFull, st.a, i);
+  }
+  if (id == 0 && at < rows) store_row(o, row, st, t, valid, xt);
+}
+
 // The largest of a 16-byte vector's elements.
 template <class T>
 __device__ __forceinline__ float vector_max(uint4 raw) {
@@ -354,7 +390,7 @@ __global__ void __launch_bounds__(kThreads)
   __shared__ uint32_t maxima[kWarps][32];
   __shared__ u64 found[W == 1 ? kWarps : 1][kFound];
   __shared__ int counts[W == 1 ? kWarps : 1];
-  __shared__ uint32_t limit;
+  __shared__ uint32_t limit;  // of one row, W > 1
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int id = W == 1 ? lane : threadIdx.x, group = W == 1 ? warp : 0;
   const uint32_t rank = W == 1 ? 0 : cluster_rank(), ranks = W == 1 ? 1 : cluster_size();
@@ -420,13 +456,15 @@ __global__ void __launch_bounds__(kThreads)
       }
       // NaN anywhere: no limit
       const bool nan = __shfl_sync(kFull, sorted, 0) == 0xFFFFFFFFu;
-      if (warp == 0 && lane == top - 1) limit = nan ? 0 : sorted;
+      if (warp == 0 && lane == top - 1) limit = nan ? 0 : max(sorted, kUnmasked);
       __syncthreads();
     } else {
       __syncwarp();
     }
-    const uint32_t least = W > 1 ? limit : __shfl_sync(kFull, sorted, 0) == 0xFFFFFFFFu ? 0 : __shfl_sync(kFull, sorted, top - 1);
-    const bool plain = least > ordered(-INFINITY);
+    uint32_t least = limit;
+    if (W == 1)
+      least = __shfl_sync(kFull, sorted, 0) == 0xFFFFFFFFu ? 0 : max(__shfl_sync(kFull, sorted, top - 1), kUnmasked);
+    const bool plain = least != 0;
     if (plain && reach >= least) {
       auto take = [&](float v, int index) {
         if (ordered(v) >= least) {
@@ -456,6 +494,20 @@ __global__ void __launch_bounds__(kThreads)
     }
     if (W > 1) __syncthreads();
     else __syncwarp();
+    if (plain && least == kUnmasked && counts[group] < top) {
+      // every element that is not masked is found: the first masked ones
+      // follow, and the first 2 kMaxTop elements hold as many as are wanted
+      if (W > 1) __syncthreads();
+      else __syncwarp();
+      const int begins = rank == 0 ? 0 : head + begin * VEC, ends = rank == 0 && ranks == 1 ? vocab : head + end * VEC;
+      for (int i = id; i < 2 * kMaxTop; i += GROUP)
+        if (begins + i < ends && ordered(Element<T>::to(x[begins + i])) < kUnmasked) {
+          const int at = atomicAdd(&counts[group], 1);
+          if (at < kFound) found[group][at] = top_key(-INFINITY, (uint32_t)(begins + i));
+        }
+      if (W > 1) __syncthreads();
+      else __syncwarp();
+    }
     const int count = counts[group];
     if (plain && count >= top && count <= kFound) {
       if (W == 1) mine = sort_found(found[group], count, lane);
@@ -549,7 +601,7 @@ __device__ __forceinline__ float element_grad(const RowGrad& r, float x, int j) 
   return r.none ? 0.f : d;
 }
 
-// A group of G threads per row (32: a warp; kThreads: the CTA).
+// A group of G threads per row (8, a warp, or the CTA).
 template <class T, int G>
 __global__ void __launch_bounds__(kThreads)
     backward_rows(const T* __restrict__ logits, size_t stride, size_t rows, int vocab, GradIn in,
@@ -583,8 +635,9 @@ __global__ void __launch_bounds__(kThreads)
           bd[j + u * G] = Element<T>::pack(v);
         }
     }
-    if (part == 0 && id < head + vocab - tail) {
-      const int at = id < head ? id : tail + id - head;
+    // fewer than 2 VEC elements left over
+    for (int i = id; part == 0 && i < head + vocab - tail; i += G) {
+      const int at = i < head ? i : tail + i - head;
       d[at] = Element<T>::from(element_grad(r, Element<T>::to(x[at]), at));
     }
   } else {
@@ -642,6 +695,12 @@ void launch_wide(const T* x, size_t stride, size_t rows, uint32_t vocab, const i
 template <class T>
 void launch_forward(const T* x, size_t stride, size_t rows, uint32_t vocab, const int* tokens, uint32_t top,
                     const Out& o, cudaStream_t st) {
+  if (vocab <= 128 && top == 0) {
+    const unsigned blocks = (unsigned)((rows + kThreads / 8 - 1) / (kThreads / 8));
+    if (vocab <= 64) forward_narrow<T, 8><<<blocks, kThreads, 0, st>>>(x, stride, rows, (int)vocab, tokens, o);
+    else forward_narrow<T, 16><<<blocks, kThreads, 0, st>>>(x, stride, rows, (int)vocab, tokens, o);
+    return;
+  }
   if (vocab <= 64) return launch_small<T, 2>(x, stride, rows, vocab, tokens, top, o, st);
   if (vocab <= 128) return launch_small<T, 4>(x, stride, rows, vocab, tokens, top, o, st);
   if (top) launch_wide<T, true>(x, stride, rows, vocab, tokens, top, o, st);
@@ -701,8 +760,14 @@ int mb_op_token_logprobs_backward(const mb_token_logprobs_backward_args* a, void
       const size_t rows = a->rows;
       const uint32_t vocab = a->vocab;
       if (vocab <= (uint32_t)kRowLanes) {
-        const unsigned blocks = (unsigned)((rows + kWarps - 1) / kWarps);
-        backward_rows<T, 32><<<blocks, kThreads, 0, st>>>(x, a->row_stride, rows, (int)vocab, in, d);
+        // 8 threads where they hold the row in their vectors in flight
+        if (vocab * sizeof(T) <= 8 * kUnroll * 16) {
+          const unsigned blocks = (unsigned)((rows + kThreads / 8 - 1) / (kThreads / 8));
+          backward_rows<T, 8><<<blocks, kThreads, 0, st>>>(x, a->row_stride, rows, (int)vocab, in, d);
+        } else {
+          const unsigned blocks = (unsigned)((rows + kWarps - 1) / kWarps);
+          backward_rows<T, 32><<<blocks, kThreads, 0, st>>>(x, a->row_stride, rows, (int)vocab, in, d);
+        }
       } else {
         backward_rows<T, kThreads><<<dim3((unsigned)rows, row_shares(rows, (int)vocab)), kThreads, 0, st>>>(
             x, a->row_stride, rows, (int)vocab, in, d);
