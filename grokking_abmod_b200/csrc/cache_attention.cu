@@ -547,8 +547,11 @@ struct TileShape {
   static_assert(kO + 2 * D <= 512, "tensor memory");
   static constexpr int kOperand = kKeys * D * 2;           // bytes of a K or V tile
   static constexpr int kQTile = kHalfRows * D * 2;         // bytes of a half's Q, a term
-  static constexpr int kQueries = kStages * 2 * kOperand;  // [half][term]
-  static constexpr int kMeta = kQueries + (kQInSmem ? 2 * TERMS * kQTile : 0);
+  // Q's FP16 tiles [half][term], also on their way into tensor memory; at the
+  // end the outputs' rows, which are as large
+  static constexpr int kQueries = kStages * 2 * kOperand;
+  static constexpr int kScales = kQueries + 2 * TERMS * kQTile;  // of Q's rows
+  static constexpr int kMeta = kScales + kTileRows * 4;
   static constexpr int kBars = kMeta + kStages * 32;
   static constexpr int kBytes = kBars + 192;
 };
@@ -565,6 +568,25 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint3
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add));
+}
+
+// The largest of three (NaN only of three NaN).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// FP16 parts of a probability pair: hi the value cut to 11 bits, which FP16
+// holds exactly, lo the rest.  (Below 2^-14 FP16 is coarser than that; the
+// pair then errs by 2^-25, 2^-36 of the row's largest probability.)
+__device__ __forceinline__ void cut_f16x2(float2 w, uint32_t& hi, uint32_t& lo) {
+  const float2 h = make_float2(__uint_as_float(__float_as_uint(w.x) & 0xFFFFE000u),
+                               __uint_as_float(__float_as_uint(w.y) & 0xFFFFE000u));
+  const float2 r = fma2(h, splat2(-1.0f), w);
+  const __half2 a = __floats2half2_rn(h.x, h.y), b = __floats2half2_rn(r.x, r.y);
+  hi = *reinterpret_cast<const uint32_t*>(&a);
+  lo = *reinterpret_cast<const uint32_t*>(&b);
 }
 
 // One lane of a converged warp.
@@ -644,75 +666,118 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   }
   tc::bar_init_fence();
   if (warp == 12) tc::tmem_alloc(tmem_at, 512);
-  tc::fence_before_sync();
-  __syncthreads();
-  tc::fence_after_sync();
-  const uint32_t tmem = __shfl_sync(kFull, *tmem_at, 0);
+  // Barriers and tensor memory are there.  Every role passes this once, after
+  // what it can do without them.
+  auto ready = [&]() -> uint32_t {
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    return __shfl_sync(kFull, *tmem_at, 0);
+  };
+  // Rows of Q and of the output move between global and shared memory with
+  // eight lanes on eight rows and four on a row's 16-byte chunks: whole sectors
+  // there, all banks here.  A thread that read or wrote its own row would touch
+  // 32 lines an instruction (12000 cycles for Q, 10000 for the output, of 65000
+  // a CTA took for 1024 tokens of 64 channels).
+  const int sub = lane & 7, quarter = lane >> 3;
+  // Row r of the unit is token token0 + n / group of the sequence's new rows and
+  // query head n % group of the key head, n = rest0 + r below 2048: exact in FP32.
+  const int token0 = u.row0 / q.group, rest0 = u.row0 - token0 * q.group;
+  const float per_group = 1.0f / (float)q.group;
+  auto token_at = [&](int r) { return token0 + (int)(((float)(rest0 + r) + 0.5f) * per_group); };
+  auto row_at = [&](int r) { return u.first_row + token_at(r); };
+  auto head_at = [&](int r) { return head * q.group + rest0 + r - (token_at(r) - token0) * q.group; };
 
   if (warp < 8) {
     const int h = warp >> 2;
     const int count = h ? (both ? count1 : 0) : (both ? count0 : count1);
     const int r = h * kHalfRows + (warp & 3) * 32 + lane;  // row of the unit
-    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t at_q = lanes + h * S::kQ, at_o = lanes + S::kO + h * D;
     const bool there = r < u.rows;
-    const int tok = (u.row0 + r) / q.group, a = head * q.group + (u.row0 + r) % q.group;
+    const int tok = token_at(r);
     const int limit = there ? old + tok : -1;
     // the last position that every row of the warp sees
-    const int sure = old + (u.row0 + (r - lane)) / q.group;
+    const int sure = old + token_at(r - lane);
     float factor = 0.f;
     float m = -INFINITY, l = 0.f;
     int ev = -126;
     bool alive = true;
+    uint8_t* tile = smem + S::kQueries + h * TERMS * S::kQTile;
+    float* scales = reinterpret_cast<float*>(smem + S::kScales);
     if (count > 0) {
-      const T* src = static_cast<const T*>(q.q) + (u.first_row + tok) * q.row_stride + (size_t)a * q.head_stride;
       // 16-byte loads where every row is aligned for them
       const bool vector = ((reinterpret_cast<uintptr_t>(q.q) | q.row_stride * sizeof(T) | q.head_stride * sizeof(T)) & 15) == 0 &&
                           q.head_dim % Element<T>::kVec == 0;
-      auto chunk = [&](int c0, float (&x)[32]) {  // channels [c0, c0 + 32)
-        if (vector) {
+      constexpr int AT_ONCE = D <= 64 ? 4 : 2;  // groups of eight rows whose loads go out together
+#pragma unroll 1
+      for (int rg = 0; rg < 4; rg += AT_ONCE) {
+        float x[AT_ONCE][D / 32][8];
 #pragma unroll
-          for (int i = 0; i < 32; i += Element<T>::kVec)
-            Element<T>::unpack(there && c0 + i < q.head_dim ? __ldg(reinterpret_cast<const uint4*>(src + c0 + i))
-                                                            : make_uint4(0u, 0u, 0u, 0u), x + i);
-        } else {
+        for (int k = 0; k < AT_ONCE; ++k) {
+          const int r8 = r - lane + 8 * (rg + k) + sub;
+          const T* src = static_cast<const T*>(q.q) + row_at(r8) * q.row_stride + (size_t)head_at(r8) * q.head_stride;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) x[i] = there && c0 + i < q.head_dim ? Element<T>::to(src[c0 + i]) : 0.f;
-        }
-      };
-      float most = 0.f;
+          for (int i = 0; i < D / 32; ++i) {
+            const int ch = (quarter + 4 * i) * 8;
+            if (vector) {
 #pragma unroll
-      for (int c0 = 0; c0 < D; c0 += 32) {
-        float x[32];
-        chunk(c0, x);
+              for (int e = 0; e < 8; e += Element<T>::kVec)
+                Element<T>::unpack(r8 < u.rows && ch + e < q.head_dim ? __ldg(reinterpret_cast<const uint4*>(src + ch + e))
+                                                                     : make_uint4(0u, 0u, 0u, 0u), x[k][i] + e);
+            } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) most = fmaxf(most, fabsf(x[i]));
-      }
-      const float up = tc::f16_scale(most);
-      factor = q.scale_log2 / up;
-      const float sign = factor < 0.f ? -up : up;  // scores are q.k times a factor that is not negative
-      factor = fabsf(factor);
-#pragma unroll
-      for (int c0 = 0; c0 < D; c0 += 32) {
-        float x[32];
-        chunk(c0, x);
-        uint32_t hi[16], lo[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) tc::split_f16x2(x[2 * i] * sign, x[2 * i + 1] * sign, hi[i], lo[i]);
-        __syncwarp();
-        if constexpr (S::kQInSmem) {
-          __half* at = reinterpret_cast<__half*>(smem + S::kQueries + h * TERMS * S::kQTile);
-#pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            const int e = tc::blk16(r & (kHalfRows - 1), c0 + 2 * i, D);
-            *reinterpret_cast<uint4*>(at + e) = make_uint4(hi[i], hi[i + 1], hi[i + 2], hi[i + 3]);
-            if constexpr (TERMS == 2)
-              *reinterpret_cast<uint4*>(at + S::kQTile / 2 + e) = make_uint4(lo[i], lo[i + 1], lo[i + 2], lo[i + 3]);
+              for (int e = 0; e < 8; ++e) x[k][i][e] = r8 < u.rows && ch + e < q.head_dim ? Element<T>::to(src[ch + e]) : 0.f;
+            }
           }
-        } else {
-          tc::tmem_st16u(at_q + c0 / 2, hi);
-          if constexpr (TERMS == 2) tc::tmem_st16u(at_q + D / 2 + c0 / 2, lo);
         }
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) {
+          const int r8 = r - lane + 8 * (rg + k) + sub;
+          float most = 0.f;
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[k][i][e]));
+          most = fmaxf(most, __shfl_xor_sync(kFull, most, 8));
+          most = fmaxf(most, __shfl_xor_sync(kFull, most, 16));
+          const float up = tc::f16_scale(most);
+          if (quarter == 0) scales[r8] = up;
+          // scores are q.k times a factor that is not negative
+          const float sign = q.scale_log2 < 0.f ? -up : up;
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) tc::split_f16x2(x[k][i][2 * e] * sign, x[k][i][2 * e + 1] * sign, hi[e], lo[e]);
+            uint8_t* at = tile + tc::blk16(r8 & (kHalfRows - 1), (quarter + 4 * i) * 8, D) * 2;
+            *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            if constexpr (TERMS == 2) *reinterpret_cast<uint4*>(at + S::kQTile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          }
+        }
+      }
+      __syncwarp();
+      factor = fabsf(q.scale_log2) / scales[r];
+    }
+    const uint32_t tmem = ready();
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t at_q = lanes + h * S::kQ, at_o = lanes + S::kO + h * D;
+    if (count > 0) {
+      if constexpr (!S::kQInSmem) {
+#pragma unroll
+        for (int term = 0; term < TERMS; ++term)
+#pragma unroll
+          for (int c0 = 0; c0 < D; c0 += 32) {
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint4 v = *reinterpret_cast<const uint4*>(
+                  tile + term * S::kQTile + tc::blk16(r & (kHalfRows - 1), c0 + 8 * i, D) * 2);
+              w[4 * i] = v.x;
+              w[4 * i + 1] = v.y;
+              w[4 * i + 2] = v.z;
+              w[4 * i + 3] = v.w;
+            }
+            tc::tmem_st16u(at_q + term * (D / 2) + c0 / 2, w);
+          }
       }
       tc::tmem_st_wait();
       tc::fence_async_smem();
@@ -753,13 +818,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          float a0 = x[16 * g], a1 = x[16 * g + 1];
-#pragma unroll
-          for (int i = 2; i < 16; i += 2) {
-            a0 = fmaxf(a0, x[16 * g + i]);
-            a1 = fmaxf(a1, x[16 * g + i + 1]);
-          }
-          mx = fmaxf(mx, fmaxf(a0, a1) * fk[2 * part32 + g]);
+          const float* y = x + 16 * g;
+          const float a0 = max3(max3(y[0], y[1], y[2]), y[3], y[4]), a1 = max3(max3(y[5], y[6], y[7]), y[8], y[9]);
+          const float a2 = max3(max3(y[10], y[11], y[12]), y[13], max3(a0, a1, y[14]));
+          mx = fmaxf(mx, fmaxf(a2, y[15]) * fk[2 * part32 + g]);
         }
       }
       int top = ev;
@@ -809,7 +871,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           sum = add2(sum, p);
           const float2 w = mul2(p, splat2(sv[g] * unit * kProbScale));
           if constexpr (TERMS == 2) {
-            tc::split_f16x2(w.x, w.y, hi[i], lo[i]);
+            cut_f16x2(w, hi[i], lo[i]);
           } else {
             const __half2 v = __floats2half2_rn(w.x, w.y);
             hi[i] = *reinterpret_cast<const uint32_t*>(&v);
@@ -831,6 +893,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     float lse = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) + log2f(l);
     if (!alive) lse = NAN;
     const size_t row = u.first_row + tok;
+    const int a = head_at(r);
     T* out = static_cast<T*>(q.out) + (row * q.heads + a) * q.head_dim;
     float* po = part.o + (slot * kTileRows + r) * D;
     const bool wide = q.head_dim % Element<T>::kVec == 0 && (reinterpret_cast<uintptr_t>(q.out) & 15) == 0;
@@ -838,27 +901,44 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if (part.chunks > 1) part.lse[slot * kTileRows + r] = lse;
       else if (q.lse) q.lse[(size_t)a * t.rows + row] = lse;
     }
+    // 16-byte chunk k of a row of outputs, where Q was (its products are done)
+    auto staged = [&](int r8, int k) {
+      return reinterpret_cast<uint4*>(tile + k / (D / 8) * S::kQTile +
+                                      tc::blk16(r8 & (kHalfRows - 1), k % (D / 8) * 8, D) * 2);
+    };
+    constexpr int VEC = Element<T>::kVec;
 #pragma unroll
     for (int c0 = 0; c0 < D; c0 += 16) {
       float o[16];
       if (count > 0) tc::tmem_ld16(at_o + c0, o);
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[i] = !alive ? NAN : l == 0.f ? 0.f : o[i] * inverse;
-      if (!there) {
-      } else if (part.chunks > 1) {
+      if (part.chunks > 1) {
+        if (there)
 #pragma unroll
-        for (int i = 0; i < 16; i += 4)
-          *reinterpret_cast<float4*>(po + c0 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<float4*>(po + c0 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
       } else if (wide) {
 #pragma unroll
-        for (int i = 0; i < 16; i += Element<T>::kVec)
-          if (c0 + i < q.head_dim) *reinterpret_cast<uint4*>(out + c0 + i) = Element<T>::pack(o + i);
-      } else {
+        for (int i = 0; i < 16; i += VEC) *staged(r, (c0 + i) / VEC) = Element<T>::pack(o + i);
+      } else if (there) {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (c0 + i < q.head_dim) out[c0 + i] = Element<T>::from(o[i]);
       }
       __syncwarp();  // tensor memory is read by whole warps
+    }
+    if (part.chunks == 1 && wide) {
+#pragma unroll
+      for (int rg = 0; rg < 4; ++rg) {
+        const int r8 = r - lane + 8 * rg + sub;
+        T* to = static_cast<T*>(q.out) + (row_at(r8) * q.heads + head_at(r8)) * q.head_dim;
+#pragma unroll
+        for (int i = 0; i < D / VEC / 4; ++i) {
+          const int k = quarter + 4 * i;
+          if (r8 < u.rows && k * VEC < q.head_dim) *reinterpret_cast<uint4*>(to + k * VEC) = *staged(r8, k);
+        }
+      }
     }
   } else if (warp < 12) {
     // 16 codes a piece; 8 lanes take one piece column of 8 rows, whose FP16
@@ -926,6 +1006,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       load(0);
       if (count1 > 1) find(1);
     }
+    ready();
     for (int j = 0; j < count1; ++j) {
       const int stage = j % kStages;
       if (j >= kStages && !tc::bar_wait(&kv_free[stage], (j / kStages - 1) & 1)) {
@@ -949,6 +1030,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     // uniform, which keeps the instructions between two products few (from a
     // single diverged lane a product took about 100 cycles to issue).  The
     // halves take turns.
+    const uint32_t tmem = ready();
     const bool elected = elect_one();
     const int counts[2] = {both ? count0 : count1, both ? count1 : 0};
     constexpr uint32_t kIdS = tc::idesc_f16(128, kKeys), kIdO = tc::idesc_f16(128, D, true);
@@ -1038,7 +1120,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   __syncthreads();
   if (warp == 12) {
     tc::fence_after_sync();
-    tc::tmem_dealloc(tmem, 512);
+    tc::tmem_dealloc(*tmem_at, 512);
   }
   if (threadIdx.x == 0 && *failed && q.status) atomicOr(q.status, kGaveUp);
 }
