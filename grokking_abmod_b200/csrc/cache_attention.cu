@@ -514,8 +514,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D, ROWS>::kResident)
 //                   where a maximum has grown
 //   warps 8-11      converters: the tile's codes from global memory (loaded a
 //                   tile ahead), as FP16 into shared memory, once for both halves
-//   warp 12         issues the products S = Q K^T and O += P V, the halves in
-//                   turn: one half's products run under the other's softmax
+//   warps 12, 13    issue the products S = Q K^T and O += P V of a half each
 //
 // Each half has two score buffers (P goes over S in place), so that the next
 // scores are there when a softmax ends and only softmax follows softmax in a
@@ -530,7 +529,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D, ROWS>::kResident)
 constexpr int kKeys = 64;
 constexpr int kHalfRows = 128;
 constexpr int kTileRows = 2 * kHalfRows;
-constexpr int kTileThreads = 13 * 32;
+constexpr int kTileThreads = 14 * 32;
 constexpr int kConverters = 128;
 constexpr int kStages = 3;
 constexpr float kLazy = 4.f;
@@ -568,6 +567,12 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint3
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add));
+}
+
+__device__ __forceinline__ void tmem_st8(uint32_t at, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(at), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 
 // The largest of three (NaN only of three NaN).
@@ -644,14 +649,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* p_full = s_full + 4;          // [half][buffer] softmax -> products: a half may be two tiles ahead
   uint64_t* q_full = p_full + 4;          // [half]
   uint64_t* o_full = q_full + 2;          // [half][tile & 1] O += P V is done
-  uint64_t* drained = o_full + 4;
-  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drained + 1);
+  uint64_t* drained = o_full + 4;         // [half]
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drained + 2);
   int* failed = reinterpret_cast<int*>(tmem_at + 1);
   float* meta = reinterpret_cast<float*>(smem + S::kMeta);  // [stage][4 K scales, 4 V scales] of 16 tokens each
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       tc::bar_init(&kv_full[s], kConverters);
-      tc::bar_init(&kv_free[s], 1);
+      tc::bar_init(&kv_free[s], both ? 2 : 1);
     }
     for (int h = 0; h < 2; ++h) {
       for (int k = 0; k < 2; ++k) {
@@ -660,8 +665,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         tc::bar_init(&p_full[2 * h + k], kHalfRows);
       }
       tc::bar_init(&q_full[h], kHalfRows);
+      tc::bar_init(&drained[h], 1);
     }
-    tc::bar_init(drained, 1);
     *failed = 0;
   }
   tc::bar_init_fence();
@@ -798,24 +803,31 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const float4 ks = *reinterpret_cast<const float4*>(meta + stage * 8);
       const float4 vs = *reinterpret_cast<const float4*>(meta + stage * 8 + 4);
       // not 0, so that a masked score stays -inf; NaN stays
-      float fk[4] = {ks.x * factor, ks.y * factor, ks.z * factor, ks.w * factor};
-#pragma unroll
-      for (int g = 0; g < 4; ++g) fk[g] = fk[g] < 2e-38f ? 2e-38f : fk[g];
+      auto positive = [](float f) { return f < 2e-38f ? 2e-38f : f; };
+      const float fk[4] = {positive(ks.x * factor), positive(ks.y * factor), positive(ks.z * factor),
+                           positive(ks.w * factor)};
       const float sv[4] = {vs.x, vs.y, vs.z, vs.w};
       const int pos = (begin + j) * kKeys;
-      const bool partial = pos < u.lo || pos + kKeys - 1 > sure;
-      // The scores are read twice, 32 columns at a time, once for their
-      // maximum and once for their exponentials: 64 at once spill.
+      if (pos < u.lo || pos + kKeys - 1 > sure) {
+        // masked scores become -inf in place; few tiles need it, so the code below does not carry it
+#pragma unroll 1
+        for (int c0 = 0; c0 < kKeys; c0 += 16) {
+          float x[16];
+          tc::tmem_ld16(at_s + c0, x);
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (pos + c0 + i < u.lo || pos + c0 + i > limit) x[i] = -INFINITY;
+          tc::tmem_st16(at_s + c0, x);
+        }
+        tc::tmem_st_wait();
+      }
+      // The scores are read twice, for their maximum and for their
+      // exponentials: 64 at once spill.
       float mx = m;
 #pragma unroll
       for (int part32 = 0; part32 < 2; ++part32) {
         float x[32];
         tc::tmem_ld32(at_s + 32 * part32, x);
-        if (partial) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (pos + 32 * part32 + i < u.lo || pos + 32 * part32 + i > limit) x[i] = -INFINITY;
-        }
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           const float* y = x + 16 * g;
@@ -839,7 +851,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           alive = __all_sync(kFull, o_done(j - 1));
           if (!alive) break;
           tc::fence_after_sync();
-#pragma unroll
+#pragma unroll 1
           for (int c0 = 0; c0 < D; c0 += 16) {
             float o[16];
             tc::tmem_ld16(at_o + c0, o);
@@ -853,33 +865,30 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const float2 nbase = splat2(-base);
       const float unit = power_of_two(-ev);
       float2 sum = make_float2(0.f, 0.f);
+      const float* page_scales = meta + stage * 8;
 #pragma unroll
-      for (int part32 = 0; part32 < 2; ++part32) {
-        float x[32];
-        tc::tmem_ld32(at_s + 32 * part32, x);
-        if (partial) {
+      for (int g = 0; g < 4; ++g) {  // 16 tokens, at most one page
+        const float2 f = splat2(positive(page_scales[g] * factor));
+        const float2 v = splat2(page_scales[4 + g] * unit * kProbScale);
+        float x[16];
+        tc::tmem_ld16(at_s + 16 * g, x);
+        uint32_t hi[8], lo[8];
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (pos + 32 * part32 + i < u.lo || pos + 32 * part32 + i > limit) x[i] = -INFINITY;
-        }
-        uint32_t hi[16], lo[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int g = 2 * part32 + i / 8;
-          const float2 y = fma2(make_float2(x[2 * i], x[2 * i + 1]), splat2(fk[g]), nbase);
+        for (int i = 0; i < 8; ++i) {
+          const float2 y = fma2(make_float2(x[2 * i], x[2 * i + 1]), f, nbase);
           const float2 p = make_float2(ex2_ftz(y.x), ex2_ftz(y.y));
           sum = add2(sum, p);
-          const float2 w = mul2(p, splat2(sv[g] * unit * kProbScale));
+          const float2 w = mul2(p, v);
           if constexpr (TERMS == 2) {
             cut_f16x2(w, hi[i], lo[i]);
           } else {
-            const __half2 v = __floats2half2_rn(w.x, w.y);
-            hi[i] = *reinterpret_cast<const uint32_t*>(&v);
+            const __half2 h2 = __floats2half2_rn(w.x, w.y);
+            hi[i] = *reinterpret_cast<const uint32_t*>(&h2);
           }
         }
-        // P of 32 tokens over their own scores' columns: hi in the first 16, lo behind
-        tc::tmem_st16u(at_s + 32 * part32, hi);
-        if constexpr (TERMS == 2) tc::tmem_st16u(at_s + 32 * part32 + 16, lo);
+        // P over its own scores' columns: hi in the first 8, lo behind
+        tmem_st8(at_s + 16 * g, hi);
+        if constexpr (TERMS == 2) tmem_st8(at_s + 16 * g + 8, lo);
       }
       l += sum.x + sum.y;
       tc::tmem_st_wait();
@@ -1026,94 +1035,85 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if (j + 2 < count1) find(j + 2);
     }
   } else {
-    // The whole warp waits, one lane issues: everything it works with is
-    // uniform, which keeps the instructions between two products few (from a
-    // single diverged lane a product took about 100 cycles to issue).  The
-    // halves take turns.
+    // The issuer of a half.  The whole warp waits, one lane issues: everything
+    // it works with is uniform, which keeps the instructions between two
+    // products few (from a single diverged lane a product took about 100
+    // cycles to issue).
+    const int h = warp - 12;
     const uint32_t tmem = ready();
     const bool elected = elect_one();
-    const int counts[2] = {both ? count0 : count1, both ? count1 : 0};
+    const int count = h ? (both ? count1 : 0) : (both ? count0 : count1);
     constexpr uint32_t kIdS = tc::idesc_f16(128, kKeys), kIdO = tc::idesc_f16(128, D, true);
     const uint64_t k0 = tc::desc_kmajor16(smem, D, 0), v0 = tc::desc_mn16(smem + S::kOperand, D, 0);
-    const uint64_t q0 = tc::desc_kmajor16(smem + S::kQueries, D, 0);
+    const uint64_t q0 = tc::desc_kmajor16(smem + S::kQueries + h * TERMS * S::kQTile, D, 0);
     constexpr uint64_t kStep = 256 >> 4, vStep = D / 8 * 256 >> 4, kStage = 2 * S::kOperand >> 4;
-    auto scores = [&](int h, int j) {
+    const uint32_t at_q = tmem + h * S::kQ, at_s = tmem + S::kS + 2 * h * kKeys, at_o = tmem + S::kO + h * D;
+    auto scores = [&](int j) {
       const uint64_t k = k0 + (j % kStages) * kStage;
-      const uint32_t to = tmem + S::kS + (2 * h + (j & 1)) * kKeys;
+      const uint32_t to = at_s + (j & 1) * kKeys;
 #pragma unroll
       for (int term = 0; term < TERMS; ++term) {
 #pragma unroll
         for (int s = 0; s < D / 16; ++s) {
           const bool add = term > 0 || s > 0;
-          if constexpr (S::kQInSmem)
-            mma_ss(to, q0 + (h * TERMS + term) * (S::kQTile >> 4) + s * kStep, k + s * kStep, kIdS, add);
-          else
-            mma_ts(to, tmem + h * S::kQ + term * (D / 2) + 8 * s, k + s * kStep, kIdS, add);
+          if constexpr (S::kQInSmem) mma_ss(to, q0 + term * (S::kQTile >> 4) + s * kStep, k + s * kStep, kIdS, add);
+          else mma_ts(to, at_q + term * (D / 2) + 8 * s, k + s * kStep, kIdS, add);
         }
       }
     };
-    auto values = [&](int h, int j) {
+    auto values = [&](int j) {
       const uint64_t v = v0 + (j % kStages) * kStage;
-      const uint32_t to = tmem + S::kO + h * D, p_at = tmem + S::kS + (2 * h + (j & 1)) * kKeys;
 #pragma unroll
       for (int s = 0; s < kKeys / 16; ++s) {
-        const uint32_t p_s = p_at + s / 2 * 32 + s % 2 * 8;  // 16 tokens
-        mma_ts(to, p_s, v + s * vStep, kIdO, j > 0 || s > 0);
-        if constexpr (TERMS == 2) mma_ts(to, p_s + 16, v + s * vStep, kIdO, true);
+        const uint32_t p = at_s + (j & 1) * kKeys + 16 * s;  // 16 tokens
+        mma_ts(at_o, p, v + s * vStep, kIdO, j > 0 || s > 0);
+        if constexpr (TERMS == 2) mma_ts(at_o, p + 8, v + s * vStep, kIdO, true);
       }
     };
     auto full = [&](int j) { return tc::bar_wait(&kv_full[j % kStages], (j / kStages) & 1); };
     bool ok = true;
+    if (count > 0) ok = __all_sync(kFull, tc::bar_wait(&q_full[h], 0));
     // the first two tiles' scores
-    for (int j = 0; j < 2 && j < count1 && ok; ++j) {
+    for (int j = 0; j < 2 && j < count && ok; ++j) {
       ok = __all_sync(kFull, full(j));
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (j >= counts[h] || !ok) continue;
-        if (j == 0) ok = __all_sync(kFull, tc::bar_wait(&q_full[h], 0));
-        tc::fence_after_sync();
-        if (ok && elected) {
-          scores(h, j);
-          tc::commit(&s_full[2 * h + j]);
-        }
-        __syncwarp();
-      }
-    }
-    // Scores of tile i go over the probabilities of tile i - 2: not before the
-    // products that read them are done (only products of one accumulator and
-    // shape are ordered among themselves).
-    auto next_scores = [&](int h, int i) {
-      if (i < 2 || i >= counts[h] || !ok) return;
-      ok = __all_sync(kFull, full(i) && tc::bar_wait(&o_full[2 * h + (i & 1)], ((i - 2) >> 1) & 1));
       tc::fence_after_sync();
       if (ok && elected) {
-        scores(h, i);
-        tc::commit(&s_full[2 * h + (i & 1)]);
+        scores(j);
+        tc::commit(&s_full[2 * h + j]);
       }
       __syncwarp();
-    };
-    for (int j = 0; j < count1 && ok; ++j) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (j < counts[h] && ok) {
-          ok = __all_sync(kFull, tc::bar_wait(&p_full[2 * h + (j & 1)], (j >> 1) & 1));
-          tc::fence_after_sync();
-          if (ok && elected) {
-            values(h, j);
-            tc::commit(&o_full[2 * h + (j & 1)]);
-            if (h == (both ? 1 : 0)) tc::commit(&kv_free[j % kStages]);
-          }
-          __syncwarp();
-        }
-        // the other half's scores: its last products were issued before these
-        if (h == 0) next_scores(1, j + 1);
-        else next_scores(0, j + 2);
+    }
+    for (int j = 0; j < count && ok; ++j) {
+      ok = __all_sync(kFull, tc::bar_wait(&p_full[2 * h + (j & 1)], (j >> 1) & 1));
+      tc::fence_after_sync();
+      if (ok && elected) {
+        values(j);
+        tc::commit(&o_full[2 * h + (j & 1)]);
+        tc::commit(&kv_free[j % kStages]);
       }
+      __syncwarp();
+      if (j + 2 >= count || !ok) continue;
+      // Scores of tile j + 2 go over the probabilities of tile j: not before
+      // the products that read them are done (only products of one
+      // accumulator and shape are ordered among themselves).
+      ok = __all_sync(kFull, full(j + 2) && tc::bar_wait(&o_full[2 * h + (j & 1)], (j >> 1) & 1));
+      tc::fence_after_sync();
+      if (ok && elected) {
+        scores(j + 2);
+        tc::commit(&s_full[2 * h + (j & 1)]);
+      }
+      __syncwarp();
+    }
+    // the tiles that only the other half sees: released once they are full, so
+    // that no phase counts this half twice
+    for (int j = count; both && j < count1 && ok; ++j) {
+      ok = __all_sync(kFull, full(j));
+      if (ok && elected) tc::bar_arrive(&kv_free[j % kStages]);
     }
     if (!ok) *failed = 1;
     // nothing is in flight when tensor memory is given back
-    if (elected) tc::commit(drained);
-    if (!tc::bar_wait(drained, 0)) *failed = 1;
+    if (elected) tc::commit(&drained[h]);
+    if (!tc::bar_wait(&drained[h], 0)) *failed = 1;
   }
   __syncwarp();
   tc::fence_before_sync();
