@@ -575,6 +575,24 @@ __device__ __forceinline__ void tmem_st8(uint32_t at, const uint32_t (&v)[8]) {
                : "memory");
 }
 
+// Sixteen columns of this thread's lane, asynchronously: the registers may be
+// read after tmem_wait, which takes them so that no use moves before it.
+__device__ __forceinline__ void tmem_ld16_async(uint32_t at, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(at)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait(uint32_t (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                 "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+               :
+               : "memory");
+}
+
 // The largest of three (NaN only of three NaN).
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -823,18 +841,21 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       // The scores are read twice, for their maximum and for their
       // exponentials: 64 at once spill.
+      // Sixteen columns at a time, the next ones on their way under the
+      // current ones' arithmetic: a load's latency is as long as that.
+      uint32_t column[2][16];
       float mx = m;
+      tmem_ld16_async(at_s, column[0]);
 #pragma unroll
-      for (int part32 = 0; part32 < 2; ++part32) {
-        float x[32];
-        tc::tmem_ld32(at_s + 32 * part32, x);
+      for (int g = 0; g < 4; ++g) {
+        tmem_wait(column[g & 1]);
+        if (g < 3) tmem_ld16_async(at_s + 16 * (g + 1), column[(g + 1) & 1]);
+        float y[16];
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const float* y = x + 16 * g;
-          const float a0 = max3(max3(y[0], y[1], y[2]), y[3], y[4]), a1 = max3(max3(y[5], y[6], y[7]), y[8], y[9]);
-          const float a2 = max3(max3(y[10], y[11], y[12]), y[13], max3(a0, a1, y[14]));
-          mx = fmaxf(mx, fmaxf(a2, y[15]) * fk[2 * part32 + g]);
-        }
+        for (int i = 0; i < 16; ++i) y[i] = __uint_as_float(column[g & 1][i]);
+        const float a0 = max3(max3(y[0], y[1], y[2]), y[3], y[4]), a1 = max3(max3(y[5], y[6], y[7]), y[8], y[9]);
+        const float a2 = max3(max3(y[10], y[11], y[12]), y[13], max3(a0, a1, y[14]));
+        mx = fmaxf(mx, fmaxf(a2, y[15]) * fk[g]);
       }
       int top = ev;
 #pragma unroll
@@ -866,16 +887,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const float unit = power_of_two(-ev);
       float2 sum = make_float2(0.f, 0.f);
       const float* page_scales = meta + stage * 8;
+      tmem_ld16_async(at_s, column[0]);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {  // 16 tokens, at most one page
         const float2 f = splat2(positive(page_scales[g] * factor));
         const float2 v = splat2(page_scales[4 + g] * unit * kProbScale);
-        float x[16];
-        tc::tmem_ld16(at_s + 16 * g, x);
+        tmem_wait(column[g & 1]);
+        if (g < 3) tmem_ld16_async(at_s + 16 * (g + 1), column[(g + 1) & 1]);
         uint32_t hi[8], lo[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float2 y = fma2(make_float2(x[2 * i], x[2 * i + 1]), f, nbase);
+          const float2 x = make_float2(__uint_as_float(column[g & 1][2 * i]), __uint_as_float(column[g & 1][2 * i + 1]));
+          const float2 y = fma2(x, f, nbase);
           const float2 p = make_float2(ex2_ftz(y.x), ex2_ftz(y.y));
           sum = add2(sum, p);
           const float2 w = mul2(p, v);
