@@ -523,6 +523,13 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D, ROWS>::kResident)
 // (two products), those of 16-bit rows one FP16 (bfloat16's 8 bits fit; a
 // probability's rounding to 11 bits is below the output's own).
 //
+// The tensor core cuts its accumulator's sums instead of rounding them, and the
+// loss grows with the number of products added to O (1024 tokens of FP32 rows:
+// 1.1e-6 of the result; rounded sums 0.4e-6).  Of FP32 rows up to 64 wide O is
+// therefore added to a sum in shared memory, rounded, every 4 tiles and begun
+// again; wider ones, for whose sums there is no room, are cut into chunks of 8
+// tiles that are joined in FP32.
+//
 // O follows a row's maximum lazily: probabilities up to 2^4 are let through,
 // so that after the first tiles O is hardly ever touched; they carry 2^11,
 // 2^15 in all, inside FP16's range.
@@ -534,6 +541,9 @@ constexpr int kConverters = 128;
 constexpr int kStages = 3;
 constexpr float kLazy = 4.f;
 constexpr float kProbScale = 2048.f;
+constexpr int kSumTiles = 4;     // FP32 rows: tiles whose products O holds at most
+constexpr int kSumChunk = 8;     // the same where chunks bound them
+constexpr int kSumWidth = 64;    // widest rows with sums in shared memory
 
 template <int D, int TERMS>
 struct TileShape {
@@ -600,14 +610,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// FP16 parts of a probability pair: hi the value cut to 11 bits, which FP16
-// holds exactly, lo the rest.  (Below 2^-14 FP16 is coarser than that; the
-// pair then errs by 2^-25, 2^-36 of the row's largest probability.)
-__device__ __forceinline__ void cut_f16x2(float2 w, uint32_t& hi, uint32_t& lo) {
-  const float2 h = make_float2(__uint_as_float(__float_as_uint(w.x) & 0xFFFFE000u),
-                               __uint_as_float(__float_as_uint(w.y) & 0xFFFFE000u));
-  const float2 r = fma2(h, splat2(-1.0f), w);
-  const __half2 a = __floats2half2_rn(h.x, h.y), b = __floats2half2_rn(r.x, r.y);
+// FP16 hi and lo parts of a pair.
+__device__ __forceinline__ void pair_f16x2(float2 w, uint32_t& hi, uint32_t& lo) {
+  const __half2 a = __floats2half2_rn(w.x, w.y);
+  const float2 r = fma2(__half22float2(a), splat2(-1.0f), w);
+  const __half2 b = __floats2half2_rn(r.x, r.y);
   hi = *reinterpret_cast<const uint32_t*>(&a);
   lo = *reinterpret_cast<const uint32_t*>(&b);
 }
@@ -624,6 +631,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     attend_tiles(View c, Batch t, Queries q, Partials part, int blocks_per_seq) {
   constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
   using S = TileShape<D, TERMS>;
+  constexpr bool SUMS = TERMS == 2 && D <= kSumWidth;
   extern __shared__ __align__(128) uint8_t smem[];
   // the shuffle makes the warp's number, and what follows from it, uniform
   const int warp = __shfl_sync(kFull, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -807,6 +815,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       tc::fence_before_sync();
       tc::bar_arrive(&q_full[h]);
     }
+    // 16-byte chunk k of a row of outputs, or of its sums, where Q was (it has
+    // gone to tensor memory, or its products are done)
+    auto staged = [&](int r8, int k) {
+      return reinterpret_cast<uint4*>(tile + k / (D / 8) * S::kQTile +
+                                      tc::blk16(r8 & (kHalfRows - 1), k % (D / 8) * 8, D) * 2);
+    };
     // The products of tile j.  A waiter may be a tile behind them or ahead, so
     // each parity of tiles has a barrier: a wait is exact within one phase only.
     auto o_done = [&](int j) { return tc::bar_wait(&o_full[2 * h + (j & 1)], (j >> 1) & 1); };
@@ -880,6 +894,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             for (int i = 0; i < 16; ++i) o[i] *= change;
             tc::tmem_st16(at_o + c0, o);
           }
+          if (SUMS && j > kSumTiles) {
+#pragma unroll 1
+            for (int k = 0; k < D / 4; ++k) {
+              float4* sum = reinterpret_cast<float4*>(staged(r, k));
+              const float4 v = *sum;
+              *sum = make_float4(v.x * change, v.y * change, v.z * change, v.w * change);
+            }
+          }
         }
       }
       const float base = m == -INFINITY ? 0.f : m;
@@ -903,7 +925,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           sum = add2(sum, p);
           const float2 w = mul2(p, v);
           if constexpr (TERMS == 2) {
-            cut_f16x2(w, hi[i], lo[i]);
+            pair_f16x2(w, hi[i], lo[i]);
           } else {
             const __half2 h2 = __floats2half2_rn(w.x, w.y);
             hi[i] = *reinterpret_cast<const uint32_t*>(&h2);
@@ -914,6 +936,26 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if constexpr (TERMS == 2) tmem_st8(at_s + 16 * g + 8, lo);
       }
       l += sum.x + sum.y;
+      if (SUMS && j > 0 && j % kSumTiles == 0) {
+        alive = __all_sync(kFull, o_done(j - 1));  // by now they are
+        if (!alive) break;
+        tc::fence_after_sync();
+#pragma unroll 1
+        for (int c0 = 0; c0 < D; c0 += 16) {
+          float o[16];
+          tc::tmem_ld16(at_o + c0, o);
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            float4* sum = reinterpret_cast<float4*>(staged(r, (c0 + i) / 4));
+            float4 v = j == kSumTiles ? make_float4(0.f, 0.f, 0.f, 0.f) : *sum;
+            v.x += o[i];
+            v.y += o[i + 1];
+            v.z += o[i + 2];
+            v.w += o[i + 3];
+            *sum = v;
+          }
+        }
+      }
       tc::tmem_st_wait();
       tc::fence_before_sync();
       tc::bar_arrive(&p_full[2 * h + (j & 1)]);
@@ -933,16 +975,21 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if (part.chunks > 1) part.lse[slot * kTileRows + r] = lse;
       else if (q.lse) q.lse[(size_t)a * t.rows + row] = lse;
     }
-    // 16-byte chunk k of a row of outputs, where Q was (its products are done)
-    auto staged = [&](int r8, int k) {
-      return reinterpret_cast<uint4*>(tile + k / (D / 8) * S::kQTile +
-                                      tc::blk16(r8 & (kHalfRows - 1), k % (D / 8) * 8, D) * 2);
-    };
     constexpr int VEC = Element<T>::kVec;
 #pragma unroll
     for (int c0 = 0; c0 < D; c0 += 16) {
       float o[16];
       if (count > 0) tc::tmem_ld16(at_o + c0, o);
+      if (SUMS && count > kSumTiles) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(staged(r, (c0 + i) / 4));
+          o[i] += v.x;
+          o[i + 1] += v.y;
+          o[i + 2] += v.z;
+          o[i + 3] += v.w;
+        }
+      }
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[i] = !alive ? NAN : l == 0.f ? 0.f : o[i] * inverse;
       if (part.chunks > 1) {
@@ -1089,7 +1136,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
       for (int s = 0; s < kKeys / 16; ++s) {
         const uint32_t p = at_s + (j & 1) * kKeys + 16 * s;  // 16 tokens
-        mma_ts(at_o, p, v + s * vStep, kIdO, j > 0 || s > 0);
+        mma_ts(at_o, p, v + s * vStep, kIdO, (SUMS ? j % kSumTiles : j) > 0 || s > 0);
         if constexpr (TERMS == 2) mma_ts(at_o, p + 8, v + s * vStep, kIdO, true);
       }
     };
@@ -1243,6 +1290,8 @@ inline Plan make_plan(size_t batch, size_t rows, uint32_t kv_heads, uint32_t gro
   size_t chunks = std::max<size_t>(1, std::min((tiles + 7) / 8, slots / have));
   for (int waves = 2; waves <= 4; ++waves)
     if (tiles * have >= slots * waves * 128) chunks = std::max(chunks, slots * waves / have);
+  if (use_tiles && dtype == MB_F32 && width > (uint32_t)kSumWidth)
+    chunks = std::max(chunks, (tiles + kSumChunk - 1) / kSumChunk);
   p.chunk_tiles = (int)((tiles + chunks - 1) / chunks + kSplitWarps - 1) / kSplitWarps * kSplitWarps;
   p.chunks = (int)((tiles + p.chunk_tiles - 1) / p.chunk_tiles);
   p.workspace = p.chunks > 1 ? p.units * kv_heads * p.chunks * unit_rows * (width + 1) * sizeof(float) : 0;
