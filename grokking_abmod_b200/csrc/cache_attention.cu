@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D, ROWS>::kResident)
 // The tensor core cuts its accumulator's sums instead of rounding them, and the
 // loss grows with the number of products added to O (1024 tokens of FP32 rows:
 // 1.1e-6 of the result; rounded sums 0.4e-6).  Of FP32 rows up to 64 wide O is
-// therefore added to a sum in shared memory, rounded, every 4 tiles and begun
+// therefore added to a sum in shared memory, rounded, every 6 tiles and begun
 // again; wider ones, for whose sums there is no room, are cut into chunks of 8
 // tiles that are joined in FP32.
 //
@@ -541,7 +541,7 @@ constexpr int kConverters = 128;
 constexpr int kStages = 3;
 constexpr float kLazy = 4.f;
 constexpr float kProbScale = 2048.f;
-constexpr int kSumTiles = 4;     // FP32 rows: tiles whose products O holds at most
+constexpr int kSumTiles = 6;     // FP32 rows: tiles whose products O holds at most
 constexpr int kSumChunk = 8;     // the same where chunks bound them
 constexpr int kSumWidth = 64;    // widest rows with sums in shared memory
 
@@ -875,7 +875,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
         if (sv[g] == sv[g]) top = max(top, exponent_of(sv[g]));
-      if (__any_sync(kFull, mx > m + kLazy || top != ev)) {
+      const bool close = SUMS && j > 0 && j % kSumTiles == 0;  // O joins the sums
+      if (__any_sync(kFull, close || mx > m + kLazy || top != ev)) {
         const float shrink = ex2_ftz(m - (mx == -INFINITY ? 0.f : mx));
         l *= shrink;
         const float change = shrink * (top != ev ? power_of_two(max(ev - top, -126)) : 1.f);
@@ -886,20 +887,24 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           alive = __all_sync(kFull, o_done(j - 1));
           if (!alive) break;
           tc::fence_after_sync();
+          const bool summed = SUMS && j > kSumTiles;  // there are sums already
 #pragma unroll 1
           for (int c0 = 0; c0 < D; c0 += 16) {
             float o[16];
             tc::tmem_ld16(at_o + c0, o);
+            if (SUMS && (close || summed)) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] *= change;
-            tc::tmem_st16(at_o + c0, o);
-          }
-          if (SUMS && j > kSumTiles) {
-#pragma unroll 1
-            for (int k = 0; k < D / 4; ++k) {
-              float4* sum = reinterpret_cast<float4*>(staged(r, k));
-              const float4 v = *sum;
-              *sum = make_float4(v.x * change, v.y * change, v.z * change, v.w * change);
+              for (int i = 0; i < 16; i += 4) {
+                float4* sum = reinterpret_cast<float4*>(staged(r, (c0 + i) / 4));
+                float4 v = summed ? *sum : make_float4(0.f, 0.f, 0.f, 0.f);
+                if (close) v = make_float4(v.x + o[i], v.y + o[i + 1], v.z + o[i + 2], v.w + o[i + 3]);
+                *sum = make_float4(v.x * change, v.y * change, v.z * change, v.w * change);
+              }
+            }
+            if (!close) {  // else this tile's products begin O again
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] *= change;
+              tc::tmem_st16(at_o + c0, o);
             }
           }
         }
@@ -936,26 +941,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if constexpr (TERMS == 2) tmem_st8(at_s + 16 * g + 8, lo);
       }
       l += sum.x + sum.y;
-      if (SUMS && j > 0 && j % kSumTiles == 0) {
-        alive = __all_sync(kFull, o_done(j - 1));  // by now they are
-        if (!alive) break;
-        tc::fence_after_sync();
-#pragma unroll 1
-        for (int c0 = 0; c0 < D; c0 += 16) {
-          float o[16];
-          tc::tmem_ld16(at_o + c0, o);
-#pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            float4* sum = reinterpret_cast<float4*>(staged(r, (c0 + i) / 4));
-            float4 v = j == kSumTiles ? make_float4(0.f, 0.f, 0.f, 0.f) : *sum;
-            v.x += o[i];
-            v.y += o[i + 1];
-            v.z += o[i + 2];
-            v.w += o[i + 3];
-            *sum = v;
-          }
-        }
-      }
       tc::tmem_st_wait();
       tc::fence_before_sync();
       tc::bar_arrive(&p_full[2 * h + (j & 1)]);

@@ -498,3 +498,49 @@ def test_refusals():
     assert out.shape == (0, 4, 64) and lse.shape == (4, 0)
     ops.cache_write(cache, none[:, :2], none[:, :2], table, lengths, _i32([0, 0, 0]))
     assert ops.cache_read(cache, table, lengths, 0)[0].shape == (2, 0, 2, 64)
+
+
+def test_launches_back_to_back_agree():
+    """Prompts whose halves and blocks end on different tiles, many launches in
+    a row without waiting: every one the same bits, no wait that gave up."""
+    torch = _torch()
+    rng = np.random.default_rng(11)
+    cases = []
+    for hd, dtype in ((64, "float32"), (128, "bfloat16"), (96, "float16"), (128, "float32")):
+        news = [300 + 37 * i for i in range(9)]
+        lengths = [n + 129 * i for i, n in enumerate(news)]
+        cache, _, table = _filled(rng, lengths, 2, hd, 32)
+        _, q = _rows(rng, (sum(news), 4, hd), dtype)
+        cases.append((q, cache, _i32(table), _i32(lengths), _i32(_offsets(news)), max(news), max(lengths)))
+    status = ops.new_status()
+    first, begin = None, torch.cuda.Event(enable_timing=True)
+    end = torch.cuda.Event(enable_timing=True)
+    for turn in range(60):
+        if turn == 1:
+            begin.record()
+        outs = [ops.cache_attention(q, c, t, n, o, max_new=m, max_tokens=most, status=status)
+                for q, c, t, n, o, m, most in cases]
+        if first is None:
+            first = outs
+    end.record()
+    ops.check_status(status)
+    for a, b in zip(first, outs):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    assert begin.elapsed_time(end) < 59 * 4 * 50  # a wait that runs out takes about a second
+
+
+def test_long_prompts_keep_single_precision():
+    """Errors of sums over many tiles do not grow with the length: against
+    float64 the output stays within twice the error of FP32 arithmetic with
+    rounded sums, 2^-24 sqrt(length) of it, and the scores' own 2^-21 S."""
+    rng = np.random.default_rng(12)
+    for hd, length in ((64, 4096), (128, 3000)):
+        cache, values, table = _filled(rng, [length], 1, hd, 64)
+        q64, q = _rows(rng, (130, 1, hd), "float32")
+        out, _ = ops.cache_attention(q, cache, _i32(table), _i32([length]), _i32([0, 130]), max_new=130)
+        want, _, s = _attend(q64, values, table, [length], [130], [0], 64, hd ** -0.5)
+        got = out.double().cpu().numpy()
+        rel = np.linalg.norm(got - want) / np.linalg.norm(want)
+        # outputs are averages of many values: smaller than them by the effective number of tokens
+        shrink = np.sqrt((values[1] ** 2).mean()) / np.sqrt((want ** 2).mean())
+        assert rel <= 2 * (2.0 ** -24 * np.sqrt(length) + 2.0 ** -21) * max(1.0, shrink)
