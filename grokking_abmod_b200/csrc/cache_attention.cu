@@ -915,12 +915,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       float2 sum = make_float2(0.f, 0.f);
       const float* page_scales = meta + stage * 8;
       tmem_ld16_async(at_s, column[0]);
+      tmem_wait(column[0]);
+      tmem_ld16_async(at_s + 16, column[1]);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {  // 16 tokens, at most one page
         const float2 f = splat2(positive(page_scales[g] * factor));
         const float2 v = splat2(page_scales[4 + g] * unit * kProbScale);
-        tmem_wait(column[g & 1]);
-        if (g < 3) tmem_ld16_async(at_s + 16 * (g + 1), column[(g + 1) & 1]);
         uint32_t hi[8], lo[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -936,6 +936,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             hi[i] = *reinterpret_cast<const uint32_t*>(&h2);
           }
         }
+        // the next columns before the store, so that their arithmetic does not
+        // wait for the end of these
+        if (g < 3) tmem_wait(column[(g + 1) & 1]);
+        if (g < 2) tmem_ld16_async(at_s + 16 * (g + 2), column[g & 1]);
         // P over its own scores' columns: hi in the first 8, lo behind
         tmem_st8(at_s + 16 * g, hi);
         if constexpr (TERMS == 2) tmem_st8(at_s + 16 * g + 8, lo);

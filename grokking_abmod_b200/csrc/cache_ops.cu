@@ -70,7 +70,7 @@ __device__ __forceinline__ void store_codes(int8_t* at, uint4 raw, float inverse
 // the reduction and the store; the two tensors' loads go out together, since
 // what a group waits for is mostly the chain length -> page -> rows.
 template <class T, int G, int HELD>
-__global__ void __launch_bounds__(G == 32 ? 128 : G)
+__global__ void __launch_bounds__(G == 32 ? 128 : G, G == 256 && HELD == 4 ? 4 : 1)
     write_pages(View c, Batch t, Rows<T> k, Rows<T> v, int head_dim, int page_slots, unsigned units, int* status) {
   constexpr int VEC = Element<T>::kVec, GROUPS = G == 32 ? 4 : 1;
   const int id = threadIdx.x % G;

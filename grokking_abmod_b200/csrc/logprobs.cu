@@ -409,6 +409,7 @@ __global__ void __launch_bounds__(kThreads)
   const int left_at = id < head ? id : tail + id - head;
 
   Stats st = empty_stats();
+  int best_at = begin + id;  // the step that raised the maximum last: the first with it
   for (int j = begin + id; j < end; j += GROUP * kUnroll) {
     uint4 raw[kUnroll];
 #pragma unroll
@@ -420,6 +421,7 @@ __global__ void __launch_bounds__(kThreads)
       for (int u = 1; u < kUnroll; ++u) mx = fmaxf(mx, vector_max<T>(raw[u]));
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) Element<T>::unpack(raw[u], v + u * VEC);
+      if (TOP && mx > st.m) best_at = j;
       accumulate(st, v, mx);
     } else {
 #pragma unroll
@@ -427,6 +429,7 @@ __global__ void __launch_bounds__(kThreads)
         if (j + u * GROUP < end) {
           float v[VEC];
           Element<T>::unpack(raw[u], v);
+          if (TOP && vector_max<T>(raw[u]) > st.m) best_at = j;
           accumulate(st, v, vector_max<T>(raw[u]));
         }
     }
@@ -472,7 +475,10 @@ __global__ void __launch_bounds__(kThreads)
           if (at < kFound) found[group][at] = top_key(v, (uint32_t)index);
         }
       };
-      for (int j = begin + id; j < end; j += GROUP * kAgain) {
+      // of one top token the step that holds the thread's first largest element is enough
+      static_assert(kAgain == kUnroll, "steps");
+      const int last = top == 1 ? min(end, best_at + GROUP * kAgain) : end;
+      for (int j = top == 1 ? best_at : begin + id; j < last; j += GROUP * kAgain) {
         uint4 raw[kAgain];
 #pragma unroll
         for (int u = 0; u < kAgain; ++u)
@@ -636,7 +642,9 @@ __global__ void __launch_bounds__(kThreads)
         }
     }
     // fewer than 2 VEC elements left over
-    for (int i = id; part == 0 && i < head + vocab - tail; i += G) {
+#pragma unroll
+    for (int i = id; i < 2 * VEC; i += G) {
+      if (part != 0 || i >= head + vocab - tail) break;
       const int at = i < head ? i : tail + i - head;
       d[at] = Element<T>::from(element_grad(r, Element<T>::to(x[at]), at));
     }
