@@ -61,6 +61,7 @@ struct Partials {
   float* o;
   int chunks;       // per unit
   int chunk_tiles;  // tiles of a chunk; the last one takes what is left
+  float4* sums;     // [unit][chunk][half][width / 4][row of the half], of wide FP32 rows in tiles
 };
 
 template <int D, int ROWS>
@@ -525,10 +526,12 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D, ROWS>::kResident)
 //
 // The tensor core cuts its accumulator's sums instead of rounding them, and the
 // loss grows with the number of products added to O (1024 tokens of FP32 rows:
-// 1.1e-6 of the result; rounded sums 0.4e-6).  Of FP32 rows up to 64 wide O is
-// therefore added to a sum in shared memory, rounded, every 6 tiles and begun
-// again; wider ones, for whose sums there is no room, are cut into chunks of 8
-// tiles that are joined in FP32.
+// 1.1e-6 of the result, 4096: 3.4e-6; rounded sums 0.7e-6 and 1.1e-6).  Of FP32
+// rows O is therefore added to a sum, rounded, every 6 tiles and begun again:
+// in shared memory where Q has gone to tensor memory, else in the workspace, by
+// additions that nothing waits for, each address its own thread's.  (Every 4,
+// 6 and 8 tiles: 0.81, 0.91 and 0.97e-6; 180, 177 and 173 us for 32 x 1024
+// tokens of 8 heads of 64, 165 without.)
 //
 // O follows a row's maximum lazily: probabilities up to 2^4 are let through,
 // so that after the first tiles O is hardly ever touched; they carry 2^11,
@@ -542,7 +545,6 @@ constexpr int kStages = 3;
 constexpr float kLazy = 4.f;
 constexpr float kProbScale = 2048.f;
 constexpr int kSumTiles = 6;     // FP32 rows: tiles whose products O holds at most
-constexpr int kSumChunk = 8;     // the same where chunks bound them
 constexpr int kSumWidth = 64;    // widest rows with sums in shared memory
 
 template <int D, int TERMS>
@@ -603,6 +605,11 @@ __device__ __forceinline__ void tmem_wait(uint32_t (&v)[16]) {
                : "memory");
 }
 
+// *at += {a, b, c, d}, without waiting for it.
+__device__ __forceinline__ void add_f32x4(float4* at, float a, float b, float c, float d) {
+  asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
+
 // The largest of three (NaN only of three NaN).
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -631,7 +638,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     attend_tiles(View c, Batch t, Queries q, Partials part, int blocks_per_seq) {
   constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;
   using S = TileShape<D, TERMS>;
-  constexpr bool SUMS = TERMS == 2 && D <= kSumWidth;
+  constexpr bool SUMS = TERMS == 2, FAR = SUMS && D > kSumWidth;  // sums of O; in the workspace
   extern __shared__ __align__(128) uint8_t smem[];
   // the shuffle makes the warp's number, and what follows from it, uniform
   const int warp = __shfl_sync(kFull, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -667,6 +674,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   // half h takes tiles begin .. begin + count[h]; the first half never more than the second
   const int count1 = end - begin, count0 = max(0, min(end0, end) - begin);
   const size_t slot = ((size_t)z * c.heads + head) * part.chunks + chunk;
+  if (begin >= end && part.chunks > 1) {  // a chunk behind the block's last row
+    for (int r = threadIdx.x; r < kTileRows; r += kTileThreads) part.lse[slot * kTileRows + r] = -INFINITY;
+    return;
+  }
 
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
   uint64_t* kv_full = bars;               // [stage] converters -> products and softmax
@@ -821,6 +832,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       return reinterpret_cast<uint4*>(tile + k / (D / 8) * S::kQTile +
                                       tc::blk16(r8 & (kHalfRows - 1), k % (D / 8) * 8, D) * 2);
     };
+    // the same of the sums
+    auto sum_at = [&](int k) {
+      return FAR ? part.sums + ((slot * 2 + h) * (D / 4) + k) * kHalfRows + (r & (kHalfRows - 1))
+                 : reinterpret_cast<float4*>(staged(r, k));
+    };
+    auto sum_read = [&](int k) { return FAR ? __ldcg(sum_at(k)) : *sum_at(k); };
     // The products of tile j.  A waiter may be a tile behind them or ahead, so
     // each parity of tiles has a barrier: a wait is exact within one phase only.
     auto o_done = [&](int j) { return tc::bar_wait(&o_full[2 * h + (j & 1)], (j >> 1) & 1); };
@@ -893,12 +910,16 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             float o[16];
             tc::tmem_ld16(at_o + c0, o);
             if (SUMS && (close || summed)) {
+              const bool add = FAR && close && summed && !__any_sync(kFull, change != 1.f);
 #pragma unroll
               for (int i = 0; i < 16; i += 4) {
-                float4* sum = reinterpret_cast<float4*>(staged(r, (c0 + i) / 4));
-                float4 v = summed ? *sum : make_float4(0.f, 0.f, 0.f, 0.f);
+                if (add) {
+                  add_f32x4(sum_at((c0 + i) / 4), o[i], o[i + 1], o[i + 2], o[i + 3]);
+                  continue;
+                }
+                float4 v = summed ? sum_read((c0 + i) / 4) : make_float4(0.f, 0.f, 0.f, 0.f);
                 if (close) v = make_float4(v.x + o[i], v.y + o[i + 1], v.z + o[i + 2], v.w + o[i + 3]);
-                *sum = make_float4(v.x * change, v.y * change, v.z * change, v.w * change);
+                *sum_at((c0 + i) / 4) = make_float4(v.x * change, v.y * change, v.z * change, v.w * change);
               }
             }
             if (!close) {  // else this tile's products begin O again
@@ -972,7 +993,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if (SUMS && count > kSumTiles) {
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
-          const float4 v = *reinterpret_cast<const float4*>(staged(r, (c0 + i) / 4));
+          const float4 v = sum_read((c0 + i) / 4);
           o[i] += v.x;
           o[i + 1] += v.y;
           o[i + 2] += v.z;
@@ -981,12 +1002,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[i] = !alive ? NAN : l == 0.f ? 0.f : o[i] * inverse;
-      if (part.chunks > 1) {
-        if (there)
+      if (sizeof(T) == 2 && part.chunks > 1) {
+        if (there) {
 #pragma unroll
           for (int i = 0; i < 16; i += 4)
             *reinterpret_cast<float4*>(po + c0 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-      } else if (wide) {
+        }
+      } else if (wide || part.chunks > 1) {
 #pragma unroll
         for (int i = 0; i < 16; i += VEC) *staged(r, (c0 + i) / VEC) = Element<T>::pack(o + i);
       } else if (there) {
@@ -996,15 +1018,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       __syncwarp();  // tensor memory is read by whole warps
     }
-    if (part.chunks == 1 && wide) {
+    const bool partial = sizeof(T) == 4 && part.chunks > 1;  // FP32 rows are staged as they are
+    if (partial || (part.chunks == 1 && wide)) {
+      const int width = partial ? D : q.head_dim;
 #pragma unroll
       for (int rg = 0; rg < 4; ++rg) {
         const int r8 = r - lane + 8 * rg + sub;
-        T* to = static_cast<T*>(q.out) + (row_at(r8) * q.heads + head_at(r8)) * q.head_dim;
+        T* to = partial ? reinterpret_cast<T*>(part.o + (slot * kTileRows + r8) * D)
+                        : static_cast<T*>(q.out) + (row_at(r8) * q.heads + head_at(r8)) * q.head_dim;
 #pragma unroll
         for (int i = 0; i < D / VEC / 4; ++i) {
           const int k = quarter + 4 * i;
-          if (r8 < u.rows && k * VEC < q.head_dim) *reinterpret_cast<uint4*>(to + k * VEC) = *staged(r8, k);
+          if (r8 < u.rows && k * VEC < width) *reinterpret_cast<uint4*>(to + k * VEC) = *staged(r8, k);
         }
       }
     }
@@ -1254,6 +1279,7 @@ struct Plan {
   int blocks_per_seq;  // row blocks of a sequence
   size_t units;        // sequences times row blocks
   int chunks, chunk_tiles;
+  size_t sums;         // bytes of the sums of O, first in the workspace
   size_t workspace;    // bytes
 };
 
@@ -1279,11 +1305,11 @@ inline Plan make_plan(size_t batch, size_t rows, uint32_t kv_heads, uint32_t gro
   size_t chunks = std::max<size_t>(1, std::min((tiles + 7) / 8, slots / have));
   for (int waves = 2; waves <= 4; ++waves)
     if (tiles * have >= slots * waves * 128) chunks = std::max(chunks, slots * waves / have);
-  if (use_tiles && dtype == MB_F32 && width > (uint32_t)kSumWidth)
-    chunks = std::max(chunks, (tiles + kSumChunk - 1) / kSumChunk);
   p.chunk_tiles = (int)((tiles + chunks - 1) / chunks + kSplitWarps - 1) / kSplitWarps * kSplitWarps;
   p.chunks = (int)((tiles + p.chunk_tiles - 1) / p.chunk_tiles);
-  p.workspace = p.chunks > 1 ? p.units * kv_heads * p.chunks * unit_rows * (width + 1) * sizeof(float) : 0;
+  const size_t rows_in = p.units * kv_heads * p.chunks * unit_rows;
+  p.sums = use_tiles && dtype == MB_F32 && width > (uint32_t)kSumWidth ? rows_in * width * sizeof(float) : 0;
+  p.workspace = p.sums + (p.chunks > 1 ? rows_in * (width + 1) * sizeof(float) : 0);
   return p;
 }
 
@@ -1291,9 +1317,9 @@ template <class T, int D, int ROWS>
 void launch_rows(const View& c, const Batch& t, const Queries& q, const Plan& p, void* workspace, cudaStream_t st) {
   constexpr bool TILES = ROWS == kTileRows;
   const size_t slots = p.units * c.heads * p.chunks;
-  // outputs first: their vectors need the workspace's alignment
-  float* o = static_cast<float*>(workspace);
-  const Partials part{o + slots * ROWS * D, o, p.chunks, p.chunk_tiles};
+  // vectors first: they need the workspace's alignment
+  float* o = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.sums);
+  const Partials part{o + slots * ROWS * D, o, p.chunks, p.chunk_tiles, static_cast<float4*>(workspace)};
   constexpr int bytes = TILES ? TileShape<D, sizeof(T) == 4 ? 2 : 1>::kBytes : SplitSmem<D, TILES ? 8 : ROWS>::kBytes;
   void (*kernel)(View, Batch, Queries, Partials, int);
   if constexpr (TILES) kernel = attend_tiles<T, D>;
