@@ -339,6 +339,18 @@ def test_prompts_of_unequal_lengths(dtype, kv_heads, group, hd, tokens):
     _check(q64, q, cache, values, table, lengths, news, tokens, dtype=dtype)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kv_heads,group,hd,tokens", [(2, 1, 64, 16), (1, 3, 128, 64), (1, 2, 90, 32)])
+def test_one_prompt_among_single_tokens(dtype, kv_heads, group, hd, tokens):
+    """Few rows on average, many in one sequence."""
+    rng = np.random.default_rng(hd + group)
+    news = [1, 0, 1, 70, 1, 1, 2, 1, 1, 1, 1, 1]
+    lengths = [n + 37 * i for i, n in enumerate(news)]
+    cache, values, table = _filled(rng, lengths, kv_heads, hd, tokens)
+    q64, q = _rows(rng, (sum(news), kv_heads * group, hd), dtype)
+    _check(q64, q, cache, values, table, lengths, news, tokens, dtype=dtype)
+
+
 @pytest.mark.parametrize("news,hd,tokens", [([1, 1, 1, 1, 1, 1], 64, 16), ([40, 33, 150, 1, 7, 200], 64, 32),
                                             ([150, 2, 129, 130, 31, 9], 128, 16)])
 def test_left_limits_and_rows_that_see_nothing(news, hd, tokens):
