@@ -36,8 +36,11 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kUnroll = 4;      // 16-byte vectors a thread has in flight
 constexpr int kAgain = 4;       // the same where it looks for top tokens
-constexpr int kRowLanes = 1024; // vocabularies up to here take one warp per row
-constexpr int kFewTop = 6;      // so many top tokens of a row in registers are picked one by one, more are sorted
+constexpr int kRowLanes = 1024; // vocabularies up to here take one warp per row, however few the rows
+// So many top tokens of a row in registers are picked one by one, more are
+// sorted: 4656 x 97 FP32, picked against sorted, 3.6 : 5.3 us for one, 5.4 : 5.4
+// for 5, 6.0 : 5.5 for 6, 11.7 : 5.7 for 20.
+constexpr int kFewTop = 6;
 constexpr unsigned kFull = 0xFFFFFFFFu;
 
 using u64 = unsigned long long;
@@ -228,7 +231,8 @@ __device__ __forceinline__ void finish(const Out& o, size_t row, const T* x, int
 }
 
 // One warp per row, the whole row in registers (R elements a lane): small
-// vocabularies, where a row is less work than a CTA's joining.
+// vocabularies, where a row is less work than a CTA's joining.  Bound by the
+// latency of one row: 4656 x 97 FP32 with 5 top tokens 5.4 us, 0.3 of it bytes.
 template <class T, int R>
 __global__ void __launch_bounds__(kThreads)
     forward_small(const T* __restrict__ logits, size_t stride, size_t rows, int vocab, const int* __restrict__ tokens,
@@ -330,7 +334,8 @@ __device__ __forceinline__ uint32_t remote_u32(const void* p, uint32_t rank) {
 }
 
 // Eight lanes per row, R elements a lane, without top tokens: the smallest
-// vocabularies are all latency, and four rows a warp share it.
+// vocabularies are all latency, and four rows a warp share it.  32768 x 64 FP32:
+// 3.5 us against 7.5 with a warp a row (2.4 TB/s, from L2).
 template <class T, int R>
 __global__ void __launch_bounds__(kThreads)
     forward_narrow(const T* __restrict__ logits, size_t stride, size_t rows, int vocab, const int* __restrict__ tokens,
@@ -378,7 +383,9 @@ __device__ __forceinline__ float vector_max(uint4 raw) {
 // Rows of W warps each: 1 (kWarps rows a CTA), or kWarps with a cluster of
 // CTAs per row, each on a contiguous share of it.  The ragged head and tail
 // around the 16-byte aligned body (odd vocabularies leave rows unaligned) are
-// fewer than 2 VEC elements, one more for the group's first threads.
+// fewer than 2 VEC elements, one more for the group's first threads.  Bound by
+// exponentials and instruction issue in 16 bits, by HBM in FP32: 4096 x 32003
+// without top tokens 53 us (4.9 TB/s) and 84 us (6.2 TB/s), with one 69 and 95.
 template <class T, int W, bool TOP>
 __global__ void __launch_bounds__(kThreads)
     forward_wide(const T* __restrict__ logits, size_t stride, size_t rows, int vocab, const int* __restrict__ tokens,
@@ -607,7 +614,9 @@ __device__ __forceinline__ float element_grad(const RowGrad& r, float x, int j) 
   return r.none ? 0.f : d;
 }
 
-// A group of G threads per row (8, a warp, or the CTA).
+// A group of G threads per row (8, a warp, or the CTA).  One read and one
+// write of the logits, bound by HBM: 4096 x 32003 bfloat16 86 us (6.1 TB/s).
+// Groups of 8 hold the smallest rows: 32768 x 64 FP32 4.0 us, 8.5 with a warp.
 template <class T, int G>
 __global__ void __launch_bounds__(kThreads)
     backward_rows(const T* __restrict__ logits, size_t stride, size_t rows, int vocab, GradIn in,
@@ -656,6 +665,24 @@ __global__ void __launch_bounds__(kThreads)
 
 // CTAs per row: enough rows fill the GPU with one each; few rows are cut into
 // up to 8 shares (the portable cluster size) of at least 4096 elements.
+// Longer vocabularies than kRowLanes take a warp a row too where the rows are
+// many: their joins cost a CTA more than its share of the row.  CTA : warp, us,
+// bfloat16 without and with 20 top tokens: 600 x 2000 4.7 : 3.9, 9.4 : 10.7;
+// 1184 x 2000 6.7 : 4.1, 14.7 : 11.1; 1184 x 4000 7.4 : 5.3, 16.5 : 22.5; 2400 x
+// 4000 12.2 : 8.1, 28.8 : 25.1; 2400 x 8000 15.0 : 12.8, 32.3 : 37.3; 4096 x 8000
+// 22.9 : 16.2, 50.5 : 42.8; 16384 x 16000 124 : 88, 256 : 233.  Up to kRowLanes
+// always: 64 x 500 3.3 : 2.8, 4096 x 1000 14.2 : 5.4.
+inline bool warp_rows(size_t rows, uint32_t vocab) {
+  return vocab <= (uint32_t)kRowLanes || (vocab <= 16384 && rows * 2 >= vocab);
+}
+
+// The gradient has no join, so a CTA loses less: 16384 x 2000 47 : 25 us, 4096 x
+// 4000 12.9 : 11.4 (FP32 21.4 : 20.7); 2400 x 4000 8.5 : 8.9 (FP32 8.9 : 10.8);
+// 4096 x 8000 FP32 42.6 : 48.8; 64 x 4000 2.4 : 5.1.
+inline bool warp_rows_backward(size_t rows, uint32_t vocab) {
+  return vocab <= (uint32_t)kRowLanes || (vocab <= 4096 && rows >= vocab);
+}
+
 inline unsigned row_shares(size_t rows, int vocab) {
   const size_t want = (size_t)sm_count() * 4;
   unsigned n = 1;
@@ -679,7 +706,7 @@ void launch_small(const T* x, size_t stride, size_t rows, uint32_t vocab, const 
 template <class T, bool TOP>
 void launch_wide(const T* x, size_t stride, size_t rows, uint32_t vocab, const int* tokens, uint32_t top, const Out& o,
                  cudaStream_t st) {
-  if (vocab <= (uint32_t)kRowLanes) {
+  if (warp_rows(rows, vocab)) {
     forward_wide<T, 1, TOP><<<(unsigned)((rows + kWarps - 1) / kWarps), kThreads, 0, st>>>(
         x, stride, rows, (int)vocab, tokens, (int)top, o);
     return;
@@ -767,7 +794,7 @@ int mb_op_token_logprobs_backward(const mb_token_logprobs_backward_args* a, void
       T* d = static_cast<T*>(a->dlogits);
       const size_t rows = a->rows;
       const uint32_t vocab = a->vocab;
-      if (vocab <= (uint32_t)kRowLanes) {
+      if (warp_rows_backward(rows, vocab)) {
         // 8 threads where they hold the row in their vectors in flight
         if (vocab * sizeof(T) <= 8 * kUnroll * 16) {
           const unsigned blocks = (unsigned)((rows + kThreads / 8 - 1) / (kThreads / 8));

@@ -224,3 +224,33 @@ def test_refusals():
     r = ops.token_logprobs(x, t, status=status)
     assert int(status.item()) == 2 and torch.isnan(r.logprob[1]) and torch.isfinite(r.logprob[::2]).all()
     assert ops.token_logprobs(x[:0], t[:0], 2).top_index.shape == (0, 2)
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab,top", [(515, 1025, 32), (750, 1499, 0), (1031, 1030, 5), (1100, 2197, 1), (2050, 4097, 20)])
+def test_many_rows_of_longer_vocabularies(rows, vocab, top, dtype, masked):
+    test_forward_and_backward(rows, vocab, top, dtype, masked)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_long_rows_with_ties_and_nan(dtype):
+    """A warp a row: more equal values than its list holds, few kinds, NaN."""
+    torch = _torch()
+    rows, vocab = 1600, 3001
+    rng = np.random.default_rng(11)
+    i = np.arange(vocab)
+    kinds = np.stack([np.zeros(vocab), rng.integers(0, 3, vocab), i * 40.0 / vocab, -i * 40.0 / vocab,
+                      np.where(i == vocab - 1, 1.0, -np.inf), np.full(vocab, -3e38), np.full(vocab, -np.inf),
+                      rng.normal(0, 3, vocab)]).astype(np.float32)
+    x = torch.from_numpy(np.tile(kinds, (rows // 8, 1))).to(getattr(torch, dtype))
+    order = np.argsort(-x.double().numpy(), axis=1, kind="stable")[:, :32]
+    t = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    clean = ops.token_logprobs(x.cuda(), t, 32)
+    assert np.array_equal(clean.top_index.cpu().numpy(), order)
+    x[9, 7] = float("nan")
+    r = ops.token_logprobs(x.cuda(), t, 32)
+    keep = torch.arange(rows) != 9
+    for a, b in zip(r, clean):
+        assert torch.equal(a.cpu()[keep], b.cpu()[keep])
+    assert torch.isnan(r.lse[9]) and r.top_index[9, 0] == 7
