@@ -556,3 +556,26 @@ def test_long_prompts_keep_single_precision():
         # outputs are averages of many values: smaller than them by the effective number of tokens
         shrink = np.sqrt((values[1] ** 2).mean()) / np.sqrt((want ** 2).mean())
         assert rel <= 2 * (2.0 ** -24 * np.sqrt(length) + 2.0 ** -21) * max(1.0, shrink)
+
+
+@pytest.mark.parametrize("dtype,head_dim,tokens", [("bfloat16", 64, 32), ("float16", 90, 16), ("float32", 64, 16)])
+def test_many_pages_in_one_write(dtype, head_dim, tokens):
+    """Pages of 129 to 256 vectors, many of them, ragged; then larger values
+    into the half-filled ones."""
+    rng = np.random.default_rng(head_dim + tokens)
+    heads, batch = 8, 16
+    steps = [rng.integers(0, 431, batch), rng.integers(1, 431, batch)]
+    for news in steps:
+        news[3] = 430
+    final = np.sum(steps, axis=0)
+    table, pages = _table(rng, final, tokens)
+    plain, cache = Plain(pages, heads, tokens, head_dim), ops.new_kv_cache(pages, heads, head_dim, tokens)
+    status = ops.new_status()
+    lengths = np.zeros(batch, dtype=np.int64)
+    for i, news in enumerate(steps):
+        lengths = lengths + news
+        (k64, k), (v64, v) = (_rows(rng, (news.sum(), heads, head_dim), dtype, 2.0 ** (3 * i)) for _ in range(2))
+        plain.write((k64, v64), table, lengths, news)
+        ops.cache_write(cache, k, v, _i32(table), _i32(lengths), _i32(_offsets(news)), max_new=430, status=status)
+        ops.check_status(status)
+        _equal(plain, cache, table, lengths, head_dim)
