@@ -328,6 +328,9 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D, ROWS>::kResident)
   }
   int ev = -126;  // o carries 2^(14 - ev)
 
+  // The first tiles' scales, which lane 0 wrote behind the copies' arrivals, are
+  // there for every lane; those of later tiles by the end of each turn.
+  __syncwarp();
   for (int n = 0; n < mine; ++n) {
     if (issued < mine) {
       if ((issued & 31) == 0) look_up(issued);
