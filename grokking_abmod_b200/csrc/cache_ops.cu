@@ -130,9 +130,10 @@ __global__ void __launch_bounds__(G == 32 ? 128 : G, G == 256 && HELD == 4 ? 4 :
         most[1] = max(most[1], magnitude<T>(raw[1][i]));
       }
   }
-  // before every group's store of a scale below: all its threads have read it
   most[0] = __reduce_max_sync(0xFFFFFFFFu, most[0]);
   most[1] = __reduce_max_sync(0xFFFFFFFFu, most[1]);
+  // The barriers also order all threads' reads of the scales before their store
+  // below; a reduction alone orders no memory.
   if constexpr (G > 32) {
     __shared__ uint2 parts[G / 32];
     if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = make_uint2(most[0], most[1]);
@@ -142,6 +143,8 @@ __global__ void __launch_bounds__(G == 32 ? 128 : G, G == 256 && HELD == 4 ? 4 :
       most[0] = max(most[0], parts[w].x);
       most[1] = max(most[1], parts[w].y);
     }
+  } else {
+    __syncwarp();
   }
   float inverse[2];
   const size_t page_at = c.row(page, head, 0);

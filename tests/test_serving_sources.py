@@ -23,3 +23,11 @@ def test_scales_of_the_first_tiles_are_ordered_before_their_reads():
     assert "__syncwarp();" in prologue[:prologue.index("for (int n = 0; n < mine; ++n)")]
     loop = _between("cache_attention.cu", "attend_split", "for (int n = 0; n < mine; ++n)", "// The four warps' results")
     assert loop.rindex("__syncwarp();") > loop.rindex("load_words<VW>")
+
+
+def test_scales_are_read_by_every_lane_before_one_writes_them():
+    """A page's earlier scales are read by the whole group; its first thread
+    stores the new ones."""
+    text = _between("cache_ops.cu", "write_pages", "before[1] = *scale_at[1];", "*scale_at[which] = scale")
+    wide, narrow = text.index("if constexpr (G > 32)"), text.index("} else {\n    __syncwarp();")
+    assert wide < text.index("__syncthreads();") < narrow
