@@ -369,6 +369,18 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D, ROWS>::kResident)
         for (int e = 0; e < 4; ++e) x[j][e] = acc[e] * (scale * row_factor[e / 2]);
       }
     }
+    // V's exponent: o is kept relative to the largest V scale so far
+    int top = ev;
+    if (sc.z == sc.z) top = max(top, exponent_of(sc.z));
+    if (sc.w == sc.w) top = max(top, exponent_of(sc.w));
+    // V's scales for this lane's rows: 0 where a row sees nothing of the 16
+    // tokens, whose scale may be NaN or far from the seen ones
+    float seen0[NB], seen1[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      seen0[nb] = sc.z;
+      seen1[nb] = sc.w;
+    }
     if (pos < u.lo || pos + kTile - 1 > sure) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -377,11 +389,12 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D, ROWS>::kResident)
           const int at = pos + 8 * j + 2 * tq + (e & 1);
           if (at < u.lo || at > limit[e / 2]) x[j][e] = -INFINITY;
         }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        if (pos + kTile / 2 <= u.lo || max(pos, u.lo) > limit[nb]) seen0[nb] = 0.f;
+        if (pos + kTile <= u.lo || max(pos + kTile / 2, u.lo) > limit[nb]) seen1[nb] = 0.f;
+      }
     }
-    // V's exponent: o is kept relative to the largest V scale so far
-    int top = ev;
-    if (sc.z == sc.z) top = max(top, exponent_of(sc.z));
-    if (sc.w == sc.w) top = max(top, exponent_of(sc.w));
     const float lower = top != ev ? power_of_two(max(ev - top, -126)) : 1.f;
     ev = top;
     float base[NB], change[NB];
@@ -404,13 +417,12 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D, ROWS>::kResident)
         for (int e = 0; e < 4; ++e) o[i][e] *= change[NB == 1 ? 0 : e / 2];
     }
     const float unit = power_of_two(-ev);
-    const float f0 = sc.z * unit * 16384.f, f1 = sc.w * unit * 16384.f;
     uint32_t pf[4][2];  // [8 tokens][operand rows g, g + 8]
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float f = j < 2 ? f0 : f1;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
+        const float f = (j < 2 ? seen0[nb] : seen1[nb]) * unit * 16384.f;
         const float p0 = ex2_ftz(x[j][2 * nb] - base[nb]), p1 = ex2_ftz(x[j][2 * nb + 1] - base[nb]);
         l[nb] += p0 + p1;
         if constexpr (NB == 1) {
@@ -567,7 +579,8 @@ struct TileShape {
   static constexpr int kQueries = kStages * 2 * kOperand;
   static constexpr int kScales = kQueries + 2 * TERMS * kQTile;  // of Q's rows
   static constexpr int kMeta = kScales + kTileRows * 4;
-  static constexpr int kBars = kMeta + kStages * 32;
+  static constexpr int kSpoilt = kMeta + kStages * 32;
+  static constexpr int kBars = kSpoilt + 32;
   static constexpr int kBytes = kBars + 192;
 };
 
@@ -694,6 +707,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drained + 2);
   int* failed = reinterpret_cast<int*>(tmem_at + 1);
   float* meta = reinterpret_cast<float*>(smem + S::kMeta);  // [stage][4 K scales, 4 V scales] of 16 tokens each
+  // meta holds numbers in the place of scales that are NaN, whose product with a
+  // masked token's weight of 0 would reach every row.  A row sees positions from
+  // the first visible one to its own, so it is spoilt if the first such token that
+  // is visible at all is no later than that: [tokens 16 g of the tiles][K, V].
+  int* spoilt = reinterpret_cast<int*>(smem + S::kSpoilt);
+  if (threadIdx.x < 8) spoilt[threadIdx.x] = INT_MAX;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       tc::bar_init(&kv_full[s], kConverters);
@@ -855,8 +874,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       tc::fence_after_sync();
       const float4 ks = *reinterpret_cast<const float4*>(meta + stage * 8);
       const float4 vs = *reinterpret_cast<const float4*>(meta + stage * 8 + 4);
-      // not 0, so that a masked score stays -inf; NaN stays
-      auto positive = [](float f) { return f < 2e-38f ? 2e-38f : f; };
+      // not 0, so that a masked score stays -inf
+      auto positive = [](float f) { return fmaxf(f, 2e-38f); };
       const float fk[4] = {positive(ks.x * factor), positive(ks.y * factor), positive(ks.z * factor),
                            positive(ks.w * factor)};
       const float sv[4] = {vs.x, vs.y, vs.z, vs.w};
@@ -894,8 +913,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       int top = ev;
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        if (sv[g] == sv[g]) top = max(top, exponent_of(sv[g]));
+      for (int g = 0; g < 4; ++g) top = max(top, exponent_of(sv[g]));
       const bool close = SUMS && j > 0 && j % kSumTiles == 0;  // O joins the sums
       if (__any_sync(kFull, close || mx > m + kLazy || top != ev)) {
         const float shrink = ex2_ftz(m - (mx == -INFINITY ? 0.f : mx));
@@ -977,7 +995,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     if (count > 0 && alive) alive = __all_sync(kFull, o_done(count - 1));
     if (!alive) *failed = 1;
     tc::fence_after_sync();
-    const float inverse = l == 0.f ? 0.f : power_of_two(ev) * (1.f / kProbScale) / l;
+    // (what a converter may still write here is behind this half's last position)
+    int bad_k = INT_MAX, bad_v = INT_MAX;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      bad_k = min(bad_k, spoilt[2 * g]);
+      bad_v = min(bad_v, spoilt[2 * g + 1]);
+    }
+    if (bad_k <= limit) l = NAN;
+    const float inverse = bad_v <= limit ? NAN : l == 0.f ? 0.f : power_of_two(ev) * (1.f / kProbScale) / l;
     float lse = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) + log2f(l);
     if (!alive) lse = NAN;
     const size_t row = u.first_row + tok;
@@ -1114,8 +1140,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       store(tile, kq);
       store(tile + S::kOperand, vq);
       if (ct < 4) {
-        meta[stage * 8 + ct] = sk;
-        meta[stage * 8 + 4 + ct] = sv;
+        meta[stage * 8 + ct] = sk == sk ? sk : 1.f;
+        meta[stage * 8 + 4 + ct] = sv == sv ? sv : 0.f;
+        const int group = (begin + j) * kKeys + 16 * ct, at = max(group, u.lo);
+        if (group + 16 > u.lo) {
+          if (sk != sk) spoilt[2 * ct] = min(spoilt[2 * ct], at);
+          if (sv != sv) spoilt[2 * ct + 1] = min(spoilt[2 * ct + 1], at);
+        }
       }
       tc::fence_async_smem();
       tc::bar_arrive(&kv_full[stage]);
