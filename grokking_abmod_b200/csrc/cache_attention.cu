@@ -12,8 +12,10 @@
 // tensor-core instructions with FP32 accumulation and the scales of K and V,
 // powers of two, multiply scores and probabilities without rounding.  q and p
 // enter as FP16 pairs hi + lo (22 bits) after an exact scaling by a power of
-// two: q by its row's largest magnitude, p times 2^14, which keeps the
-// smallest kept part 2^-39 of the row's largest probability.
+// two: q by its row's largest magnitude; p, times its V's scale, by the largest
+// V scale that the row has seen so far, and 2^14 (2^11 in tiles).  So what a
+// weight loses is 2^-22 of it, or 2^-39 (2^-36) of the largest |v| that the row
+// sees, and nothing that it does not see moves that.
 //
 // The split kernel serves rows that share a key head and are few, one tile of
 // 32 tokens after the other, bound by the bytes of the cache.  The tensor
@@ -326,7 +328,9 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D, ROWS>::kResident)
     m[nb] = -INFINITY;
     l[nb] = 0.f;
   }
-  int ev = -126;  // o carries 2^(14 - ev)
+  int ev[NB];  // o carries 2^(14 - ev)
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) ev[nb] = -126;
 
   // The first tiles' scales, which lane 0 wrote behind the copies' arrivals, are
   // there for every lane; those of later tiles by the end of each turn.
@@ -369,10 +373,6 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D, ROWS>::kResident)
         for (int e = 0; e < 4; ++e) x[j][e] = acc[e] * (scale * row_factor[e / 2]);
       }
     }
-    // V's exponent: o is kept relative to the largest V scale so far
-    int top = ev;
-    if (sc.z == sc.z) top = max(top, exponent_of(sc.z));
-    if (sc.w == sc.w) top = max(top, exponent_of(sc.w));
     // V's scales for this lane's rows: 0 where a row sees nothing of the 16
     // tokens, whose scale may be NaN or far from the seen ones
     float seen0[NB], seen1[NB];
@@ -395,11 +395,15 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D, ROWS>::kResident)
         if (pos + kTile <= u.lo || max(pos + kTile / 2, u.lo) > limit[nb]) seen1[nb] = 0.f;
       }
     }
-    const float lower = top != ev ? power_of_two(max(ev - top, -126)) : 1.f;
-    ev = top;
     float base[NB], change[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
+      // V's exponent: o is kept relative to the largest V scale that the row has seen
+      int top = ev[nb];
+      if (seen0[nb] == seen0[nb]) top = max(top, exponent_of(seen0[nb]));
+      if (seen1[nb] == seen1[nb]) top = max(top, exponent_of(seen1[nb]));
+      const float lower = top != ev[nb] ? power_of_two(max(ev[nb] - top, -126)) : 1.f;
+      ev[nb] = top;
       float mx = fmaxf(x[0][2 * nb], x[0][2 * nb + 1]);
 #pragma unroll
       for (int j = 1; j < 4; ++j) mx = fmaxf(mx, fmaxf(x[j][2 * nb], x[j][2 * nb + 1]));
@@ -416,13 +420,12 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D, ROWS>::kResident)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[i][e] *= change[NB == 1 ? 0 : e / 2];
     }
-    const float unit = power_of_two(-ev);
     uint32_t pf[4][2];  // [8 tokens][operand rows g, g + 8]
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
-        const float f = (j < 2 ? seen0[nb] : seen1[nb]) * unit * 16384.f;
+        const float f = (j < 2 ? seen0[nb] : seen1[nb]) * power_of_two(-ev[nb]) * 16384.f;
         const float p0 = ex2_ftz(x[j][2 * nb] - base[nb]), p1 = ex2_ftz(x[j][2 * nb + 1] - base[nb]);
         l[nb] += p0 + p1;
         if constexpr (NB == 1) {
@@ -469,7 +472,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D, ROWS>::kResident)
       float* w = join + (warp * ROWS + 8 * nb + g) * 3;
       w[0] = m[nb];
       w[1] = sum;
-      w[2] = power_of_two(ev);
+      w[2] = power_of_two(ev[nb]);
     }
   }
   __syncwarp();
@@ -878,7 +881,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       auto positive = [](float f) { return fmaxf(f, 2e-38f); };
       const float fk[4] = {positive(ks.x * factor), positive(ks.y * factor), positive(ks.z * factor),
                            positive(ks.w * factor)};
-      const float sv[4] = {vs.x, vs.y, vs.z, vs.w};
+      float sv[4] = {vs.x, vs.y, vs.z, vs.w};
       const int pos = (begin + j) * kKeys;
       if (pos < u.lo || pos + kKeys - 1 > sure) {
         // masked scores become -inf in place; few tiles need it, so the code below does not carry it
@@ -892,6 +895,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           tc::tmem_st16(at_s + c0, x);
         }
         tc::tmem_st_wait();
+        // scales of 16 tokens that the row sees nothing of do not move its O's
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          if (pos + 16 * g + 16 <= u.lo || pos + 16 * g > limit) sv[g] = 0.f;
       }
       // The scores are read twice, for their maximum and for their
       // exponentials: 64 at once spill.
@@ -963,7 +970,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {  // 16 tokens, at most one page
         const float2 f = splat2(positive(page_scales[g] * factor));
-        const float2 v = splat2(page_scales[4 + g] * unit * kProbScale);
+        // finite also where the row does not see the tokens: their weights stay 0
+        const float2 v = splat2(fminf(page_scales[4 + g] * unit * kProbScale, 1e38f));
         uint32_t hi[8], lo[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {

@@ -58,7 +58,7 @@ def _close(got, want, tol, vmax, dtype, keep):
         tol = tol + (2.0 ** -8 if dtype == "bfloat16" else 2.0 ** -11) * np.abs(want) + 2.0 ** -11 * vmax
     over = np.abs(got - want) - tol
     assert np.isfinite(got[keep]).all()
-    assert over[keep].max() <= 0, (over[keep] / tol[keep]).max()
+    assert over[keep].max() <= 0, (over / tol)[keep].max()
 
 
 @pytest.mark.parametrize("which", ["k", "v"])
@@ -113,3 +113,26 @@ def test_rows_in_front_of_a_spoilt_first_page_stay_empty(dtype, group, hd, news,
     blind, spoilt = (seq == 0) & (pos < first[0]), (seq == 0) & (pos >= first[0])
     assert blind.any() and not out[blind].any() and np.isneginf(lse[:, blind]).all()
     assert np.isnan(out[spoilt]).all() and np.isnan(lse[:, spoilt]).all() and np.isfinite(out[seq == 1]).all()
+
+
+@pytest.mark.parametrize("k", [20, 28, 40, 100])
+@pytest.mark.parametrize("tokens", [16, 32, 64])
+@pytest.mark.parametrize("dtype,group,hd,news", FORMS)
+def test_pages_that_a_row_does_not_see_do_not_move_its_precision(dtype, group, hd, news, tokens, k):
+    """V scales 2^k larger behind a row's own position and in front of the
+    first one seen: every row keeps the precision of what it sees."""
+    rng = np.random.default_rng(hd + tokens + k)
+    lengths = [news[0] + 75, news[1] + 133]
+    first = [0, 100]
+    cache, values, table = _filled(rng, lengths, 2, hd, tokens)
+    q64, q = _rows(rng, (sum(news), 2 * group, hd), dtype)
+    late, early = (lengths[0] - 2) // tokens, 100 // tokens - 1
+    for page in (int(table[0, late]), int(table[1, early])):
+        cache.v_scale[page, 1] *= 2.0 ** k
+        values[1, page, 1] *= 2.0 ** k
+    out, _ = ops.cache_attention(q, cache, _i32(table), _i32(lengths), _i32(_offsets(news)), first=_i32(first),
+                                 max_new=max(news), max_tokens=max(lengths))
+    want, tol, vmax = _exact(q64, values, table, lengths, news, first, tokens)
+    # what sees the large page may be past float16's numbers
+    keep = np.broadcast_to(vmax < 6e4 if dtype == "float16" else vmax < np.inf, want.shape)
+    _close(out.double().cpu().numpy(), want, tol, vmax, dtype, keep)
