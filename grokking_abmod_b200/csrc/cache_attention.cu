@@ -176,6 +176,27 @@ __device__ __forceinline__ void refuse_rows(const Batch& t, const Queries& q, in
   }
 }
 
+// Rows in front of the first sequence's and behind the last one's, as of a batch
+// padded to a fixed size, see nothing: 0 and -inf (NaN where that sequence's
+// numbers do not fit).  The CTAs of those two sequences share them, this one the
+// `part`-th of `parts`.
+template <class T>
+__device__ __forceinline__ void unowned_rows(const Batch& t, const Queries& q, int head, const Unit& u, unsigned part,
+                                             unsigned parts, int threads) {
+  const bool first = u.b == 0 && u.first_row > 0, last = u.b == t.count - 1 && u.first_row + u.fresh < t.rows;
+  if (!first && !last) return;
+  const size_t end = u.first_row + u.fresh, before = first ? u.first_row : 0;
+  const size_t count = (before + (last ? t.rows - end : 0)) * q.group;
+#pragma unroll 1
+  for (size_t r = part; r < count; r += parts) {
+    const size_t at = r / q.group, row = at < before ? at : end + at - before;
+    const int a = head * q.group + (int)(r % q.group);
+    T* out = static_cast<T*>(q.out) + (row * q.heads + a) * q.head_dim;
+    for (int ch = threadIdx.x; ch < q.head_dim; ch += threads) out[ch] = Element<T>::from(u.bad ? NAN : 0.f);
+    if (threadIdx.x == 0 && q.lse) q.lse[(size_t)a * t.rows + row] = u.bad ? NAN : -INFINITY;
+  }
+}
+
 template <class T, int D, int ROWS>
 __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D, ROWS>::kResident)
     attend_split(View c, Batch t, Queries q, Partials part, int blocks_per_seq) {
@@ -193,6 +214,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D, ROWS>::kResident)
   const Unit u = unit_of<ROWS>(c, t, q, z, blocks_per_seq);
   const bool last_block = z % blocks_per_seq == blocks_per_seq - 1;
 
+  unowned_rows<T>(t, q, head, u, z % blocks_per_seq * part.chunks + chunk, blocks_per_seq * part.chunks, kSplitThreads);
   if (u.bad) {
     if (chunk == 0 && z % blocks_per_seq == 0) {
       refuse_rows<T>(t, q, head, u, 0, kSplitThreads);
@@ -667,6 +689,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const int block = blockIdx.x / part.chunks;
   const int z = block / blocks_per_seq * blocks_per_seq + (blocks_per_seq - 1 - block % blocks_per_seq);
   const Unit u = unit_of<kTileRows>(c, t, q, z, blocks_per_seq);
+  unowned_rows<T>(t, q, head, u, z % blocks_per_seq * part.chunks + chunk, blocks_per_seq * part.chunks, kTileThreads);
   if (u.bad) {
     if (chunk == 0 && z % blocks_per_seq == 0) {
       refuse_rows<T>(t, q, head, u, 0, kTileThreads);
@@ -1426,7 +1449,8 @@ int mb_op_cache_attention(const mb_cache_attention_args* a, void* stream) {
                 "the cache's heads must divide q_heads");
     mb::require(std::isfinite(a->scale), "scale must be finite");
     mb::require(max_tokens <= (uint32_t)INT_MAX, "max_tokens must be below 2^31");
-    if (t.rows == 0 || t.count == 0) return;
+    if (t.rows == 0) return;
+    mb::require(t.count > 0, "rows without a sequence");
     mb::require(max_new >= 1, "max_new must be positive where there are rows");
     const void* q = a->q;
     void *out = a->out, *workspace = a->workspace;

@@ -282,7 +282,8 @@ def cache_attention(q, cache: KvCache, table, lengths, offsets=None, *, first=No
     (``first`` None: 0) .. lengths[b] - n + i; query head a reads key head
     a // (q_heads // heads).  out has q's shape and type; lse2
     [q_heads][rows] is the base-2 log-sum-exp of the scaled scores times
-    log2(e).  A row that sees nothing gives 0 and -inf.
+    log2(e).  A row that sees nothing gives 0 and -inf, as do rows of a padded
+    q outside offsets[0] .. offsets[batch].
 
     table, lengths, offsets, max_new as in ``cache_write``; ``scale`` defaults
     to 1 / sqrt(head_dim); ``max_tokens``, about the largest length, is how

@@ -375,11 +375,14 @@ int mb_op_cache_read(const mb_cache_read_args* args, void* stream);
 /* Attention of the new rows over their sequences' cached tokens (written
  * before, the new ones too): row i of n of sequence b sees positions
  * first[b] (NULL: 0) .. lengths[b] - n + i; the others take no part, whatever
- * they hold (a page whose scale is NaN spoils the rows that see a token of
- * it).  Query head a reads key head a / (q_heads / heads).  out [rows][q_heads][head_dim] in the type of q; lse
- * [q_heads][rows] (may be NULL), the base-2 log-sum-exp of the scores scaled
- * by scale * log2(e).  A row that sees nothing gives 0 and -inf; rows of a
- * sequence whose numbers do not fit, and rows past max_new, NaN.  max_tokens:
+ * they hold (a page whose scale is NaN spoils the rows that see a token of it).
+ * Query head a reads key head a / (q_heads / heads).  out
+ * [rows][q_heads][head_dim] in the type of q; lse [q_heads][rows] (may be
+ * NULL), the base-2 log-sum-exp of the scores scaled by scale * log2(e).  A row
+ * that sees nothing, or that belongs to no sequence (before offsets[0], from
+ * offsets[batch] on), gives 0 and -inf; rows of a sequence whose numbers do not
+ * fit, and rows past max_new, NaN.  Rows without any sequence (batch 0) are
+ * refused.  max_tokens:
  * about the largest length, by which long sequences are cut over the GPU (any
  * value is right).  workspace: 16-byte aligned, workspace_bytes at least what
  * mb_op_cache_attention_workspace says for the same sizes on this device. */

@@ -136,3 +136,38 @@ def test_pages_that_a_row_does_not_see_do_not_move_its_precision(dtype, group, h
     # what sees the large page may be past float16's numbers
     keep = np.broadcast_to(vmax < 6e4 if dtype == "float16" else vmax < np.inf, want.shape)
     _close(out.double().cpu().numpy(), want, tol, vmax, dtype, keep)
+
+
+@pytest.mark.parametrize("max_tokens", [None, 100000])
+@pytest.mark.parametrize("dtype,group,hd,news", FORMS)
+def test_rows_that_no_sequence_owns_are_empty(dtype, group, hd, news, max_tokens):
+    """A batch padded to a fixed number of rows, in front and behind; memory
+    that held something else."""
+    torch = _torch()
+    rng = np.random.default_rng(hd)
+    lengths = [n + 40 for n in news] + [17]
+    cache, values, table = _filled(rng, lengths, 2, hd, 32)
+    front, behind = 3, 7 + news[0]
+    rows = front + sum(news) + behind
+    q64, q = _rows(rng, (rows, 2 * group, hd), dtype)
+    offsets = front + np.concatenate([_offsets(news), [sum(news)]])  # the last sequence brings nothing
+    status = ops.new_status()
+    for fill in (float("nan"), 7.0):
+        dirty = [torch.full((rows * 2 * group * hd + i * 1000,), fill, device="cuda") for i in range(4)]
+        del dirty
+        out, lse = ops.cache_attention(q, cache, _i32(table), _i32(lengths), _i32(offsets), max_new=max(news),
+                                       max_tokens=max_tokens, status=status)
+        ops.check_status(status)
+        owned = slice(front, front + sum(news))
+        want, tol, vmax = _exact(q64[owned], values, table, lengths, news + [0], [0, 0, 0], 32)
+        got = out.double().cpu().numpy()
+        _close(got[owned], want, tol, vmax, dtype, np.ones(want.shape, dtype=bool))
+        for outside in (slice(0, front), slice(front + sum(news), rows)):
+            assert not got[outside].any() and torch.isneginf(lse[:, outside]).all()
+    # numbers of the last sequence that do not fit: the rows behind it are not taken for results
+    offsets[-1] -= 1
+    out, lse = ops.cache_attention(q, cache, _i32(table), _i32(lengths), _i32(offsets), max_new=max(news),
+                                   max_tokens=max_tokens, status=status)
+    assert int(status.item()) == 8 and torch.isnan(out[front + sum(news):]).all()
+    with pytest.raises(ops._lib.MeshError):
+        ops.cache_attention(q, cache, _i32(table)[:0], _i32([]), _i32([0]))
