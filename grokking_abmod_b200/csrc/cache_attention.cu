@@ -62,8 +62,18 @@ struct Partials {
   float* o;
   int chunks;       // per unit
   int chunk_tiles;  // tiles of a chunk; the last one takes what is left
-  float4* sums;     // [unit][chunk][half][width / 4][row of the half], of wide FP32 rows in tiles
+  float4* sums;     // [block][head][chunk][half][width / 4][row of the half], of wide FP32 rows in tiles
+  bool packed;      // the blocks of the sums are packed_block's, else the units
 };
+
+// Numbers for the row blocks that hold rows, whatever the sequences' shares: the
+// ceil(n G / 256) blocks of sequence b, which brings n rows from row r of the
+// packed array on, begin at floor(r G / 256) + b and end before the next sequence's
+// begin (floor(x + y) + 1 >= floor(x) + ceil(y)).  Units count a longest prompt
+// for each sequence.
+__host__ __device__ inline size_t packed_block(size_t first_row, int group, int block_rows, size_t b) {
+  return first_row * group / block_rows + b;
+}
 
 template <int D, int ROWS>
 struct SplitSmem {
@@ -882,8 +892,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                                       tc::blk16(r8 & (kHalfRows - 1), k % (D / 8) * 8, D) * 2);
     };
     // the same of the sums
+    const size_t sum_slot =
+        part.packed ? ((packed_block(u.first_row, q.group, kTileRows, u.b) + z % blocks_per_seq) * c.heads + head) *
+                              part.chunks + chunk
+                    : slot;
     auto sum_at = [&](int k) {
-      return FAR ? part.sums + ((slot * 2 + h) * (D / 4) + k) * kHalfRows + (r & (kHalfRows - 1))
+      return FAR ? part.sums + ((sum_slot * 2 + h) * (D / 4) + k) * kHalfRows + (r & (kHalfRows - 1))
                  : reinterpret_cast<float4*>(staged(r, k));
     };
     auto sum_read = [&](int k) { return FAR ? __ldcg(sum_at(k)) : *sum_at(k); };
@@ -1347,6 +1361,7 @@ struct Plan {
   int blocks_per_seq;  // row blocks of a sequence
   size_t units;        // sequences times row blocks
   int chunks, chunk_tiles;
+  size_t packed;       // row blocks that all rows can fill
   size_t sums;         // bytes of the sums of O, first in the workspace
   size_t workspace;    // bytes
 };
@@ -1379,7 +1394,10 @@ inline Plan make_plan(size_t batch, size_t rows, uint32_t kv_heads, uint32_t gro
   p.chunk_tiles = (int)((tiles + chunks - 1) / chunks + kSplitWarps - 1) / kSplitWarps * kSplitWarps;
   p.chunks = (int)((tiles + p.chunk_tiles - 1) / p.chunk_tiles);
   const size_t rows_in = p.units * kv_heads * p.chunks * unit_rows;
-  p.sums = use_tiles && dtype == MB_F32 && width > (uint32_t)kSumWidth ? rows_in * width * sizeof(float) : 0;
+  p.packed = packed_block(rows, (int)group, kTileRows, batch);
+  p.sums = 0;
+  if (use_tiles && dtype == MB_F32 && width > (uint32_t)kSumWidth)
+    p.sums = std::min(p.units, p.packed) * kv_heads * p.chunks * kTileRows * width * sizeof(float);
   p.workspace = p.sums + (p.chunks > 1 ? rows_in * (width + 1) * sizeof(float) : 0);
   return p;
 }
@@ -1390,7 +1408,8 @@ void launch_rows(const View& c, const Batch& t, const Queries& q, const Plan& p,
   const size_t slots = p.units * c.heads * p.chunks;
   // vectors first: they need the workspace's alignment
   float* o = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.sums);
-  const Partials part{o + slots * ROWS * D, o, p.chunks, p.chunk_tiles, static_cast<float4*>(workspace)};
+  const Partials part{o + slots * ROWS * D, o, p.chunks, p.chunk_tiles, static_cast<float4*>(workspace),
+                      p.packed < p.units};
   constexpr int bytes = TILES ? TileShape<D, sizeof(T) == 4 ? 2 : 1>::kBytes : SplitSmem<D, TILES ? 8 : ROWS>::kBytes;
   void (*kernel)(View, Batch, Queries, Partials, int);
   if constexpr (TILES) kernel = attend_tiles<T, D>;

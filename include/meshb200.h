@@ -385,7 +385,10 @@ int mb_op_cache_read(const mb_cache_read_args* args, void* stream);
  * refused.  max_tokens:
  * about the largest length, by which long sequences are cut over the GPU (any
  * value is right).  workspace: 16-byte aligned, workspace_bytes at least what
- * mb_op_cache_attention_workspace says for the same sizes on this device. */
+ * mb_op_cache_attention_workspace says for the same sizes on this device: the
+ * cuts' results, below 200 MB whatever the sizes, and for FP32 heads wider than
+ * 64 with many rows about the rows of q in FP32, 256 more a sequence and key
+ * head. */
 typedef struct mb_cache_attention_args {
   mb_kv_cache cache;
   mb_cache_rows where;

@@ -171,3 +171,37 @@ def test_rows_that_no_sequence_owns_are_empty(dtype, group, hd, news, max_tokens
     assert int(status.item()) == 8 and torch.isnan(out[front + sum(news):]).all()
     with pytest.raises(ops._lib.MeshError):
         ops.cache_attention(q, cache, _i32(table)[:0], _i32([]), _i32([0]))
+
+
+def _workspace(batch, rows, q_heads, kv_heads, hd, max_new, max_tokens):
+    import ctypes
+    n = ctypes.c_size_t()
+    ops.check(ops._lib.load().mb_op_cache_attention_workspace(batch, rows, q_heads, kv_heads, hd, 0, max_new, max_tokens,
+                                                              ctypes.byref(n)))
+    return n.value
+
+
+@pytest.mark.parametrize("batch,rows,q_heads,kv_heads,hd,max_new", [(64, 4096 + 63 * 64, 64, 8, 128, 4096),
+                                                                    (64, 64 * 2048, 8, 8, 128, 64 * 2048),
+                                                                    (128, 131072, 8, 8, 96, 131072), (3, 700, 4, 2, 128, 700),
+                                                                    (1, 100000, 8, 8, 128, 1)])
+def test_workspace_follows_the_rows(batch, rows, q_heads, kv_heads, hd, max_new):
+    """Not the batch times its longest prompt: FP32 sums of the rows there
+    are, and a block a sequence."""
+    assert _workspace(batch, rows, q_heads, kv_heads, hd, max_new, 4096) <= \
+        2 * (rows * q_heads + batch * kv_heads * 256) * hd * 4 + 2e8
+
+
+@pytest.mark.parametrize("hd,group,announced", [(128, 2, None), (96, 3, 700), (128, 1, 100000)])
+def test_ragged_prompts_of_wide_single_precision(hd, group, announced):
+    """One long prompt among short ones, nothing and single tokens: sums in
+    the workspace that begin at any row, with the number of new rows given,
+    not given and too large."""
+    rng = np.random.default_rng(hd)
+    news, tokens = [1, 700, 0, 129, 5, 260, 1, 511], 32
+    lengths = [n + 41 * i for i, n in enumerate(news)]
+    cache, values, table = _filled(rng, lengths, 2, hd, tokens)
+    q64, q = _rows(rng, (sum(news), 2 * group, hd), "float32")
+    out, _ = ops.cache_attention(q, cache, _i32(table), _i32(lengths), _i32(_offsets(news)), max_new=announced)
+    want, tol, vmax = _exact(q64, values, table, lengths, news, [0] * len(news), tokens)
+    _close(out.double().cpu().numpy(), want, tol, vmax, "float32", np.ones(want.shape, dtype=bool))
