@@ -195,8 +195,8 @@ def load(build_if_missing: bool = True):
         return _lib
     if build_if_missing:
         try:
-            from .build import build
-            build()
+            from .build import build_library
+            build_library()
         except Exception:
             if not os.path.exists(LIB_PATH):
                 raise

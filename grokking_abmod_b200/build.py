@@ -1,5 +1,6 @@
 """Builds ``libmeshb200.so`` (sm_100a) in-tree with nvcc, and ``_serving``, the
-Python binding of its serving operators, with the host compiler.
+Python binding of its serving operators, with the host compiler where torch is
+installed.
 
 Usage: ``python -m grokking_abmod_b200.build`` (or ``build()`` from Python).
 The library exports the C ABI declared in ``include/meshb200.h``.
@@ -52,7 +53,20 @@ def _run(cmd, target, verbose):
 
 def build(force: bool = False, verbose: bool = False) -> str:
     """Compiles the library and the binding if any source is newer than them;
-    returns the library's path."""
+    returns the library's path.  Without torch there is no binding, which only
+    ``ops`` of torch tensors needs."""
+    build_library(force, verbose)
+    try:
+        import torch  # noqa: F401
+    except ImportError:
+        print("no torch: the library is built, its Python binding is not", file=sys.stderr)
+        return LIB
+    build_binding(force, verbose)
+    return LIB
+
+
+def build_library(force: bool = False, verbose: bool = False) -> str:
+    """Compiles the library if any source is newer than it; returns its path."""
     if force or _stale():
         cmd = [_nvcc(), "-std=c++17", "-O3", "-lineinfo", "--threads", "0", *ARCH, "-shared", "-Xcompiler",
                "-fPIC,-ffp-contract=off",
@@ -60,7 +74,6 @@ def build(force: bool = False, verbose: bool = False) -> str:
         cmd += [os.path.join(CSRC, s) for s in SOURCES]
         cmd += ["-ldl"]
         _run(cmd, LIB, verbose)
-    build_binding(force, verbose)
     return LIB
 
 

@@ -218,10 +218,12 @@ class TokenLogprobs(NamedTuple):
 @functools.cache
 def _binding():
     """The compiled binding (csrc/binding.cpp), which checks the tensors and
-    calls the library; built with it."""
+    calls the library; built here if it is older than its sources."""
     _lib.load()
     import torch  # noqa: F401  (its libraries first)
 
+    from .build import build_binding
+    build_binding()
     from . import _serving
     return _serving
 
