@@ -58,6 +58,7 @@ class UnsupportedShape(MeshError):
 # name -> (restype, argtypes)
 SIGNATURES = {
     "mb_last_error": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_size_t]),
+    "mb_header_key": (ctypes.c_int, [ctypes.POINTER(ctypes.c_uint64)]),
     "mb_version": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_int)]),
     "mb_device_count": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int)]),
     "mb_gpt_validate": (ctypes.c_int, [ctypes.POINTER(GptConfigC)]),

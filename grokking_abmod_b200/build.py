@@ -6,6 +6,8 @@ Usage: ``python -m grokking_abmod_b200.build`` (or ``build()`` from Python).
 The library exports the C ABI declared in ``include/meshb200.h``.
 """
 
+import glob
+import hashlib
 import os
 import subprocess
 import sys
@@ -15,7 +17,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmeshb200.so")
-BINDING = os.path.join(HERE, "_serving.so")
+HEADER = os.path.join(ROOT, "include", "meshb200.h")
+BINDING_SOURCE = os.path.join(CSRC, "binding.cpp")
 
 SOURCES = ["gpt_model.cu", "mesh_ops.cu", "gemm_tc.cu", "simple_model.cu", "config.cpp", "data.cpp",
            "simple_config.cpp", "checkpoint.cpp", "cache_ops.cu", "cache_attention.cu", "logprobs.cu"]
@@ -38,8 +41,14 @@ def _older(target, deps):
 
 def _stale():
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f != "binding.cpp"]
-    deps.append(os.path.join(ROOT, "include", "meshb200.h"))
+    deps.append(HEADER)
     return _older(LIB, deps)
+
+
+def _header_key():
+    """What library and binding hold of the header that they were built from."""
+    with open(HEADER, "rb") as f:
+        return f"-DMB_HEADER_KEY=0x{hashlib.sha256(f.read()).hexdigest()[:16]}ull"
 
 
 def _run(cmd, target, verbose):
@@ -48,7 +57,7 @@ def _run(cmd, target, verbose):
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"{os.path.basename(cmd[0])} failed:\n" + res.stdout + res.stderr)
-    os.replace(target + ".tmp", target)
+    os.replace(cmd[cmd.index("-o") + 1], target)
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -70,31 +79,45 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
     if force or _stale():
         cmd = [_nvcc(), "-std=c++17", "-O3", "-lineinfo", "--threads", "0", *ARCH, "-shared", "-Xcompiler",
                "-fPIC,-ffp-contract=off",
-               "-I", os.path.join(ROOT, "include"), "-o", LIB + ".tmp"]
+               _header_key(), "-I", os.path.join(ROOT, "include"), "-o", LIB + ".tmp"]
         cmd += [os.path.join(CSRC, s) for s in SOURCES]
         cmd += ["-ldl"]
         _run(cmd, LIB, verbose)
     return LIB
 
 
+def binding_path() -> str:
+    """Where the binding of these sources, this torch and this Python is: its
+    name says what it was built from, so another one is never taken for it."""
+    import torch
+    made = hashlib.sha256(f"{torch.__version__} {sysconfig.get_config_var('SOABI')}".encode())
+    for name in (BINDING_SOURCE, HEADER):
+        with open(name, "rb") as f:
+            made.update(f.read())
+    return os.path.join(HERE, f"_serving_{made.hexdigest()[:16]}.so")
+
+
 def build_binding(force: bool = False, verbose: bool = False) -> str:
-    """Compiles ``_serving.so`` against the installed torch and the library
-    (found beside it at run time) if it is older than its sources."""
-    source, header = os.path.join(CSRC, "binding.cpp"), os.path.join(ROOT, "include", "meshb200.h")
-    if not force and not _older(BINDING, [source, header]):
-        return BINDING
+    """Compiles the binding against the installed torch and the library (found
+    beside it at run time) unless it is there; returns its path."""
+    target = binding_path()
+    if os.path.exists(target) and not force:
+        return target
     import torch
     home = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(_nvcc()))
     cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", _header_key(),
            "-I", os.path.join(ROOT, "include"), "-I", os.path.join(home, "include"),
            "-I", os.path.join(home, "include", "torch", "csrc", "api", "include"),
            "-I", os.path.join(cuda, "include"), "-I", sysconfig.get_paths()["include"],
-           source, "-o", BINDING + ".tmp", "-L", HERE, "-l:libmeshb200.so", "-Wl,-rpath,$ORIGIN",
+           BINDING_SOURCE, "-o", f"{target}.{os.getpid()}.o", "-L", HERE, "-l:libmeshb200.so", "-Wl,-rpath,$ORIGIN",
            "-L", os.path.join(home, "lib"), "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
-    _run(cmd, BINDING, verbose)
-    return BINDING
+    _run(cmd, target, verbose)
+    for old in glob.glob(os.path.join(HERE, "_serving*.so")):
+        if old != target:
+            os.remove(old)
+    return target
 
 
 if __name__ == "__main__":

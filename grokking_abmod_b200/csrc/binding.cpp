@@ -380,4 +380,13 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_serving", nullptr, -1, methods, n
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__serving() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__serving() {
+  uint64_t key = 0;
+  if (mb_header_key(&key) != 0 || key != MB_HEADER_KEY) {
+    PyErr_SetString(PyExc_ImportError,
+                    "the library was built from another header (meshb200.h) than its Python binding: build both "
+                    "(python -m grokking_abmod_b200.build)");
+    return nullptr;
+  }
+  return PyModule_Create(&module);
+}

@@ -1097,6 +1097,17 @@ int mb_version(int* major, int* minor) {
   });
 }
 
+#ifndef MB_HEADER_KEY
+#define MB_HEADER_KEY 0
+#endif
+
+int mb_header_key(uint64_t* key) {
+  return guarded([&] {
+    need(key, "key");
+    *key = MB_HEADER_KEY;
+  });
+}
+
 int mb_device_count(int* count) {
   return guarded([&] {
     need(count, "count");

@@ -218,14 +218,17 @@ class TokenLogprobs(NamedTuple):
 @functools.cache
 def _binding():
     """The compiled binding (csrc/binding.cpp), which checks the tensors and
-    calls the library; built here if it is older than its sources."""
+    calls the library; built here unless that of these sources and this torch
+    is there."""
+    import importlib.util
     _lib.load()
     import torch  # noqa: F401  (its libraries first)
 
     from .build import build_binding
-    build_binding()
-    from . import _serving
-    return _serving
+    spec = importlib.util.spec_from_file_location(__package__ + "._serving", build_binding())
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
 
 
 def new_kv_cache(pages: int, heads: int, head_dim: int, page_tokens: int = 32, device="cuda") -> KvCache:

@@ -76,6 +76,9 @@ int mb_last_error(char* buf, size_t len);
 
 /* Library / device queries. */
 int mb_version(int* major, int* minor);
+/* A number of this header's text, set by the build (0 without it): a caller that
+ * was compiled with the same number passes the structures the library takes. */
+int mb_header_key(uint64_t* key);
 int mb_device_count(int* count);
 
 /* ---- configuration and seeded initialisation (host only, no GPU) ---- */

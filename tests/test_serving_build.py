@@ -58,3 +58,21 @@ def test_a_binding_that_does_not_build_is_an_error(copy):
     # the library needs no binding
     r = _run(copy, "from grokking_abmod_b200 import _lib; _lib.load().mb_version", CXX="/bin/false")
     assert r.returncode == 0, r.stderr
+
+
+def test_a_binding_of_another_torch_is_not_used(copy):
+    r = _run(copy, "import torch; torch.__version__ = '2.0.0'\n" + BINDING, CXX="/bin/false")
+    assert r.returncode != 0 and "false failed" in r.stderr, r.stdout + r.stderr
+
+
+@pytest.mark.slow
+def test_a_binding_does_not_meet_a_library_of_another_header(copy):
+    """A library that stayed older while the binding was built: refused when
+    it is loaded, before any argument structure is passed."""
+    with open(copy / "include" / "meshb200.h", "a") as f:
+        f.write("/* newer */\n")
+    library = copy / "grokking_abmod_b200" / "libmeshb200.so"
+    later = os.path.getmtime(copy / "include" / "meshb200.h") + 10
+    os.utime(library, (later, later))
+    r = _run(copy, BINDING)
+    assert r.returncode != 0 and "ImportError" in r.stderr and "header" in r.stderr, r.stdout + r.stderr
