@@ -84,12 +84,20 @@ class CachedGpt:
             x = x + ops.mesh_forward(ops.rmsnorm_forward(x)[0], wf, conn)
         return ops.rmsnorm_forward(x)[0] @ self.embeddings.t()
 
+    def _followed(self, tokens):
+        """Checks that every sequence brings a token for the next one to follow."""
+        if len(tokens) != self.sequences or not all(len(t) for t in tokens):
+            raise ValueError("a list of at least one token for each sequence")
+
     def generate(self, tokens, steps: int, top: int = 1):
-        """Extends the sequences by ``tokens``, then by their most likely token
-        ``steps`` times.  Returns [(TokenLogprobs of the chosen tokens, with
+        """Extends each sequence by ``tokens[b]`` (one token at least) and
+        chooses its most likely token, which extends it for the next of
+        ``steps`` choices.  Returns [(TokenLogprobs of the chosen tokens, with
         the ``top`` alternatives) per step]; the chosen tokens are
-        ``top_index[:, 0]``."""
+        ``top_index[:, 0]``.  The last ones are not part of the sequences yet:
+        pass them in to go on."""
         import torch
+        self._followed(tokens)
         out = []
         for _ in range(steps):
             logits = self.extend(tokens)
@@ -103,8 +111,10 @@ class CachedGpt:
 
     def score(self, tokens, answers, top: int = 0):
         """Log-probabilities, entropies and alternatives of ``answers[b]`` as
-        the token that follows ``tokens[b]``."""
+        the token that follows ``tokens[b]`` (one token at least), by which the
+        sequences are extended."""
         import torch
+        self._followed(tokens)
         logits = self.extend(tokens)
         ends = torch.from_numpy(np.cumsum([len(t) for t in tokens]) - 1).cuda()
         given = torch.from_numpy(np.asarray(answers, dtype=np.int32)).cuda()

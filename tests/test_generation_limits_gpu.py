@@ -1,0 +1,33 @@
+"""What CachedGpt refuses, and that a refusal moves nothing: the sequences go
+on afterwards as if it had not been asked.  Going on means the same operators
+on the same inputs, so results are equal bit for bit."""
+
+import numpy as np
+import pytest
+
+from grokking_abmod_b200 import CachedGpt, GptConfig, MeshGpt, ops
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def model():
+    return MeshGpt(0, GptConfig(vocab_size=17, context=12, width=128, heads=4, layers=2), 7)
+
+
+PROMPTS = [[3, 1, 4], [1, 5]]
+
+
+@pytest.mark.parametrize("tokens", [[[], [1, 2]], [[1, 2], []], [[], []]])
+def test_every_sequence_needs_a_token_to_follow(model, tokens):
+    """An empty list has no row of its own whose logits could be used."""
+    run = CachedGpt(model, 2)
+    run.extend(PROMPTS)
+    with pytest.raises(ValueError):
+        run.score(tokens, [0, 0])
+    with pytest.raises(ValueError):
+        run.generate(tokens, 1)
+    assert run.lengths.tolist() == [3, 2]
+    fresh = CachedGpt(model, 2)
+    fresh.extend(PROMPTS)
+    assert all((a == b).all() for a, b in zip(run.score([[7], [8]], [1, 2], 3), fresh.score([[7], [8]], [1, 2], 3)))
