@@ -66,9 +66,9 @@ class CachedGpt:
         if not flat.size:
             return self.embeddings.new_empty((0, c.vocab_size))
         positions = np.concatenate([np.arange(n, n + m) for n, m in zip(self.lengths, news)])
-        self.lengths += news
+        held = self.lengths + news
         ints = lambda v: torch.from_numpy(np.asarray(v, dtype=np.int32)).cuda()  # noqa: E731
-        lengths, offsets = ints(self.lengths), ints(np.concatenate([[0], np.cumsum(news)]))
+        lengths, offsets = ints(held), ints(np.concatenate([[0], np.cumsum(news)]))
         positions = torch.from_numpy(positions).cuda()
         most = dict(max_new=int(news.max()), status=self.status)
         conn = 0 if c.connectivity == "neighbor" else 1
@@ -79,10 +79,12 @@ class CachedGpt:
             q, k, v = (ops.mesh_forward(n, w, conn) for w in (wq, wk, wv))
             q, k = (self._rotate(ops.rmsnorm_forward(t, c.heads)[0], positions) for t in (q, k))
             ops.cache_write(cache, k, heads(v), self.table, lengths, offsets, **most)
-            y, _ = ops.cache_attention(q, cache, self.table, lengths, offsets, max_tokens=int(self.lengths.max()), **most)
+            y, _ = ops.cache_attention(q, cache, self.table, lengths, offsets, max_tokens=int(held.max()), **most)
             x = x + ops.mesh_forward(ops.xsa_forward(y.flatten(1), v, c.heads), wo, conn)
             x = x + ops.mesh_forward(ops.rmsnorm_forward(x)[0], wf, conn)
-        return ops.rmsnorm_forward(x)[0] @ self.embeddings.t()
+        logits = ops.rmsnorm_forward(x)[0] @ self.embeddings.t()
+        self.lengths = held  # not before: what a failed step wrote past the lengths is written again
+        return logits
 
     def _followed(self, tokens):
         """Checks that every sequence brings a token for the next one to follow."""

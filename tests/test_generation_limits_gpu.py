@@ -31,3 +31,24 @@ def test_every_sequence_needs_a_token_to_follow(model, tokens):
     fresh = CachedGpt(model, 2)
     fresh.extend(PROMPTS)
     assert all((a == b).all() for a, b in zip(run.score([[7], [8]], [1, 2], 3), fresh.score([[7], [8]], [1, 2], 3)))
+
+
+def test_a_step_that_fails_leaves_the_sequences_as_they_were(model, monkeypatch):
+    run, fresh = CachedGpt(model, 2), CachedGpt(model, 2)
+    for r in (run, fresh):
+        r.extend(PROMPTS)
+    attention, calls = ops.cache_attention, []
+
+    def fails(*args, **kw):
+        calls.append(1)
+        if len(calls) == 2:  # the second layer's
+            raise RuntimeError("no memory")
+        return attention(*args, **kw)
+
+    monkeypatch.setattr(ops, "cache_attention", fails)
+    with pytest.raises(RuntimeError):
+        run.extend([[7], [8, 9]])
+    monkeypatch.undo()
+    assert run.lengths.tolist() == [3, 2]
+    assert (run.extend([[7], [8, 9]]) == fresh.extend([[7], [8, 9]])).all()
+    assert run.lengths.tolist() == [4, 4]
