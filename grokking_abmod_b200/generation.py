@@ -55,14 +55,7 @@ class CachedGpt:
         returns the logits [rows][vocab] of the new rows, in order."""
         import torch
         c = self.config
-        news = np.array([len(t) for t in tokens], dtype=np.int64)
-        if len(news) != self.sequences:
-            raise ValueError("one list of tokens for each sequence")
-        if (self.lengths + news > c.context).any():
-            raise ValueError("a sequence would outgrow the model's context")
-        flat = np.concatenate([np.asarray(t, dtype=np.int64) for t in tokens]) if news.sum() else np.zeros(0, np.int64)
-        if ((flat < 0) | (flat >= c.vocab_size)).any():
-            raise ValueError("token ID is outside the vocabulary")
+        news, flat = self._checked(tokens)
         if not flat.size:
             return self.embeddings.new_empty((0, c.vocab_size))
         positions = np.concatenate([np.arange(n, n + m) for n, m in zip(self.lengths, news)])
@@ -86,10 +79,28 @@ class CachedGpt:
         self.lengths = held  # not before: what a failed step wrote past the lengths is written again
         return logits
 
-    def _followed(self, tokens):
-        """Checks that every sequence brings a token for the next one to follow."""
-        if len(tokens) != self.sequences or not all(len(t) for t in tokens):
+    def _checked(self, tokens, more: int = 0):
+        """(number of tokens of each sequence, all of them), if they and
+        ``more`` after them fit."""
+        c = self.config
+        news = np.array([len(t) for t in tokens], dtype=np.int64)
+        if len(news) != self.sequences:
+            raise ValueError("one list of tokens for each sequence")
+        if (self.lengths + news + more > c.context).any():
+            raise ValueError("a sequence would outgrow the model's context")
+        flat = np.concatenate([np.asarray(t, dtype=np.int64) for t in tokens]) if news.sum() else np.zeros(0, np.int64)
+        if ((flat < 0) | (flat >= c.vocab_size)).any():
+            raise ValueError("token ID is outside the vocabulary")
+        return news, flat
+
+    def _followed(self, tokens, top: int, more: int = 0):
+        """Checks, before anything moves, that every sequence brings a token
+        for the next one to follow, that ``more`` fit behind, and ``top``."""
+        news, _ = self._checked(tokens, more)
+        if not news.all():
             raise ValueError("a list of at least one token for each sequence")
+        if not 0 <= top <= min(32, self.config.vocab_size):
+            raise ValueError("top must be in 0..32 and at most the vocabulary")
 
     def generate(self, tokens, steps: int, top: int = 1):
         """Extends each sequence by ``tokens[b]`` (one token at least) and
@@ -99,7 +110,7 @@ class CachedGpt:
         ``top_index[:, 0]``.  The last ones are not part of the sequences yet:
         pass them in to go on."""
         import torch
-        self._followed(tokens)
+        self._followed(tokens, top, steps - 1)
         out = []
         for _ in range(steps):
             logits = self.extend(tokens)
@@ -116,10 +127,13 @@ class CachedGpt:
         the token that follows ``tokens[b]`` (one token at least), by which the
         sequences are extended."""
         import torch
-        self._followed(tokens)
+        self._followed(tokens, top)
+        given = np.asarray(answers, dtype=np.int64)
+        if given.shape != (self.sequences,) or ((given < -1) | (given >= self.config.vocab_size)).any():
+            raise ValueError("one answer for each sequence, inside the vocabulary (or -1: none)")
         logits = self.extend(tokens)
         ends = torch.from_numpy(np.cumsum([len(t) for t in tokens]) - 1).cuda()
-        given = torch.from_numpy(np.asarray(answers, dtype=np.int32)).cuda()
+        given = torch.from_numpy(given.astype(np.int32)).cuda()
         r = ops.token_logprobs(logits[ends], given, top, status=self.status)
         ops.check_status(self.status)
         return r

@@ -52,3 +52,29 @@ def test_a_step_that_fails_leaves_the_sequences_as_they_were(model, monkeypatch)
     assert run.lengths.tolist() == [3, 2]
     assert (run.extend([[7], [8, 9]]) == fresh.extend([[7], [8, 9]])).all()
     assert run.lengths.tolist() == [4, 4]
+
+
+def _moves_nothing(model, asked):
+    run, fresh = CachedGpt(model, 2), CachedGpt(model, 2)
+    for r in (run, fresh):
+        r.extend(PROMPTS)
+    with pytest.raises((ValueError, ops._lib.MeshError)):
+        asked(run)
+    assert run.lengths.tolist() == [3, 2] and int(run.status.item()) == 0
+    assert (run.extend([[7], [8, 9]]) == fresh.extend([[7], [8, 9]])).all()
+
+
+def test_generation_past_the_context_is_refused_before_it_begins(model):
+    """Steps that cannot all be done would be lost with the exception."""
+    _moves_nothing(model, lambda run: run.generate([[7], [8, 9]], 10))  # 3 + 1 + 9 > 12
+    run = CachedGpt(model, 2)
+    run.extend(PROMPTS)
+    assert len(run.generate([[7], [8, 9]], 9)) == 9 and run.lengths.tolist() == [12, 12]
+
+
+@pytest.mark.parametrize("asked", [lambda r: r.score([[7], [8]], [1]), lambda r: r.score([[7], [8]], [1, 17]),
+                                   lambda r: r.score([[7], [8]], [1, -2]), lambda r: r.score([[7], [8]], [1, 2], 18),
+                                   lambda r: r.score([[7], [8]], [1, 2], -1), lambda r: r.generate([[7], [8]], 2, 33),
+                                   lambda r: r.generate([[7], [17]], 2), lambda r: r.generate([[7]], 2)])
+def test_what_cannot_be_answered_is_refused_before_anything_moves(model, asked):
+    _moves_nothing(model, asked)
