@@ -272,7 +272,7 @@ int mb_op_cache_write(const mb_cache_write_args* a, void* stream) {
     const View c = view_of(a->cache, a->head_dim);
     const Batch t = batch_of(a->where, a->max_new);
     const uint32_t max_new = a->max_new;
-    if (t.rows == 0 || max_new == 0 || t.count == 0) return;
+    if (t.rows == 0 || t.count == 0) return;
     mb::need(a->k, "k");
     mb::need(a->v, "v");
     const int page_slots = (int)(((size_t)max_new + c.tokens - 2) / c.tokens + 1);

@@ -205,3 +205,17 @@ def test_ragged_prompts_of_wide_single_precision(hd, group, announced):
     out, _ = ops.cache_attention(q, cache, _i32(table), _i32(lengths), _i32(_offsets(news)), max_new=announced)
     want, tol, vmax = _exact(q64, values, table, lengths, news, [0] * len(news), tokens)
     _close(out.double().cpu().numpy(), want, tol, vmax, "float32", np.ones(want.shape, dtype=bool))
+
+
+def test_rows_that_a_write_did_not_announce_are_reported():
+    """max_new 0 with new rows: not a write of nothing with a clean status."""
+    torch = _torch()
+    cache = ops.new_kv_cache(2, 2, 32, 16)
+    x = torch.ones((20, 2, 32), device="cuda")
+    status = ops.new_status()
+    ops.cache_write(cache, x, x, _i32([[0, 1]]), _i32([20]), _i32([0, 20]), max_new=0, status=status)
+    assert int(status.item()) == 8
+    # no new rows: nothing to report, however many rows stand behind
+    status.zero_()
+    ops.cache_write(cache, x, x, _i32([[0, 1]]), _i32([20]), _i32([0, 0]), max_new=0, status=status)
+    assert int(status.item()) == 0
