@@ -2,7 +2,7 @@
 // entropy and their k most likely tokens, and the gradient of the first two.
 //
 //   m = max_j x_j, d_j = x_j - m, s = sum_j e^d_j
-//   lse = m + ln s, logprob = x_t - lse, H = ln s - (sum_j e^d_j d_j) / s
+//   lse = m + ln s, logprob = d_t - ln s, H = ln s - (sum_j e^d_j d_j) / s
 //   dx_j = g (1[j = t] - p_j) - h p_j (ln p_j + H),  p_j = e^(x_j - lse)
 //
 // H is a sum of nonnegative terms, so nothing cancels where one token takes
@@ -198,17 +198,22 @@ struct Out {
   int* status;
 };
 
+// ln p of a logit x.  x - lse would carry the rounding of lse, as large as that of
+// the logits, where ln p is small.
+__device__ __forceinline__ float log_p(float x, Stats st, float log_s) {
+  return (x - st.m) - log_s;
+}
+
 // A row's statistics; t its token, valid: inside the vocabulary, xt its logit.
-// Returns lse.
+// Returns ln s.
 __device__ __forceinline__ float store_row(const Out& o, size_t row, Stats st, int t, bool valid, float xt) {
   const bool none = st.m == -INFINITY && st.s == 0.f;  // every token masked
   const float log_s = logf(st.s);
-  const float lse = none ? -INFINITY : (st.m == -INFINITY ? st.s : st.m + log_s);
-  o.lse[row] = lse;
+  o.lse[row] = none ? -INFINITY : (st.m == -INFINITY ? st.s : st.m + log_s);
   o.entropy[row] = none ? 0.f : log_s - st.a / st.s * kLn2;
   if (t != -1 && !valid && o.status) atomicOr(o.status, 2);
-  o.logprob[row] = t == -1 ? 0.f : !valid ? NAN : none ? -INFINITY : xt - lse;
-  return lse;
+  o.logprob[row] = t == -1 ? 0.f : !valid ? NAN : none ? -INFINITY : log_p(xt, st, log_s);
+  return log_s;
 }
 
 // Writes a row's results; one warp, with the joined statistics in every lane
@@ -216,16 +221,16 @@ __device__ __forceinline__ float store_row(const Out& o, size_t row, Stats st, i
 template <class T>
 __device__ __forceinline__ void finish(const Out& o, size_t row, const T* x, int vocab, const int* tokens, int top,
                                        Stats st, u64 mine, int lane) {
-  float lse = 0.f;
+  float log_s = 0.f;
   if (lane == 0) {
     const int t = tokens[row];
     const bool valid = (unsigned)t < (unsigned)vocab;
-    lse = store_row(o, row, st, t, valid, valid ? Element<T>::to(x[t]) : 0.f);
+    log_s = store_row(o, row, st, t, valid, valid ? Element<T>::to(x[t]) : 0.f);
   }
-  lse = __shfl_sync(kFull, lse, 0);
+  log_s = __shfl_sync(kFull, log_s, 0);
   if (lane < top) {
     const float v = unordered((uint32_t)(mine >> 32));
-    o.top_logprob[row * top + lane] = v == -INFINITY ? v : v - lse;
+    o.top_logprob[row * top + lane] = v == -INFINITY ? v : log_p(v, st, log_s);
     o.top_index[row * top + lane] = (int)~(uint32_t)mine;
   }
 }
