@@ -375,8 +375,8 @@ __global__ void __launch_bounds__(kSplitThreads, SplitSmem<D, ROWS>::kResident)
     const int s = n % STAGES;
     if (!__all_sync(kFull, tc::bar_wait(&bars[s], (n / STAGES) & 1))) {
       *gave_up = 1;
-      // the copies behind it may still land: none is left when the CTA ends
-      for (int k = n + 1; k < issued; ++k) tc::bar_wait(&bars[k % STAGES], (k / STAGES) & 1);
+      // it and the copies behind it may still land: none is left when the CTA ends
+      for (int k = n; k < issued; ++k) tc::bar_wait(&bars[k % STAGES], (k / STAGES) & 1);
       break;
     }
     const float4 sc = meta[s];

@@ -31,3 +31,9 @@ def test_scales_are_read_by_every_lane_before_one_writes_them():
     text = _between("cache_ops.cu", "write_pages", "before[1] = *scale_at[1];", "*scale_at[which] = scale")
     wide, narrow = text.index("if constexpr (G > 32)"), text.index("} else {\n    __syncwarp();")
     assert wide < text.index("__syncthreads();") < narrow
+
+
+def test_a_copy_whose_wait_ran_out_is_waited_for_again():
+    """With the ones behind it: none may land when the block has ended."""
+    text = _between("cache_attention.cu", "attend_split", "*gave_up = 1;", "break;")
+    assert "for (int k = n; k < issued; ++k) tc::bar_wait(" in text
