@@ -67,6 +67,9 @@ int64_t integer(PyObject* o, int64_t otherwise) {
   return v;
 }
 
+// Elements of the last dimension are adjacent; an empty tensor may say anything.
+bool adjacent(const at::Tensor& t) { return t.numel() == 0 || t.size(-1) <= 1 || t.stride(-1) == 1; }
+
 void on_device(const at::Tensor& t, c10::DeviceIndex device) {
   require(t.is_cuda() && t.get_device() == device, "the operands must be on one CUDA device");
 }
@@ -102,8 +105,7 @@ Place place(PyObject* const* a, int64_t rows) {
   require(ks.scalar_type() == at::kFloat && vs.scalar_type() == at::kFloat && ks.sizes() == scales &&
               vs.sizes() == scales && ks.is_contiguous() && vs.is_contiguous(),
           "cache.k_scale and cache.v_scale must be contiguous float32 tensors [pages][heads]");
-  require(table.scalar_type() == at::kInt && table.dim() == 2 && (table.size(1) <= 1 || table.stride(1) == 1) &&
-              table.stride(0) >= 0,
+  require(table.scalar_type() == at::kInt && table.dim() == 2 && adjacent(table) && table.stride(0) >= 0,
           "table must be an int32 tensor [batch][pages] with adjacent page numbers");
   Place p;
   p.device = k.get_device();
@@ -136,7 +138,7 @@ struct RowView {
 };
 
 RowView rows_of(const at::Tensor& t, const char* name, c10::DeviceIndex device) {
-  if (t.dim() != 3 || (t.size(2) > 1 && t.stride(2) != 1) || t.stride(0) < 0 || t.stride(1) < 0)
+  if (t.dim() != 3 || !adjacent(t) || t.stride(0) < 0 || t.stride(1) < 0)
     throw BadArgument(std::string(name) + " must be [rows][heads][head_dim] with adjacent channels");
   on_device(t, device);
   return RowView{t.data_ptr(), (size_t)t.stride(0), (size_t)t.stride(1)};
@@ -302,7 +304,7 @@ struct Logits {
 
 Logits logits_of(PyObject* o) {
   const at::Tensor& t = tensor(o, "logits");
-  require(t.is_cuda() && t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1) && t.stride(0) >= 0,
+  require(t.is_cuda() && t.dim() == 2 && adjacent(t) && t.stride(0) >= 0,
           "logits must be a CUDA tensor [rows][vocab] with adjacent columns");
   const int64_t rows = t.size(0), vocab = t.size(1);
   return Logits{&t, rows, vocab, (size_t)(rows > 1 ? t.stride(0) : vocab), element_type(t.scalar_type(), "logits"),

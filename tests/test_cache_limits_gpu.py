@@ -219,3 +219,22 @@ def test_rows_that_a_write_did_not_announce_are_reported():
     status.zero_()
     ops.cache_write(cache, x, x, _i32([[0, 1]]), _i32([20]), _i32([0, 0]), max_new=0, status=status)
     assert int(status.item()) == 0
+
+
+def test_empty_tensors_of_any_strides_are_taken():
+    """Empty arrays of NumPy come with strides of 0: nothing to do, not an error."""
+    torch = _torch()
+    cache = ops.new_kv_cache(2, 3, 40, 16)
+    rows = torch.from_numpy(np.random.default_rng(0).normal(0, 1, (0, 3, 40))).float().cuda()
+    assert rows.stride(2) == 0
+    status = ops.new_status()
+    ops.cache_write(cache, rows, rows, _i32([[0, 1]]), _i32([20]), _i32([0, 0]), status=status)
+    out, lse = ops.cache_attention(rows, cache, _i32([[0, 1]]), _i32([20]), _i32([0, 0]), status=status)
+    assert out.shape == (0, 3, 40) and lse.shape == (3, 0)
+    none = torch.from_numpy(np.random.default_rng(0).normal(0, 1, (0, 5))).cuda()
+    r = ops.token_logprobs(none.float(), _i32([]), 2, status=status)
+    assert r.top_index.shape == (0, 2)
+    assert ops.token_logprobs_backward(none.float(), _i32([]), r.lse, r.entropy).shape == (0, 5)
+    k, _ = ops.cache_read(cache, none.int(), _i32([]), 4, head_dim=40, status=status)
+    assert k.shape == (0, 4, 3, 40)
+    ops.check_status(status)
