@@ -747,6 +747,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   // masked token's weight of 0 would reach every row.  A row sees positions from
   // the first visible one to its own, so it is spoilt if the first such token that
   // is visible at all is no later than that: [tokens 16 g of the tiles][K, V].
+  // (Selecting scales by row where the weights are made takes 32 x 1024 FP32 tokens
+  // of 8 heads of 64 from 143.7 to 149 us, this to 144.9.)
   int* spoilt = reinterpret_cast<int*>(smem + S::kSpoilt);
   if (threadIdx.x < 8) spoilt[threadIdx.x] = INT_MAX;
   if (threadIdx.x == 0) {

@@ -67,9 +67,10 @@ __device__ __forceinline__ void store_codes(int8_t* at, uint4 raw, float inverse
 
 // A group of G threads (32: a warp, else the CTA) writes one page of one head,
 // of K and of V.  A thread holds up to HELD 16-byte vectors of each between
-// the reduction and the store; the two tensors' loads go out together, since
-// what a group waits for is mostly the chain length -> page -> rows.  16 x 2011
-// ragged tokens of 8 bfloat16 heads of 96, pages of 64: 29 us, 16 of them bytes.
+// the reduction and the store; the two tensors' loads go out together, since a
+// group begins with the chain length -> page -> rows.  16 x 2011 ragged tokens of
+// 8 bfloat16 heads of 96, pages of 64: 29 us, 16 of them bytes; with 2048 tokens
+// each the issue slots are 76% busy, mostly with magnitudes and codes.
 template <class T, int G, int HELD>
 __global__ void __launch_bounds__(G == 32 ? 128 : G, G == 256 && HELD == 4 ? 4 : 1)
     write_pages(View c, Batch t, Rows<T> k, Rows<T> v, int head_dim, int page_slots, unsigned units, int* status) {

@@ -337,7 +337,9 @@ typedef struct mb_cache_rows {
 /* Writes the new rows of K and V (row r, head h at element r * row_stride +
  * h * head_stride, channels adjacent) as the last tokens of their sequences.
  * Per page and head: scale = the smallest 2^e >= 2^-126 with amax <= 127
- * scale, code = round-half-even(x / scale).  In a page that holds earlier
+ * scale, code = round-half-even(x / scale); what is read back is off by half a
+ * step at most, which may round the very largest numbers up (float16 above 65024
+ * read as float16, FP32 above 1.98 2^127: infinity).  In a page that holds earlier
  * tokens the scale never shrinks; where it grows their codes are rounded to
  * it.  An infinity or NaN makes the page and head's scale NaN until the
  * page's first token is written again.  max_new: at least the largest number
